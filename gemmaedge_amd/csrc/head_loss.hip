@@ -1,0 +1,456 @@
+// Cross entropy over the vocabulary and its gradients without the logits
+// (include/gemmaedge_head.h), on the matrix product of head_gemm.h.
+//
+// Forward: a tile of vocabulary x rows of logits stays in the accumulators; its
+// epilogue leaves, for each row, the tile's largest logit and the sum of
+// exp(l - largest), and the target's logit where the tile has it. A second
+// launch joins a row's tiles into lse and loss.
+//
+// Backward, for a piece of the vocabulary at a time: the logits again, whose
+// epilogue makes dz = g (exp(l - lse) - [target]) (1 - (l / c)^2) and stores it
+// for the piece; dhidden += dz . weights (the piece's sum in parts, each added
+// to its own float32 array, joined at the end in a fixed order); dweight rows
+// of the piece = dz^T . hidden.
+//
+// The vocabulary is the tile's M side: a lane of the accumulators then holds 4
+// logits of one row per 16 x 16 product, and, with the rows of a wave's tile
+// dealt out by epi_row, a contiguous run of the vocabulary: sums over the
+// vocabulary are mostly sums over a lane's own registers, and dz is stored in
+// 16-byte pieces.
+#include <hip/hip_runtime.h>
+
+#include "head_gemm.h"
+#include "head_internal.h"
+
+namespace ge {
+namespace head {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// softcap * tanh(z / softcap). bf16 operands: tanh = 1 - 2 / (exp(2 x) + 1) with
+// the hardware's exp2 and reciprocal, 1e-7 of the cap off at most, far below
+// what the operands' 8 bits leave of z; float32 operands: tanhf.
+struct Softcap {
+    float cap, inv, two;  // cap <= 0: none; two = 2 log2(e) / cap
+    template <bool kFast>
+    __device__ __forceinline__ float apply(float z) const {
+        if (cap <= 0.f) return z;
+        if (!kFast) return cap * tanhf(z * inv);
+        return cap - 2.0f * cap * __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f);
+    }
+};
+
+template <bool kFast>
+struct StatsEpi {
+    Softcap sc;
+    int vocab;   // end of the vocabulary, counted from the product's first row
+    int v0;      // number of the product's first row in the whole vocabulary
+    int rows;
+    const int32_t* targets;
+    float* target_logit;
+    float2* stats;   // [rows][ld]
+    int ld, tile0;
+
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
+                                           int wave, char* lds) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN, kRun = kWm / 4;
+        float2* part = reinterpret_cast<float2*>(lds);  // [kWavesM][kBn]
+        const int run0 = m0 + wm * kWm + (lane >> 4) * kRun;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float l = run0 + i * 4 + q < vocab ? sc.apply<kFast>(acc[i][j][q]) : -__builtin_inff();
+                    acc[i][j][q] = l;
+                    top = fmaxf(top, l);
+                }
+            const int n = n0 + wn * kWn + j * 16 + (lane & 15);
+            int t = n < rows ? targets[n] : -1;
+            t = t >= v0 && t - v0 < vocab ? t - v0 : -1;
+            const int at = t - run0;
+            if (t >= 0 && at >= 0 && at < kRun) {
+#pragma unroll
+                for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (at == i * 4 + q) target_logit[n] = acc[i][j][q];
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // A wave whose rows all lie past the vocabulary has nothing to add.
+            const float ref = top == -__builtin_inff() ? 0.f : top;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum += exp2_fast((acc[i][j][q] - ref) * kLog2e);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane < 16) part[wm * kBn + wn * kWn + j * 16 + lane] = make_float2(top, sum);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < kBn; c += 64 * kWavesM * kWavesN) {
+            const int n = n0 + c;
+            if (n >= rows) continue;
+            float top = part[c].x, sum = part[c].y;
+#pragma unroll
+            for (int i = 1; i < kWavesM; ++i) {
+                const float2 p = part[i * kBn + c];
+                const float m = fmaxf(top, p.x);
+                const float ref = m == -__builtin_inff() ? 0.f : m;
+                sum = sum * exp2_fast((top - ref) * kLog2e) + p.y * exp2_fast((p.x - ref) * kLog2e);
+                top = m;
+            }
+            stats[static_cast<int64_t>(n) * ld + tile0 + place.m] = make_float2(top, sum);
+        }
+    }
+};
+
+// lse and loss of a row from its tiles' statistics: a workgroup per row.
+__global__ __launch_bounds__(256) void join_kernel(const float2* stats, int ld, int tiles, int vocab, const int32_t* targets,
+                                                   const float* target_logit, float* loss, float* lse) {
+    __shared__ float2 red[4];
+    const int64_t r = blockIdx.x;
+    const float2* s = stats + r * ld;
+    float top = -__builtin_inff(), sum = 0.f;
+    auto add = [&](float2 p) {
+        const float m = fmaxf(top, p.x);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        sum = sum * exp2_fast((top - ref) * kLog2e) + p.y * exp2_fast((p.x - ref) * kLog2e);
+        top = m;
+    };
+    for (int i = threadIdx.x; i < tiles; i += 256) add(s[i]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) add(make_float2(__shfl_xor(top, o), __shfl_xor(sum, o)));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 4; ++i) add(red[i]);
+    const float z = top + logf(sum);
+    lse[r] = z;
+    if (loss) {
+        const int t = targets[r];
+        loss[r] = t >= 0 && t < vocab ? z - target_logit[r] : 0.f;
+    }
+}
+
+// hi + mid + lo = x to 24 bits; a non-finite x keeps its value in hi alone.
+__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
+    p[0] = to_bf16(x);
+    const float r = x - to_f32(p[0]);
+    p[1] = to_bf16(r);
+    p[2] = to_bf16(r - to_f32(p[1]));
+}
+
+template <bool kFast, int kPlanes>
+struct GradEpi {
+    Softcap sc;
+    int vocab, v0, rows, vocab_all;
+    const int32_t* targets;
+    const float* lse;
+    const float* grad;
+    uint16_t* out;  // kPlanes x [rows_pad][ld]
+    int64_t ld, plane;
+
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
+                                           int wave, char* lds) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN, kRun = kWm / 4;
+        const int run0 = m0 + wm * kWm + (lane >> 4) * kRun;
+        const float sq = sc.cap > 0.f ? sc.inv : 0.f;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            const int n = n0 + wn * kWn + j * 16 + (lane & 15);
+            int t = n < rows ? targets[n] : -1;
+            const bool live = t >= 0 && t < vocab_all;
+            if (!live) t = -1;
+            const float z = live ? lse[n] : 0.f, g = live ? grad[n] : 0.f;
+            const int at = t - v0 - run0;
+            uint16_t* o = out + static_cast<int64_t>(n) * ld + run0;
+#pragma unroll
+            for (int i = 0; i < kMt; i += 2) {
+                s16x8 pack[kPlanes];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const int e = i * 4 + q;
+                    const float l = sc.apply<kFast>(acc[i + q / 4][j][q & 3]);
+                    float p = exp2_fast((l - z) * kLog2e);
+                    if (at == e) p -= 1.0f;
+                    const float y = l * sq;
+                    float d = p * fmaf(-y, y, 1.0f) * g;
+                    if (!live || run0 + e >= vocab) d = 0.f;
+                    if (kPlanes == 1) {
+                        pack[0][q] = static_cast<short>(to_bf16(d));
+                    } else {
+                        uint16_t s[3];
+                        split3(d, s);
+#pragma unroll
+                        for (int k = 0; k < kPlanes; ++k) pack[k][q] = static_cast<short>(s[k]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<s16x8*>(o + k * plane + i * 4) = pack[k];
+            }
+        }
+    }
+};
+
+// dhidden of a piece and part of it: float32, added to what earlier pieces left.
+struct HiddenEpi {
+    float* out;  // [splits][rows_pad][ld]
+    int64_t ld, split;
+    int dim, rows;
+    bool add;
+
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
+                                           int wave, char* lds) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            const int n = n0 + wn * kWn + j * 16 + (lane & 15);
+            if (n >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) {
+                const int d = m0 + wm * kWm + i * 16 + 4 * (lane >> 4);
+                if (d >= dim) continue;  // ld is a multiple of 4 above dim
+                f32x4* o = reinterpret_cast<f32x4*>(out + place.split * split + n * ld + d);
+                *o = add ? *o + acc[i][j] : acc[i][j];
+            }
+        }
+    }
+};
+
+template <typename T>
+struct WeightEpi {
+    T* out;  // the piece's first row of dweight
+    int64_t ld;
+    int dim, vocab;
+    bool vec;  // rows take 4-element stores
+
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
+                                           int wave, char* lds) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            const int v = n0 + wn * kWn + j * 16 + (lane & 15);
+            if (v >= vocab) continue;
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) {
+                const int d = m0 + wm * kWm + i * 16 + 4 * (lane >> 4);
+                T* o = out + v * ld + d;
+                T q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = from_f32<T>(acc[i][j][e]);
+                if (vec && d + 4 <= dim) {
+                    if constexpr (sizeof(T) == 4)
+                        *reinterpret_cast<f32x4*>(o) = acc[i][j];
+                    else
+                        *reinterpret_cast<uint2*>(o) = make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16,
+                                                                  q[2] | static_cast<uint32_t>(q[3]) << 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < dim) o[e] = q[e];
+                }
+            }
+        }
+    }
+};
+
+// The parts of dhidden in order, rounded once. A workgroup per 256 channels of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int64_t ld, int64_t split, int splits, int dim,
+                                                         T* out, int64_t out_ld) {
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d >= dim) return;
+    const int64_t r = blockIdx.y;
+    float s = 0.f;
+    for (int i = 0; i < splits; ++i) s += parts[i * split + r * ld + d];
+    out[r * out_ld + d] = from_f32<T>(s);
+}
+
+// Rows of T into bf16 planes whose rows are `kpad` long, zeros behind `dim`.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, int dim, int kpad, uint16_t* out, int64_t plane) {
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d >= kpad) return;
+    const int64_t r = blockIdx.y;
+    const int64_t o = r * kpad + d;
+    const T x = d < dim ? in[r * ld + d] : T(0);
+    if constexpr (sizeof(T) == 4) {
+        uint16_t s[3];
+        split3(x, s);
+        for (int k = 0; k < 3; ++k) out[k * plane + o] = s[k];
+    } else {
+        out[o] = x;
+    }
+}
+
+__global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, int64_t ld, int dim) {
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d < dim) p[blockIdx.y * ld + d] = 0;
+}
+
+// Launches over rows on a grid's y, at most 65,535 at a time.
+template <typename F>
+void for_rows(int64_t rows, F launch) {
+    for (int64_t r = 0; r < rows; r += 65535) launch(r, static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535));
+}
+
+template <typename T>
+void pack(const T* in, int64_t ld, int64_t rows, int dim, int64_t kpad, uint16_t* out, int64_t plane, hipStream_t st) {
+    for_rows(rows, [&](int64_t r, unsigned n) {
+        pack_kernel<T><<<dim3(static_cast<unsigned>((kpad + 255) / 256), n), 256, 0, st>>>(in + r * ld, ld, dim, static_cast<int>(kpad),
+                                                                                out + r * kpad, plane);
+    });
+}
+
+template <typename T>
+struct Call {
+    const ge_loss_args& x;
+    const LossPlan& plan;
+    const Buffers& b;
+    hipStream_t st;
+    static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+    static constexpr int kSegments = sizeof(T) == 4 ? kMaxSegments : 1;
+    static constexpr bool kFast = sizeof(T) == 2;
+
+    Operand hidden() const {
+        if (plan.pack_h) {
+            const int64_t plane = x.rows * plan.kpad;
+            pack(static_cast<const T*>(x.hidden), x.hidden_stride, x.rows, x.dim, plan.kpad, b.hpack, plane, st);
+            return Operand{b.hpack, plan.kpad, plane, plane};
+        }
+        const int64_t ld = x.rows > 1 ? x.hidden_stride : x.dim;
+        return Operand{static_cast<const uint16_t*>(x.hidden), ld, (x.rows - 1) * ld + x.dim, 0};
+    }
+    // Rows v0 .. v0 + n of the weights.
+    Operand weights(int v0, int n) const {
+        const int64_t ld = x.vocab > 1 ? x.weight_stride : x.dim;
+        if (plan.pack_w) {
+            const int64_t plane = n * plan.kpad;
+            pack(static_cast<const T*>(x.weight) + v0 * ld, ld, n, x.dim, plan.kpad, b.wpack, plane, st);
+            return Operand{b.wpack, plan.kpad, plane, plane};
+        }
+        return Operand{static_cast<const uint16_t*>(x.weight) + v0 * ld, ld, (n - 1) * ld + x.dim, 0};
+    }
+    Softcap softcap() const {
+        if (!(x.softcap > 0.f)) return Softcap{0.f, 0.f, 0.f};
+        return Softcap{x.softcap, 1.0f / x.softcap, 2.0f * kLog2e / x.softcap};
+    }
+    GemmArgs gemm(const Operand& a, const Operand& bb, int64_t k, int m, int n, int bm, int bn, int splits) const {
+        GemmArgs g{};
+        g.a = a;
+        g.b = bb;
+        g.k = static_cast<int>(k);
+        g.segments = kSegments;
+        g.tiles_m = (m + bm - 1) / bm;
+        g.tiles_n = (n + bn - 1) / bn;
+        const int steps = (g.k + kStepK - 1) / kStepK;
+        g.steps_per_split = (steps + splits - 1) / splits;
+        g.splits = splits;
+        g.group_m = 4;
+        return g;
+    }
+    template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
+    void run(const GemmArgs& g, const Epi& e) const {
+        const unsigned blocks = static_cast<unsigned>(g.tiles_m) * g.tiles_n * g.splits;
+        gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 64 * kWm * kWn, 0, st>>>(g, e);
+    }
+    template <typename Epi>
+    void logits(const Operand& w, const Operand& h, int n, const Epi& e) const {
+        // A packed row's padding is zeros on both sides; a direct row ends at dim.
+        const int64_t k = plan.pack_w && plan.pack_h ? plan.kpad : x.dim;
+        const GemmArgs g = gemm(w, h, k, n, x.rows, plan.tile_m, plan.tile_n, 1);
+        if (plan.small)
+            run<kSmallTileM, kSmallTileN, 4, 1, true, true>(g, e);
+        else
+            run<256, 256, 2, 4, true, true>(g, e);
+    }
+    void forward() const {
+        const Operand h = hidden();
+        const int tiles = (x.vocab + plan.tile_m - 1) / plan.tile_m;
+        for (int v0 = 0; v0 < x.vocab; v0 += plan.pack_piece) {
+            const int n = std::min(plan.pack_piece, x.vocab - v0);
+            StatsEpi<kFast> e{softcap(), n, v0, x.rows, x.targets, b.row, reinterpret_cast<float2*>(b.stats), tiles, v0 / plan.tile_m};
+            logits(weights(v0, n), h, n, e);
+        }
+        join_kernel<<<x.rows, 256, 0, st>>>(reinterpret_cast<const float2*>(b.stats), tiles, tiles, x.vocab, x.targets, b.row, x.loss, x.lse);
+    }
+    void backward() const {
+        T* dw = static_cast<T*>(x.dweight);
+        T* dh = static_cast<T*>(x.dhidden);
+        const int64_t dw_ld = x.vocab > 1 ? x.dweight_stride : x.dim, dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
+        const Operand h = hidden();
+        const int64_t ld = plan.piece, dlp = ld * plan.rows_pad;
+        const int64_t hld = (x.dim + 3) / 4 * 4;
+        const int64_t split = x.rows * hld;
+        int splits = plan.splits;
+        for (int v0 = 0; v0 < x.vocab; v0 += plan.piece) {
+            const int n = std::min(plan.piece, x.vocab - v0);
+            const Operand w = weights(v0, n);
+            GradEpi<kFast, kPlanes> e{softcap(), n, v0, x.rows, x.vocab, x.targets, x.lse, x.grad, b.dlogits, ld, dlp};
+            logits(w, h, n, e);
+            // Rows past the batch read as zeros: they are no rows of the hidden states either.
+            const Operand dz{b.dlogits, ld, x.rows * ld, dlp};
+            if (dh) {
+                GemmArgs g = gemm(w, dz, n, x.dim, x.rows, 256, 256, splits);
+                HiddenEpi he{b.dhidden, hld, split, x.dim, x.rows, v0 > 0};
+                run<256, 256, 2, 4, false, true>(g, he);
+            }
+            if (dw) {
+                GemmArgs g = gemm(h, dz, x.rows, x.dim, n, 256, 256, 1);
+                WeightEpi<T> we{dw + v0 * dw_ld, dw_ld, x.dim, n, false};
+                we.vec = aligned_to(we.out, 4 * sizeof(T)) && (x.vocab <= 1 || dw_ld % 4 == 0);
+                run<256, 256, 2, 4, false, false>(g, we);
+            }
+        }
+        if (dh) {
+            for_rows(x.rows, [&](int64_t r, unsigned n) {
+                hidden_sum_kernel<T><<<dim3((x.dim + 255) / 256, n), 256, 0, st>>>(b.dhidden + r * hld, hld, split, splits, x.dim, dh + r * dh_ld,
+                                                                         dh_ld);
+            });
+        }
+    }
+};
+
+}  // namespace
+
+hipError_t launch_loss(const ge_loss_args& x, int dtype, const LossPlan& plan, const Buffers& b, hipStream_t st) {
+    if (x.rows == 0) return hipSuccess;
+    if (dtype == GE_DTYPE_F32)
+        Call<float>{x, plan, b, st}.forward();
+    else
+        Call<uint16_t>{x, plan, b, st}.forward();
+    return hipGetLastError();
+}
+
+hipError_t launch_loss_backward(const ge_loss_args& x, int dtype, const LossPlan& plan, const Buffers& b, hipStream_t st) {
+    if (x.rows == 0) {  // no rows: the weights' gradient is zero
+        if (x.dweight) {
+            const int64_t ld = (x.vocab > 1 ? x.dweight_stride : x.dim) * elem_size(dtype) / 2;
+            const int dim = x.dim * elem_size(dtype) / 2;
+            for_rows(x.vocab, [&](int64_t r, unsigned n) {
+                fill_zero_kernel<<<dim3((dim + 255) / 256, n), 256, 0, st>>>(static_cast<uint16_t*>(x.dweight) + r * ld, ld, dim);
+            });
+        }
+        return hipGetLastError();
+    }
+    if (dtype == GE_DTYPE_F32)
+        Call<float>{x, plan, b, st}.backward();
+    else
+        Call<uint16_t>{x, plan, b, st}.backward();
+    return hipGetLastError();
+}
+
+}  // namespace head
+}  // namespace ge

@@ -1,0 +1,191 @@
+// Host-side checks and geometry of the head's calls (include/gemmaedge_head.h),
+// kept apart from the HIP launches so that they can be built and run without a
+// device. Nothing here reads device memory.
+#pragma once
+
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/gemmaedge_head.h"
+#include "sampler_validate.h"
+
+namespace ge {
+namespace head {
+
+constexpr int kTileM = 256;       // vocabulary (or channels) of a large tile
+constexpr int kSmallRows = 64;    // batches up to this take the small tiles
+constexpr int kSmallTileM = 128;
+constexpr int kSmallTileN = 32;
+constexpr int kPadK = 64;         // packed planes' rows are padded to this
+constexpr int kNormParts = 512;   // row groups whose weight gradients are summed last
+
+inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+inline int planes_of(int dtype) { return dtype == GE_DTYPE_F32 ? 3 : 1; }
+inline int elem_size(int dtype) { return dtype == GE_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == GE_DTYPE_F32 || dtype == GE_DTYPE_BF16; }
+
+// What a handle was created for and the workspaces' sizes in bytes.
+struct Capacity {
+    int max_rows, max_dim, max_vocab;
+    int dtype;
+    bool train;
+    int64_t stats;    // float2 per row and vocabulary tile
+    int64_t row;      // floats per row: target logits, norm's row sums
+    int64_t hpack;    // hidden states as padded bf16 planes
+    int64_t wpack;    // a piece of the weights as padded bf16 planes
+    int64_t dlogits;  // the logits' gradient of a piece of the vocabulary
+    int64_t dhidden;  // float32 parts of the hidden states' gradient
+    int64_t norm;     // float32 parts of the norm weights' gradients
+};
+
+// Workspace of a handle. Pieces of the vocabulary are as large as fits 256 MB
+// of logits' gradient, the card's last-level cache, where two products read it
+// again; a packed piece of weights likewise takes at most 64 MB a plane.
+inline void size_workspace(Capacity& c) {
+    const int64_t rows = c.max_rows, dim = round_up(c.max_dim, kPadK), vocab = round_up(c.max_vocab, kTileM);
+    const int64_t planes = planes_of(c.dtype), rows_pad = round_up(rows, 256);
+    c.stats = 8 * std::max(rows * (vocab / kTileM), std::min<int64_t>(rows, kSmallRows) * (vocab / kSmallTileM));
+    c.row = 8 * rows;
+    c.hpack = 2 * planes * rows * dim;
+    const int64_t cols = std::min(vocab, std::max<int64_t>(kTileM, ((64LL << 20) / (2 * dim)) / kTileM * kTileM));
+    c.wpack = 2 * planes * cols * dim;
+    c.dlogits = c.dhidden = c.norm = 0;
+    if (!c.train) return;
+    const int64_t per_col = 2 * planes * rows_pad;
+    c.dlogits = std::min(per_col * vocab, std::max<int64_t>(per_col * kTileM, 256LL << 20));
+    const int64_t tiles = (rows_pad / 256) * ((dim + 255) / 256);
+    c.dhidden = 4LL * 256 * 256 * std::max<int64_t>(tiles, 1024);
+    c.norm = 4LL * 2 * kNormParts * c.max_dim;
+}
+
+inline int check_create(int max_rows, int max_dim, int max_vocab, int dtype, char* msg, size_t n) {
+    if (max_rows < 1 || max_dim < 1 || max_vocab < 1)
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "max_rows=%d max_dim=%d max_vocab=%d", max_rows, max_dim, max_vocab);
+    if (!dtype_ok(dtype)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dtype %d", dtype);
+    if (max_dim > GE_HEAD_MAX_DIM || max_vocab > (1 << 24) || max_rows > (1 << 22))
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "max_rows %d / max_dim %d / max_vocab %d above %d / %d / %d", max_rows,
+                         max_dim, max_vocab, 1 << 22, GE_HEAD_MAX_DIM, 1 << 24);
+    return GE_OK;
+}
+
+inline int check_sizes(const Capacity& c, int rows, int dim, char* msg, size_t n) {
+    if (rows < 0 || dim < 1) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "rows %d, dim %d", rows, dim);
+    if (rows > c.max_rows || dim > c.max_dim)
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "rows %d / dim %d above capacity %d / %d", rows, dim, c.max_rows, c.max_dim);
+    return GE_OK;
+}
+
+// Rows `stride` elements apart of `dim` elements: a single row may carry any stride.
+inline bool stride_ok(int64_t stride, int rows, int64_t dim) {
+    return rows <= 1 || (stride >= dim && stride <= (int64_t{1} << 40));
+}
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline int check_norm(const Capacity& c, const ge_norm_args& x, bool backward, char* msg, size_t n) {
+    if (const int rc = check_sizes(c, x.rows, x.dim, msg, n)) return rc;
+    if (!dtype_ok(x.weight_dtype)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "weight_dtype %d", x.weight_dtype);
+    if (x.center != 0 && x.center != 1) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "center %d", x.center);
+    if (backward && c.norm == 0)
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "the handle was created without train");
+    if (!backward && !(x.eps >= 0.f)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "eps %g", static_cast<double>(x.eps));
+    const size_t es = elem_size(c.dtype), ws = elem_size(x.weight_dtype);
+    if (x.rows > 0) {
+        if (!x.x || !x.weight || !x.rstd || (x.center && !x.mean))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "x, weight, rstd or (with center) mean is NULL");
+        if (!stride_ok(x.x_stride, x.rows, x.dim))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "x_stride %lld < dim %d", static_cast<long long>(x.x_stride), x.dim);
+        if (!backward && (!x.y || !stride_ok(x.y_stride, x.rows, x.dim)))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "y is NULL or its rows overlap");
+        if (backward && (!x.dy || !stride_ok(x.dy_stride, x.rows, x.dim)))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dy is NULL or its rows overlap");
+        if (backward && x.dx && !stride_ok(x.dx_stride, x.rows, x.dim))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dx rows overlap");
+        if (!aligned_to(x.x, es) || !aligned_to(x.y, es) || !aligned_to(x.dy, es) || !aligned_to(x.dx, es) ||
+            !aligned_to(x.mean, 4) || !aligned_to(x.rstd, 4))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a tensor is not aligned to its elements");
+    }
+    if (!aligned_to(x.weight, ws) || !aligned_to(x.bias, ws) || !aligned_to(x.dweight, ws) || !aligned_to(x.dbias, ws))
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a weight is not aligned to its elements");
+    return GE_OK;
+}
+
+// How a loss call runs.
+struct LossPlan {
+    bool pack_h, pack_w;  // operands copied into padded bf16 planes first
+    int planes;           // 1 or 3
+    int64_t kpad;         // packed planes' row length
+    int small;            // small tiles (few rows)
+    int tile_m, tile_n;   // of the logits' product
+    int rows_pad;         // rows of the logits' gradient
+    int piece;            // vocabulary per piece of the backward (a multiple of kTileM)
+    int pack_piece;       // vocabulary per packed piece of the forward
+    int splits;           // parts of the vocabulary's sum in dhidden
+};
+
+inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, LossPlan& plan, char* msg, size_t n) {
+    if (const int rc = check_sizes(c, x.rows, x.dim, msg, n)) return rc;
+    if (x.vocab < 1) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "empty vocabulary");
+    if (x.vocab > c.max_vocab)
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "vocab %d above capacity %d", x.vocab, c.max_vocab);
+    if (backward && c.dlogits == 0) return plan_fail(msg, n, GE_ERR_CAPACITY, "the handle was created without train");
+    if (!(std::fabs(x.softcap) <= 3.0e38f)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "softcap is not finite");
+    const size_t es = elem_size(c.dtype);
+    if (x.rows > 0) {
+        if (!x.hidden || !x.weight || !x.targets || !x.lse)
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "hidden, weight, targets or lse is NULL");
+        if (!stride_ok(x.hidden_stride, x.rows, x.dim) || !stride_ok(x.weight_stride, x.vocab, x.dim))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "hidden_stride %lld or weight_stride %lld < dim %d",
+                             static_cast<long long>(x.hidden_stride), static_cast<long long>(x.weight_stride), x.dim);
+        if (backward && !x.grad) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "grad is NULL");
+        if (!aligned_to(x.targets, 4) || !aligned_to(x.loss, 4) || !aligned_to(x.lse, 4) || !aligned_to(x.grad, 4))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a tensor is not aligned to its elements");
+    }
+    if (backward) {
+        if (x.dhidden && !stride_ok(x.dhidden_stride, x.rows, x.dim))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dhidden rows overlap");
+        if (x.dweight && !stride_ok(x.dweight_stride, x.vocab, x.dim))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dweight rows overlap");
+    }
+    if (!aligned_to(x.hidden, es) || !aligned_to(x.weight, es) || !aligned_to(x.dhidden, es) || !aligned_to(x.dweight, es))
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a tensor is not aligned to its elements");
+
+    plan.planes = planes_of(c.dtype);
+    // Tiles are fetched 16 bytes a lane: other rows are packed first.
+    auto direct = [&](const void* p, int64_t stride, int rows) {
+        return c.dtype == GE_DTYPE_BF16 && aligned_to(p, 16) && (rows <= 1 || stride % 8 == 0) && x.dim % 8 == 0 &&
+               stride <= (1 << 21);
+    };
+    plan.pack_h = !direct(x.hidden, x.hidden_stride, x.rows);
+    plan.pack_w = !direct(x.weight, x.weight_stride, x.vocab);
+    plan.kpad = round_up(x.dim, kPadK);
+    plan.small = x.rows <= kSmallRows;
+    plan.tile_m = plan.small ? kSmallTileM : kTileM;
+    plan.tile_n = plan.small ? kSmallTileN : 256;
+    plan.rows_pad = static_cast<int>(round_up(std::max(x.rows, 1), 256));
+    const int64_t vpad = round_up(x.vocab, kTileM);
+    const int64_t pack_cols = c.wpack / (2 * plan.planes * plan.kpad) / kTileM * kTileM;
+    plan.pack_piece = static_cast<int>(plan.pack_w ? std::min(vpad, pack_cols) : vpad);
+    if (backward) {
+        const int64_t cols = c.dlogits / (2LL * plan.planes * plan.rows_pad) / kTileM * kTileM;
+        plan.piece = static_cast<int>(std::min<int64_t>(std::min<int64_t>(vpad, cols), plan.pack_piece));
+        // Parts of the sum over the piece: about two tiles a compute unit.
+        const int64_t tiles = static_cast<int64_t>(plan.rows_pad / 256) * ((x.dim + 255) / 256);
+        const int64_t steps = plan.piece / 64;
+        const int64_t fit = c.dhidden / (4LL * 256 * 256 * tiles);
+        plan.splits = static_cast<int>(std::max<int64_t>(1, std::min({(511 + tiles) / tiles, steps, fit})));
+    }
+    return GE_OK;
+}
+
+inline int check_adamw_params(const ge_adamw_params& p, char* msg, size_t n) {
+    if (!(p.beta1 >= 0 && p.beta1 < 1 && p.beta2 >= 0 && p.beta2 < 1 && p.eps >= 0) || !std::isfinite(p.lr) ||
+        !std::isfinite(p.eps) || !std::isfinite(p.weight_decay) || std::isnan(p.grad_scale) || p.step < 1)
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "lr %g, betas %g and %g, eps %g, weight_decay %g, grad_scale %g, step %u",
+                         p.lr, p.beta1, p.beta2, p.eps, p.weight_decay, p.grad_scale, p.step);
+    return GE_OK;
+}
+
+}  // namespace head
+}  // namespace ge

@@ -93,6 +93,11 @@ constexpr int64_t kMaxChunkLen = static_cast<int64_t>(ge::kBlock) * ge::kMaxEpt;
 
 }  // namespace
 
+namespace ge {
+// Sets the calling thread's last message (ge_sampler_last_error) for the calls of other sources.
+int report(int code, const char* msg) { return fail(code, "%s", msg); }
+}  // namespace ge
+
 extern "C" {
 
 const char* ge_sampler_last_error(void) { return g_last_error.c_str(); }
