@@ -19,7 +19,8 @@ constexpr int kSmallRows = 64;    // batches up to this take the small tiles
 constexpr int kSmallTileM = 128;
 constexpr int kSmallTileN = 32;
 constexpr int kPadK = 64;         // packed planes' rows are padded to this
-constexpr int kNormParts = 512;   // row groups whose weight gradients are summed last
+constexpr int kNormParts = 512;   // workgroups of the norm's backward pass, whose weight gradients are summed last
+constexpr int kNormBlocks = 1280; // and of the forward pass, at most
 
 inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 inline int planes_of(int dtype) { return dtype == GE_DTYPE_F32 ? 3 : 1; }
