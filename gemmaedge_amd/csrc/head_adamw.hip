@@ -4,10 +4,10 @@
 // of up to 16 bytes a lane at any address (tensors need no alignment beyond
 // their elements'), and a lane's loads are all issued before its first sum.
 //
-// States of 32 bits are bound by memory: 56 million elements in bf16 with float32
-// masters in 288 us (5.5 TB/s). States of 8 bits are bound by the arithmetic of
-// the rounding (a hash, two codes): 738 million elements in bf16 in 2.12 ms
-// (3.5 TB/s).
+// Bound by memory, at 5.2 to 5.5 TB/s: 56 million elements in bf16 with float32
+// masters and states in 297 us, 738 million in bf16 with 8-bit states in 1.42 ms
+// (2.13 ms with loads converted where they are issued: each branch on a type
+// then waits for its own).
 #include <hip/hip_runtime.h>
 
 #include "head_internal.h"
@@ -78,11 +78,11 @@ using Global = __attribute__((address_space(1))) T*;
 template <typename T, int kN>
 using Some = T __attribute__((ext_vector_type(kN), aligned(sizeof(T))));
 
-// `count` (at most kN) elements from element i on, zeros behind them.
-template <int kN, typename T>
+// `count` (at most kN) elements from element i on, zeros behind them; kFull: all kN are there.
+template <bool kFull, int kN, typename T>
 __device__ __forceinline__ void load_some(const void* base, int64_t i, int count, T (&x)[kN]) {
     const Global<const T> p = (Global<const T>)base + i;
-    if (count >= kN) {
+    if (kFull || count >= kN) {
         const Some<T, kN> q = *(Global<const Some<T, kN>>)p;
 #pragma unroll
         for (int j = 0; j < kN; ++j) x[j] = q[j];
@@ -91,10 +91,10 @@ __device__ __forceinline__ void load_some(const void* base, int64_t i, int count
         for (int j = 0; j < kN; ++j) x[j] = j < count ? p[j] : T(0);
     }
 }
-template <int kN, typename T>
+template <bool kFull, int kN, typename T>
 __device__ __forceinline__ void store_some(void* base, int64_t i, int count, const T (&x)[kN]) {
     const Global<T> p = (Global<T>)base + i;
-    if (count >= kN) {
+    if (kFull || count >= kN) {
         Some<T, kN> q;
 #pragma unroll
         for (int j = 0; j < kN; ++j) q[j] = x[j];
@@ -105,27 +105,17 @@ __device__ __forceinline__ void store_some(void* base, int64_t i, int count, con
             if (j < count) p[j] = x[j];
     }
 }
-// The same for elements of either type, as float32.
-template <int kN>
-__device__ __forceinline__ void load_any(const void* base, int dtype, int64_t i, int count, float (&x)[kN]) {
-    if (dtype == GE_DTYPE_F32) {
-        load_some<kN>(base, i, count, x);
-    } else {
-        uint16_t h[kN];
-        load_some<kN>(base, i, count, h);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) x[j] = to_f32(h[j]);
-    }
-}
-template <int kN>
-__device__ __forceinline__ void store_any(void* base, int dtype, int64_t i, int count, const float (&x)[kN]) {
-    if (dtype == GE_DTYPE_F32) {
-        store_some<kN>(base, i, count, x);
+// The parameter, rounded to its type, and its master where there is one.
+template <bool kFull, int kN>
+__device__ __forceinline__ void store_param(const ge_adamw_tensor& t, int64_t i, int count, const float (&x)[kN]) {
+    if (t.master) store_some<kFull>(t.master, i, count, x);
+    if (t.param_dtype == GE_DTYPE_F32) {
+        store_some<kFull>(t.param, i, count, x);
     } else {
         uint16_t h[kN];
 #pragma unroll
         for (int j = 0; j < kN; ++j) h[j] = to_bf16(x[j]);
-        store_some<kN>(base, i, count, h);
+        store_some<kFull>(t.param, i, count, h);
     }
 }
 
@@ -162,71 +152,71 @@ __device__ __forceinline__ void block_scale(uint32_t big_bits, float top, float&
     if (bad) scale = __builtin_bit_cast(float, 0x7fc00000u);
 }
 
+// A chunk's elements. kFull: the tensor does not end in it; P and G: types of the
+// value to update (the master's or the parameter's) and of the gradient. These
+// are constants because a conversion inside a branch would wait for its load
+// there, one tensor after another.
+struct Chunk {
+    const ge_adamw_tensor& t;
+    int64_t first_block;  // of the tensor, in the whole list
+    int32_t chunk;
+};
+
 // States of 32 bits: 4 elements a lane, 4 blocks a wave.
-__global__ __launch_bounds__(256) void adamw32_kernel(const AdamTensor* tensors, const AdamChunk* chunks, AdamCoeff hc,
-                                                      const ge_adamw_params* dp) {
-    const AdamCoeff c = dp ? coefficients(*dp) : hc;
-    const AdamChunk ch = chunks[blockIdx.x];
-    const ge_adamw_tensor t = tensors[ch.tensor].t;
+template <bool kFull, typename P, typename G>
+__device__ __forceinline__ void step32(const AdamCoeff& c, const Chunk& ch) {
+    const ge_adamw_tensor& t = ch.t;
     constexpr int kN = 4, kBlocks = kAdamBlocks / 4;
     const int64_t e0 = static_cast<int64_t>(ch.chunk) * kAdamChunk + threadIdx.x * kN;
-    float p[kBlocks][kN], g[kBlocks][kN], m[kBlocks][kN], v[kBlocks][kN];
+    P p[kBlocks][kN];
+    G g[kBlocks][kN];
+    float m[kBlocks][kN], v[kBlocks][kN];
     int count[kBlocks];
 #pragma unroll
     for (int u = 0; u < kBlocks; ++u) {
         const int64_t i = e0 + u * 256 * kN;
         count[u] = t.n - i >= kN ? kN : t.n > i ? static_cast<int>(t.n - i) : 0;
-        if (t.master)
-            load_some<kN>(t.master, i, count[u], p[u]);
-        else
-            load_any<kN>(t.param, t.param_dtype, i, count[u], p[u]);
-        load_any<kN>(t.grad, t.grad_dtype, i, count[u], g[u]);
-        load_some<kN>(t.m, i, count[u], m[u]);
-        load_some<kN>(t.v, i, count[u], v[u]);
+        load_some<kFull>(t.master ? t.master : t.param, i, count[u], p[u]);
+        load_some<kFull>(t.grad, i, count[u], g[u]);
+        load_some<kFull>(t.m, i, count[u], m[u]);
+        load_some<kFull>(t.v, i, count[u], v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kBlocks; ++u) {
         const int64_t i = e0 + u * 256 * kN;
+        float q[kN];
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
-            moments(c, g[u][j], m[u][j], v[u][j]);
-            p[u][j] = updated<false>(c, m[u][j], v[u][j], p[u][j]);
+            moments(c, to_f32(g[u][j]), m[u][j], v[u][j]);
+            q[j] = updated<false>(c, m[u][j], v[u][j], to_f32(p[u][j]));
         }
-        if (t.master) store_some<kN>(t.master, i, count[u], p[u]);
-        store_any<kN>(t.param, t.param_dtype, i, count[u], p[u]);
-        store_some<kN>(t.m, i, count[u], m[u]);
-        store_some<kN>(t.v, i, count[u], v[u]);
+        store_param<kFull>(t, i, count[u], q);
+        store_some<kFull>(t.m, i, count[u], m[u]);
+        store_some<kFull>(t.v, i, count[u], v[u]);
     }
 }
 
 // States of 8 bits: 8 elements a lane, a block on each half of a wave.
-__global__ __launch_bounds__(256) void adamw8_kernel(const AdamTensor* tensors, const AdamChunk* chunks, AdamCoeff hc,
-                                                     const ge_adamw_params* dp) {
-    const AdamCoeff c = dp ? coefficients(*dp) : hc;
-    const AdamChunk ch = chunks[blockIdx.x];
-    const AdamTensor& at = tensors[ch.tensor];
-    const ge_adamw_tensor t = at.t;
+template <bool kFull, typename P, typename G>
+__device__ __forceinline__ void step8(const AdamCoeff& c, const Chunk& ch) {
+    const ge_adamw_tensor& t = ch.t;
     constexpr int kN = 8, kPasses = kAdamChunk / (256 * kN);
     const int place = (threadIdx.x & 31) * kN;  // of the lane's first element in its block
-    float p[kPasses][kN], g[kPasses][kN], ms[kPasses], vs[kPasses];
-    uint2 qm[kPasses], qv[kPasses];
+    P p[kPasses][kN];
+    G g[kPasses][kN];
+    float ms[kPasses], vs[kPasses];
+    uint8_t qm[kPasses][kN], qv[kPasses][kN];
     int count[kPasses];
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         const int64_t block = static_cast<int64_t>(ch.chunk) * kAdamBlocks + u * 8 + (threadIdx.x >> 5);
         const int64_t i = block * GE_ADAMW_BLOCK + place;
         count[u] = t.n - i >= kN ? kN : t.n > i ? static_cast<int>(t.n - i) : 0;
-        if (t.master)
-            load_some<kN>(t.master, i, count[u], p[u]);
-        else
-            load_any<kN>(t.param, t.param_dtype, i, count[u], p[u]);
-        load_any<kN>(t.grad, t.grad_dtype, i, count[u], g[u]);
-        uint8_t bytes[kN];
-        load_some<kN>(t.m, i, count[u], bytes);
-        __builtin_memcpy(&qm[u], bytes, kN);
-        load_some<kN>(t.v, i, count[u], bytes);
-        __builtin_memcpy(&qv[u], bytes, kN);
-        const bool live = block * GE_ADAMW_BLOCK < t.n;
+        load_some<kFull>(t.master ? t.master : t.param, i, count[u], p[u]);
+        load_some<kFull>(t.grad, i, count[u], g[u]);
+        load_some<kFull>(t.m, i, count[u], qm[u]);
+        load_some<kFull>(t.v, i, count[u], qv[u]);
+        const bool live = kFull || block * GE_ADAMW_BLOCK < t.n;
         ms[u] = live ? ((Global<const float>)t.m_scale)[block] : 0.f;
         vs[u] = live ? ((Global<const float>)t.v_scale)[block] : 0.f;
     }
@@ -234,32 +224,34 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamTensor* tensors, 
     for (int u = 0; u < kPasses; ++u) {
         const int64_t block = static_cast<int64_t>(ch.chunk) * kAdamBlocks + u * 8 + (threadIdx.x >> 5);
         const int64_t i = block * GE_ADAMW_BLOCK + place;
-        float m[kN], v[kN];
+        float m[kN], v[kN], q[kN];
         uint32_t mbig = 0, vbig = 0;
 #pragma unroll
-        for (int j = 0; j < kN; j += 2) {
-            const int wm = static_cast<int>(j < 4 ? qm[u].x : qm[u].y), wv = static_cast<int>(j < 4 ? qv[u].x : qv[u].y);
-            const auto a = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(wm, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wm, false);
-            const auto b = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_bf8(wv, true) : __builtin_amdgcn_cvt_pk_f32_bf8(wv, false);
+        for (int j = 0; j < kN; j += 4) {
+            uint32_t wm, wv;
+            __builtin_memcpy(&wm, qm[u] + j, 4);
+            __builtin_memcpy(&wv, qv[u] + j, 4);
+            const auto a0 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, false), a1 = __builtin_amdgcn_cvt_pk_f32_fp8(wm, true);
+            const auto b0 = __builtin_amdgcn_cvt_pk_f32_bf8(wv, false), b1 = __builtin_amdgcn_cvt_pk_f32_bf8(wv, true);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                m[j + k] = a[k] * ms[u];
-                v[j + k] = b[k] * vs[u];
-                moments(c, g[u][j + k], m[j + k], v[j + k]);
+            for (int k = 0; k < 4; ++k) {
+                const int e = j + k;
+                m[e] = (k < 2 ? a0[k & 1] : a1[k & 1]) * ms[u];
+                v[e] = (k < 2 ? b0[k & 1] : b1[k & 1]) * vs[u];
+                moments(c, to_f32(g[u][e]), m[e], v[e]);
                 // Elements behind the tensor's end are zeros and no largest value.
-                mbig = max(mbig, __builtin_bit_cast(uint32_t, m[j + k]) & 0x7fffffffu);
-                vbig = max(vbig, __builtin_bit_cast(uint32_t, v[j + k]) & 0x7fffffffu);
-                p[u][j + k] = updated<true>(c, m[j + k], v[j + k], p[u][j + k]);
+                mbig = max(mbig, __builtin_bit_cast(uint32_t, m[e]) & 0x7fffffffu);
+                vbig = max(vbig, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+                q[e] = updated<true>(c, m[e], v[e], to_f32(p[u][e]));
             }
         }
-        if (t.master) store_some<kN>(t.master, i, count[u], p[u]);
-        store_any<kN>(t.param, t.param_dtype, i, count[u], p[u]);
+        store_param<kFull>(t, i, count[u], q);
         mbig = half_wave_max(mbig);
         vbig = half_wave_max(vbig);
         float mscale, minv, vscale, vinv;
         block_scale(mbig, 448.f, mscale, minv);
         block_scale(vbig, 57344.f, vscale, vinv);
-        const uint32_t key = mix(mix(static_cast<uint32_t>(at.first_block + block) + c.seed_mul) + c.step_mul) +
+        const uint32_t key = mix(mix(static_cast<uint32_t>(ch.first_block + block) + c.seed_mul) + c.step_mul) +
                              static_cast<uint32_t>(place) * 0x9E3779B9u;
         uint32_t cm[kN], cv[kN];
 #pragma unroll
@@ -281,12 +273,50 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamTensor* tensors, 
             om[j] = static_cast<uint8_t>(cm[j] | (m[j] < 0.f ? 0x80u : 0u));
             ov[j] = static_cast<uint8_t>(cv[j]);
         }
-        store_some<kN>(t.m, i, count[u], om);
-        store_some<kN>(t.v, i, count[u], ov);
+        store_some<kFull>(t.m, i, count[u], om);
+        store_some<kFull>(t.v, i, count[u], ov);
         if (place == 0 && count[u] > 0) {
             ((Global<float>)t.m_scale)[block] = mscale;
             ((Global<float>)t.v_scale)[block] = vscale;
         }
+    }
+}
+
+template <bool k8, bool kFull, typename P, typename G>
+__device__ __forceinline__ void step_chunk(const AdamCoeff& c, const Chunk& ch) {
+    if constexpr (k8)
+        step8<kFull, P, G>(c, ch);
+    else
+        step32<kFull, P, G>(c, ch);
+}
+
+template <bool k8>
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamTensor* tensors, const AdamChunk* chunks, AdamCoeff hc,
+                                                    const ge_adamw_params* dp) {
+    const AdamCoeff c = dp ? coefficients(*dp) : hc;
+    const AdamChunk at = chunks[blockIdx.x];
+    const AdamTensor& a = tensors[at.tensor];
+    const ge_adamw_tensor t = a.t;
+    const Chunk ch{t, a.first_block, at.chunk};
+    const bool pf = t.master || t.param_dtype == GE_DTYPE_F32, gf = t.grad_dtype == GE_DTYPE_F32;
+    if (t.n - static_cast<int64_t>(at.chunk) * kAdamChunk >= kAdamChunk) {
+        if (pf && gf)
+            step_chunk<k8, true, float, float>(c, ch);
+        else if (pf)
+            step_chunk<k8, true, float, uint16_t>(c, ch);
+        else if (gf)
+            step_chunk<k8, true, uint16_t, float>(c, ch);
+        else
+            step_chunk<k8, true, uint16_t, uint16_t>(c, ch);
+    } else {
+        if (pf && gf)
+            step_chunk<k8, false, float, float>(c, ch);
+        else if (pf)
+            step_chunk<k8, false, float, uint16_t>(c, ch);
+        else if (gf)
+            step_chunk<k8, false, uint16_t, float>(c, ch);
+        else
+            step_chunk<k8, false, uint16_t, uint16_t>(c, ch);
     }
 }
 
@@ -297,7 +327,7 @@ hipError_t launch_adamw(const ge_adamw_args& x, int64_t chunks, hipStream_t st) 
     const AdamTensor* t = static_cast<const AdamTensor*>(x.table);
     const AdamChunk* c = reinterpret_cast<const AdamChunk*>(t + x.count);
     const AdamCoeff coeff = x.device_params ? AdamCoeff{} : coefficients(x.params);
-    auto* kernel = x.state_bits == 8 ? adamw8_kernel : adamw32_kernel;
+    auto* kernel = x.state_bits == 8 ? adamw_kernel<true> : adamw_kernel<false>;
     kernel<<<static_cast<unsigned>(chunks), 256, 0, st>>>(t, c, coeff, x.device_params);
     return hipGetLastError();
 }
