@@ -109,6 +109,8 @@ def _dtype(t, what: str) -> int:
 
 def _want(t, what: str, dtype, shape, device) -> None:
     """A tensor of this dtype, shape and device with contiguous last axis (all axes but the first)."""
+    if t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return
     if t.dtype != dtype:
         raise ValueError(f"{what} has dtype {t.dtype}: {dtype} is wanted")
     if tuple(t.shape) != tuple(shape):
@@ -131,12 +133,28 @@ def _on_gpu(t, what: str):
     return t.device
 
 
-def _stream(stream, device):
-    import torch
+class _Stream:
+    """The stream of a call: ``handle`` for the launch, and a context for the
+    outputs it allocates. The current stream, the usual case, needs no switch."""
 
-    if stream is None:
-        return torch.cuda.current_stream(device)
-    return torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    def __init__(self, stream, device):
+        import torch
+
+        self._switch = None
+        if stream is None:
+            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
+        else:
+            stream = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+            self.handle = stream.cuda_stream
+            self._switch = torch.cuda.stream(stream)
+
+    def __enter__(self):
+        if self._switch is not None:
+            self._switch.__enter__()
+
+    def __exit__(self, *exc):
+        if self._switch is not None:
+            self._switch.__exit__(*exc)
 
 
 class Head:
@@ -193,8 +211,8 @@ class Head:
         _want(weight, "weight", weight.dtype, (dim,), self.device)
         if bias is not None:
             _want(bias, "bias", weight.dtype, (dim,), self.device)
-        stream = _stream(stream, self.device)
-        with torch.cuda.stream(stream):
+        stream = _Stream(stream, self.device)
+        with stream:
             if y is None:
                 y = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
             if mean is None and center:
@@ -209,7 +227,7 @@ class Head:
         a.center, a.eps = int(center), eps
         a.weight, a.bias = weight.data_ptr(), S._ptr(bias)
         a.y, a.y_stride, a.mean, a.rstd = y.data_ptr(), _stride(y), S._ptr(mean), rstd.data_ptr()
-        _check(_library().ge_head_norm(self._h, stream.cuda_stream, ctypes.byref(a)))
+        _check(_library().ge_head_norm(self._h, stream.handle, ctypes.byref(a)))
         return y, mean, rstd
 
     def norm_backward(self, grad, x, weight, mean, rstd, bias: bool = False, dx=None, dweight=None, dbias=None,
@@ -227,8 +245,8 @@ class Head:
         _want(rstd, "rstd", torch.float32, (rows,), self.device)
         if mean is not None:
             _want(mean, "mean", torch.float32, (rows,), self.device)
-        stream = _stream(stream, self.device)
-        with torch.cuda.stream(stream):
+        stream = _Stream(stream, self.device)
+        with stream:
             if dx is None and need_input:
                 dx = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
             if dweight is None and need_weight:
@@ -246,7 +264,7 @@ class Head:
         a.weight, a.mean, a.rstd = weight.data_ptr(), S._ptr(mean), rstd.data_ptr()
         a.dy, a.dy_stride, a.dx = grad.data_ptr(), _stride(grad), S._ptr(dx)
         a.dweight, a.dbias = S._ptr(dweight), S._ptr(dbias)
-        _check(_library().ge_head_norm_backward(self._h, stream.cuda_stream, ctypes.byref(a)))
+        _check(_library().ge_head_norm_backward(self._h, stream.handle, ctypes.byref(a)))
         return dx, dweight, dbias
 
     def _loss_args(self, hidden, weight, targets, softcap):
@@ -270,14 +288,14 @@ class Head:
         import torch
 
         a, rows, _, _ = self._loss_args(hidden, weight, targets, softcap)
-        stream = _stream(stream, self.device)
-        with torch.cuda.stream(stream):
+        stream = _Stream(stream, self.device)
+        with stream:
             loss = torch.empty(rows, dtype=torch.float32, device=self.device) if loss is None else loss
             lse = torch.empty(rows, dtype=torch.float32, device=self.device) if lse is None else lse
         _want(loss, "loss", torch.float32, (rows,), self.device)
         _want(lse, "lse", torch.float32, (rows,), self.device)
         a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-        _check(_library().ge_head_loss(self._h, stream.cuda_stream, ctypes.byref(a)))
+        _check(_library().ge_head_loss(self._h, stream.handle, ctypes.byref(a)))
         return loss, lse
 
     def loss_backward(self, grad, hidden, weight, targets, lse, softcap: float = 0.0, dhidden=None, dweight=None,
@@ -290,8 +308,8 @@ class Head:
         a, rows, dim, vocab = self._loss_args(hidden, weight, targets, softcap)
         _want(grad, "grad", torch.float32, (rows,), self.device)
         _want(lse, "lse", torch.float32, (rows,), self.device)
-        stream = _stream(stream, self.device)
-        with torch.cuda.stream(stream):
+        stream = _Stream(stream, self.device)
+        with stream:
             if dhidden is None and need_hidden:
                 dhidden = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
             if dweight is None and need_weight:
@@ -303,7 +321,7 @@ class Head:
             _want(dweight, "dweight", self.dtype, (vocab, dim), self.device)
             a.dweight, a.dweight_stride = dweight.data_ptr(), _stride(dweight)
         a.grad, a.lse = grad.data_ptr(), lse.data_ptr()
-        _check(_library().ge_head_loss_backward(self._h, stream.cuda_stream, ctypes.byref(a)))
+        _check(_library().ge_head_loss_backward(self._h, stream.handle, ctypes.byref(a)))
         return dhidden, dweight
 
 
@@ -371,7 +389,8 @@ class AdamW:
         _check(L.ge_adamw_table_bytes(table, len(params), state_bits, ctypes.byref(size)))
         host = torch.empty((size.value + 7) // 8, dtype=torch.int64)
         _check(L.ge_adamw_table(table, len(params), state_bits, host.data_ptr(), size.value))
-        self._table, self._bytes = host.to(device), size.value
+        self._table = host.to(device)
+        self._args = AdamwArgs(self._table.data_ptr(), size.value, len(params), state_bits)
         self.params, self.grads, self.masters, self.device = params, grads, masters, device
         self.state_bits, self.seed, self.steps = state_bits, seed, 0
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
@@ -394,15 +413,19 @@ class AdamW:
         ``device_params`` (see there) the launch reads those and counts nothing."""
         import torch
 
-        a = AdamwArgs()
-        a.table, a.table_bytes, a.count, a.state_bits = self._table.data_ptr(), self._bytes, len(self.params), self.state_bits
+        a = self._args
         if device_params is None:
             a.params = self._params(self.steps + 1, lr, grad_scale)
+            a.device_params = None
         else:
             _want(device_params, "device_params", torch.uint8, (ctypes.sizeof(AdamwParams),), self.device)
             a.device_params = device_params.data_ptr()
-        stream = _stream(stream, self.device)
-        with torch.cuda.device(self.device):
-            _check(_library().ge_adamw_step(stream.cuda_stream, ctypes.byref(a)))
+        stream = _Stream(stream, self.device)
+        if torch.cuda.current_device() == self.device.index:
+            rc = _library().ge_adamw_step(stream.handle, ctypes.byref(a))
+        else:
+            with torch.cuda.device(self.device):
+                rc = _library().ge_adamw_step(stream.handle, ctypes.byref(a))
+        _check(rc)
         if device_params is None:
             self.steps += 1
