@@ -31,6 +31,12 @@ __device__ __forceinline__ float to_f32(uint16_t x) { return __builtin_bit_cast(
 __device__ __forceinline__ uint16_t to_bf16(float x) {
     return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
 }
+// Two of them, the first in the low half.
+__device__ __forceinline__ uint32_t to_bf16(float x, float y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+}
 template <typename T>
 __device__ __forceinline__ T from_f32(float x);
 template <>

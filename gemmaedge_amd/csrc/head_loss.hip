@@ -30,18 +30,36 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// softcap * tanh(z / softcap). bf16 operands: tanh = 1 - 2 / (exp(2 x) + 1) with
-// the hardware's exp2 and reciprocal, 1e-7 of the cap off at most, far below
+// softcap * tanh(z / softcap). bf16 operands: tanh = 1 - 2 r with r = 1 / (exp(2 x) + 1)
+// of the hardware's exp2 and reciprocal, 3e-7 of the cap off at most, far below
 // what the operands' 8 bits leave of z; float32 operands: tanhf.
 struct Softcap {
     float cap, inv, two;  // cap <= 0: none; two = 2 log2(e) / cap
+    __device__ __forceinline__ float r(float z) const { return __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f); }
     template <bool kFast>
     __device__ __forceinline__ float apply(float z) const {
-        if (cap <= 0.f) return z;
-        if (!kFast) return cap * tanhf(z * inv);
-        return cap - 2.0f * cap * __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f);
+        return kFast ? fmaf(r(z), -2.0f * cap, cap) : cap * tanhf(z * inv);
     }
+    // exp(-2 cap) is a normal number: sums of exp(l - cap) need no largest logit.
+    __device__ __forceinline__ bool bounded() const { return cap > 0.f && cap <= 40.f; }
 };
+
+// Where a row's target lies among a lane's logits of one column of tiles: element
+// 4 i + q is acc[i][.][q], row epi_row(i, 4 * (lane / 16) + q) of the wave's `kWm`. -1: not here.
+template <int kWm>
+__device__ __forceinline__ int target_place(int target, int first_row, int lane) {
+    const int off = target - first_row;
+    return off >= 0 && off < kWm && ((off >> 3) & 3) == (lane >> 4) ? (off >> 5) * 8 + (off & 7) : -1;
+}
+
+// The targets of a lane's columns, counted from the product's first row; -1: no loss or not in its vocabulary.
+template <int kNt>
+__device__ __forceinline__ void load_targets(const int32_t* targets, int n_first, int rows, int v0, int vocab, int (&t)[kNt]) {
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) t[j] = targets[min(n_first + j * 16, rows - 1)];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) t[j] = n_first + j * 16 < rows && t[j] >= v0 && t[j] - v0 < vocab ? t[j] - v0 : -1;
+}
 
 template <bool kFast>
 struct StatsEpi {
@@ -57,40 +75,65 @@ struct StatsEpi {
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
     __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
                                            int wave, char* lds) const {
-        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN, kRun = kWm / 4;
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         float2* part = reinterpret_cast<float2*>(lds);  // [kWavesM][kBn]
-        const int run0 = m0 + wm * kWm + (lane >> 4) * kRun;
+        const int row0 = m0 + wm * kWm;
+        const int n_first = n0 + wn * kWn + (lane & 15);
+        int t[kNt];
+        load_targets(targets, n_first, rows, v0, vocab, t);
+        const bool tail = row0 + kWm > vocab;
+        const bool simple = kFast && sc.bounded() && !tail;
+        if (!simple && sc.cap > 0.f) {
 #pragma unroll
-        for (int j = 0; j < kNt; ++j) {
-            float top = -__builtin_inff();
+            for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                for (int j = 0; j < kNt; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j][q] = sc.apply<kFast>(acc[i][j][q]);
+        }
+        if (tail) {
 #pragma unroll
             for (int i = 0; i < kMt; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float l = run0 + i * 4 + q < vocab ? sc.apply<kFast>(acc[i][j][q]) : -__builtin_inff();
-                    acc[i][j][q] = l;
-                    top = fmaxf(top, l);
+                    const bool past = row0 + epi_row(i, 4 * (lane >> 4) + q) >= vocab;
+#pragma unroll
+                    for (int j = 0; j < kNt; ++j) acc[i][j][q] = past ? -__builtin_inff() : acc[i][j][q];
                 }
-            const int n = n0 + wn * kWn + j * 16 + (lane & 15);
-            int t = n < rows ? targets[n] : -1;
-            t = t >= v0 && t - v0 < vocab ? t - v0 : -1;
-            const int at = t - run0;
-            if (t >= 0 && at >= 0 && at < kRun) {
+        }
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            const int at = target_place<kWm>(t[j], row0, lane);
+            if (t[j] >= 0 && at >= 0) {
+                float l = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4 * kMt; ++e)
+                    if (at == e) l = acc[e >> 2][j][e & 3];
+                target_logit[n_first + j * 16] = simple ? sc.apply<kFast>(l) : l;
+            }
+            float top, sum = 0.f;
+            if (simple) {
+                top = sc.cap;
+                const float k = -2.0f * kLog2e * sc.cap;
 #pragma unroll
                 for (int i = 0; i < kMt; ++i)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (at == i * 4 + q) target_logit[n] = acc[i][j][q];
+                    for (int q = 0; q < 4; ++q) sum += exp2_fast(sc.r(acc[i][j][q]) * k);
+            } else {
+                top = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) top = fmaxf(top, acc[i][j][q]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                // A wave whose rows all lie past the vocabulary has nothing to add.
+                const float ref = top == -__builtin_inff() ? 0.f : top * kLog2e;
+#pragma unroll
+                for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) sum += exp2_fast(fmaf(acc[i][j][q], kLog2e, -ref));
             }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // A wave whose rows all lie past the vocabulary has nothing to add.
-            const float ref = top == -__builtin_inff() ? 0.f : top;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) sum += exp2_fast((acc[i][j][q] - ref) * kLog2e);
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (lane < 16) part[wm * kBn + wn * kWn + j * 16 + lane] = make_float2(top, sum);
@@ -149,54 +192,122 @@ __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
     p[2] = to_bf16(r - to_f32(p[1]));
 }
 
+// The largest finite |grad| of the rows that carry a loss, 1 if there is none. The
+// logits' gradient is held in units of it: where all rows weigh the same, as in
+// a mean, the factor's own rounding to 8 bits would scale whole gradients.
+__global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, const int32_t* targets, int rows, int vocab, float* unit) {
+    __shared__ float red[16];
+    float m = 0.f;
+    for (int r = threadIdx.x; r < rows; r += 1024) {
+        const float g = fabsf(grad[r]);
+        const int t = targets[r];
+        if (t >= 0 && t < vocab && g < __builtin_inff()) m = fmaxf(m, g);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
+    *unit = m > 0.f ? m : 1.f;
+}
+
 template <bool kFast, int kPlanes>
 struct GradEpi {
     Softcap sc;
-    int vocab, v0, rows, vocab_all;
+    int v0, rows, vocab_all;
     const int32_t* targets;
     const float* lse;
     const float* grad;
+    const float* unit;
     uint16_t* out;  // kPlanes x [rows_pad][ld]
     int64_t ld, plane;
+
+    // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is that of base 2, `g` four times it
+    // with a softcap, whose slope is 4 (r - r^2) and whose l is cap - 2 cap r.
+    __device__ __forceinline__ float dz(float z, float lse, float g, float one) const {
+        if (kFast && sc.cap > 0.f) {
+            const float r = sc.r(z);
+            const float p = exp2_fast(fmaf(r, -2.0f * kLog2e * sc.cap, lse));
+            return (p - one) * fmaf(-r, r, r) * g;
+        }
+        if (kFast) return (exp2_fast(fmaf(z, kLog2e, lse)) - one) * g;
+        const float l = sc.cap > 0.f ? sc.apply<false>(z) : z;
+        const float y = sc.cap > 0.f ? l * sc.inv : 0.f;
+        return (exp2_fast((l - lse) * kLog2e) - one) * fmaf(-y, y, 1.0f) * g;
+    }
 
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
     __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
                                            int wave, char* lds) const {
-        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN, kRun = kWm / 4;
-        const int run0 = m0 + wm * kWm + (lane >> 4) * kRun;
-        const float sq = sc.cap > 0.f ? sc.inv : 0.f;
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+        const int row0 = m0 + wm * kWm;
+        const int n_first = n0 + wn * kWn + (lane & 15);
+        int t[kNt];
+        float ls[kNt], gr[kNt];
+        load_targets(targets, n_first, rows, 0, vocab_all, t);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
-            const int n = n0 + wn * kWn + j * 16 + (lane & 15);
-            int t = n < rows ? targets[n] : -1;
-            const bool live = t >= 0 && t < vocab_all;
-            if (!live) t = -1;
-            const float z = live ? lse[n] : 0.f, g = live ? grad[n] : 0.f;
-            const int at = t - v0 - run0;
-            uint16_t* o = out + static_cast<int64_t>(n) * ld + run0;
+            const int n = min(n_first + j * 16, rows - 1);
+            ls[j] = lse[n];
+            gr[j] = grad[n];
+        }
+        const float u = *unit;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            float g = gr[j] / u;
+            if (kFast) {
+                ls[j] = sc.cap > 0.f ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
+                if (sc.cap > 0.f) g *= 4.0f;
+            }
+            gr[j] = g;
+        }
+        if (sc.cap > 0.f)
+            store<kWm, true>(acc, row0, n_first, lane, t, ls, gr);
+        else
+            store<kWm, false>(acc, row0, n_first, lane, t, ls, gr);
+    }
+    template <int kWm, bool kCap, int kMt, int kNt>
+    __device__ __forceinline__ void store(f32x4 (&acc)[kMt][kNt], int row0, int n_first, int lane, const int (&t)[kNt],
+                                          const float (&ls)[kNt], const float (&gr)[kNt]) const {
+        __builtin_assume(kCap ? sc.cap > 0.f : !(sc.cap > 0.f));
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            float d[kMt * 4];
+#pragma unroll
+            for (int e = 0; e < kMt * 4; ++e) d[e] = dz(acc[e >> 2][j][e & 3], ls[j], gr[j], 0.f);
+            const int at = t[j] < v0 ? -1 : target_place<kWm>(t[j] - v0, row0, lane);
+            if (at >= 0) {
+                float z = 0.f;
+#pragma unroll
+                for (int e = 0; e < kMt * 4; ++e)
+                    if (at == e) z = acc[e >> 2][j][e & 3];
+                const float x = dz(z, ls[j], gr[j], 1.0f);
+#pragma unroll
+                for (int e = 0; e < kMt * 4; ++e)
+                    if (at == e) d[e] = x;
+            }
+            uint16_t* o = out + static_cast<int64_t>(n_first + j * 16) * ld + row0 + (lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < kMt; i += 2) {
-                s16x8 pack[kPlanes];
+                u32x4 pack[kPlanes];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const int e = i * 4 + q;
-                    const float l = sc.apply<kFast>(acc[i + q / 4][j][q & 3]);
-                    float p = exp2_fast((l - z) * kLog2e);
-                    if (at == e) p -= 1.0f;
-                    const float y = l * sq;
-                    float d = p * fmaf(-y, y, 1.0f) * g;
-                    if (!live || run0 + e >= vocab) d = 0.f;
+                for (int q = 0; q < 4; ++q) {
+                    const float a = d[i * 4 + 2 * q], b = d[i * 4 + 2 * q + 1];
                     if (kPlanes == 1) {
-                        pack[0][q] = static_cast<short>(to_bf16(d));
+                        pack[0][q] = to_bf16(a, b);
                     } else {
-                        uint16_t s[3];
-                        split3(d, s);
+                        uint16_t x[3], y[3];
+                        split3(a, x);
+                        split3(b, y);
 #pragma unroll
-                        for (int k = 0; k < kPlanes; ++k) pack[k][q] = static_cast<short>(s[k]);
+                        for (int k = 0; k < kPlanes; ++k) pack[k][q] = x[k] | static_cast<uint32_t>(y[k]) << 16;
                     }
+#pragma unroll
+                    for (int k = 0; k < kPlanes; ++k) pack[k][q] = t[j] < 0 ? 0u : pack[k][q];  // no loss: nothing, not NaN either
                 }
 #pragma unroll
-                for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<s16x8*>(o + k * plane + i * 4) = pack[k];
+                for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<u32x4*>(o + k * plane + i * 16) = pack[k];
             }
         }
     }
@@ -234,11 +345,13 @@ struct WeightEpi {
     int64_t ld;
     int dim, vocab;
     bool vec;  // rows take 4-element stores
+    const float* unit;
 
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
     __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
                                            int wave, char* lds) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+        const float u = *unit;
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             const int v = n0 + wn * kWn + j * 16 + (lane & 15);
@@ -249,10 +362,10 @@ struct WeightEpi {
                 T* o = out + v * ld + d;
                 T q[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[e] = from_f32<T>(acc[i][j][e]);
+                for (int e = 0; e < 4; ++e) q[e] = from_f32<T>(acc[i][j][e] * u);
                 if (vec && d + 4 <= dim) {
                     if constexpr (sizeof(T) == 4)
-                        *reinterpret_cast<f32x4*>(o) = acc[i][j];
+                        *reinterpret_cast<f32x4*>(o) = f32x4{q[0], q[1], q[2], q[3]};
                     else
                         *reinterpret_cast<uint2*>(o) = make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16,
                                                                   q[2] | static_cast<uint32_t>(q[3]) << 16);
@@ -269,13 +382,13 @@ struct WeightEpi {
 // The parts of dhidden in order, rounded once. A workgroup per 256 channels of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int64_t ld, int64_t split, int splits, int dim,
-                                                         T* out, int64_t out_ld) {
+                                                         const float* unit, T* out, int64_t out_ld) {
     const int d = blockIdx.x * 256 + threadIdx.x;
     if (d >= dim) return;
     const int64_t r = blockIdx.y;
     float s = 0.f;
     for (int i = 0; i < splits; ++i) s += parts[i * split + r * ld + d];
-    out[r * out_ld + d] = from_f32<T>(s);
+    out[r * out_ld + d] = from_f32<T>(s * *unit);
 }
 
 // Rows of T into bf16 planes whose rows are `kpad` long, zeros behind `dim`.
@@ -374,7 +487,7 @@ struct Call {
         if (plan.small)
             run<kSmallTileM, kSmallTileN, 4, 1, true, true>(g, e);
         else
-            run<256, 256, 2, 4, true, true>(g, e);
+            run<256, 256, 2, 2, true, true>(g, e);
     }
     void forward() const {
         const Operand h = hidden();
@@ -391,32 +504,34 @@ struct Call {
         T* dh = static_cast<T*>(x.dhidden);
         const int64_t dw_ld = x.vocab > 1 ? x.dweight_stride : x.dim, dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
         const Operand h = hidden();
-        const int64_t ld = plan.piece, dlp = ld * plan.rows_pad;
+        const int64_t ld = plan.dz_ld, dlp = ld * plan.rows_pad;
+        float* unit = b.row;
+        grad_unit_kernel<<<1, 1024, 0, st>>>(x.grad, x.targets, x.rows, x.vocab, unit);
         const int64_t hld = (x.dim + 3) / 4 * 4;
         const int64_t split = x.rows * hld;
         int splits = plan.splits;
         for (int v0 = 0; v0 < x.vocab; v0 += plan.piece) {
             const int n = std::min(plan.piece, x.vocab - v0);
             const Operand w = weights(v0, n);
-            GradEpi<kFast, kPlanes> e{softcap(), n, v0, x.rows, x.vocab, x.targets, x.lse, x.grad, b.dlogits, ld, dlp};
+            GradEpi<kFast, kPlanes> e{softcap(), v0, x.rows, x.vocab, x.targets, x.lse, x.grad, unit, b.dlogits, ld, dlp};
             logits(w, h, n, e);
             // Rows past the batch read as zeros: they are no rows of the hidden states either.
             const Operand dz{b.dlogits, ld, x.rows * ld, dlp};
             if (dh) {
                 GemmArgs g = gemm(w, dz, n, x.dim, x.rows, 256, 256, splits);
                 HiddenEpi he{b.dhidden, hld, split, x.dim, x.rows, v0 > 0};
-                run<256, 256, 2, 4, false, true>(g, he);
+                run<256, 256, 2, 2, false, true>(g, he);
             }
             if (dw) {
                 GemmArgs g = gemm(h, dz, x.rows, x.dim, n, 256, 256, 1);
-                WeightEpi<T> we{dw + v0 * dw_ld, dw_ld, x.dim, n, false};
+                WeightEpi<T> we{dw + v0 * dw_ld, dw_ld, x.dim, n, false, unit};
                 we.vec = aligned_to(we.out, 4 * sizeof(T)) && (x.vocab <= 1 || dw_ld % 4 == 0);
-                run<256, 256, 2, 4, false, false>(g, we);
+                run<256, 256, 2, 2, false, false>(g, we);
             }
         }
         if (dh) {
             for_rows(x.rows, [&](int64_t r, unsigned n) {
-                hidden_sum_kernel<T><<<dim3((x.dim + 255) / 256, n), 256, 0, st>>>(b.dhidden + r * hld, hld, split, splits, x.dim, dh + r * dh_ld,
+                hidden_sum_kernel<T><<<dim3((x.dim + 255) / 256, n), 256, 0, st>>>(b.dhidden + r * hld, hld, split, splits, x.dim, unit, dh + r * dh_ld,
                                                                          dh_ld);
             });
         }
