@@ -11,11 +11,6 @@
 // columns and lane i gets column i's 4 values), so no transposed copy of the
 // weights, the hidden states or the gradient is ever written.
 //
-// float32 operands arrive as three bf16 planes (x = hi + mid + lo, 24 bits of
-// mantissa in all) and the product is the sum of the six plane pairs above
-// 2^-24: the same loop with six times the steps ("segments"), about 400
-// TFLOP/s at most against 157 of the f32 matrix instructions.
-//
 // Tiles go from memory to LDS without passing registers (buffer loads to LDS,
 // 16 bytes a lane). The hardware's bounds check gives zeros beyond an operand's
 // end, so ragged rows and a ragged last step need no code of their own; along k
@@ -46,30 +41,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStepK = 64;        // k per step of the loop: 128-byte rows along k
-constexpr int kMaxSegments = 6;
 
-// One operand: planes of bf16 elements, `ld` elements from row to row, `end`
-// elements readable from the start of a plane, `plane` elements between planes.
+// One operand: elements of its type, `ld` from row to row, `end` readable from the start.
 struct Operand {
-    const uint16_t* p;
+    const void* p;
     int64_t ld;
     int64_t end;
-    int64_t plane;
 };
 
 struct GemmArgs {
     Operand a, b;
     int k;               // length of the sum
-    int segments;        // 1 (bf16) or 6 (float32 in three planes)
     int tiles_m, tiles_n;
     int splits;          // parts of the sum, each with an output of its own
-    int steps_per_split; // steps of kStepK in a part
+    int steps_per_split; // steps of the kernel's k in a part
     int group_m;         // tiles along m that run together
 };
-
-// Plane pairs of the segments, the smallest products first.
-__device__ __forceinline__ int seg_a(int s, int segments) { return segments == 1 ? 0 : (0x210100 >> (4 * (5 - s))) & 3; }
-__device__ __forceinline__ int seg_b(int s, int segments) { return segments == 1 ? 0 : (0x012010 >> (4 * (5 - s))) & 3; }
 
 // Which of the wave's rows row i of its tile mt of 16 is, for an operand of the M
 // side along k: lanes that hold rows 4 a .. 4 a + 3 of the accumulators get 8
@@ -107,10 +94,8 @@ struct TileLoader {
     uint32_t left_lo;      // readable bytes from `base`
     int32_t left_hi;
     int64_t step;          // bytes from one k step to the next
-    int64_t plane;
 
     __device__ __forceinline__ void init(const Operand& o, int row0, int first, int wave, int lane) {
-        plane = o.plane * 2;
         step = kAlong ? kStepK * 2 : kStepK * o.ld * 2;
         const int64_t skip = (kAlong ? static_cast<int64_t>(row0) * o.ld : row0) * 2 + step * first;
         base = reinterpret_cast<const char*>(o.p) + skip;
@@ -134,10 +119,10 @@ struct TileLoader {
             }
         }
     }
-    // The step's resource: of plane `seg`, nothing of it if `none`.
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(int seg, bool none) const {
+    // The step's resource, nothing of it if `none`.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(bool none) const {
         const uint32_t n = left_hi > 0 ? 0x7ffffff0u : min(left_lo, 0x7ffffff0u);
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + plane * seg), 0, static_cast<int>(none ? 0u : n), 0x00027000);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(none ? 0u : n), 0x00027000);
     }
     __device__ __forceinline__ void advance() {
         base += step;
@@ -269,7 +254,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
     const int steps = (g.k + kStepK - 1) / kStepK;
     const int first = place.split * g.steps_per_split;
     const int last = min(steps, first + g.steps_per_split);
-    const int total = max(0, last - first) * g.segments;
+    const int total = max(0, last - first);
     using LoaderA = TileLoader<kBm, kAAlong, true, kWaves>;
     using LoaderB = TileLoader<kBn, kBAlong, false, kWaves>;
     LoaderA la;
@@ -293,7 +278,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
     constexpr int kProducts = kMt * kNt;
     constexpr bool kInPlace = kProducts >= 32;
     // Loads of steps past the end bring zeros, whose products change nothing.
-    int load_left = total, seg = 0, k_left = g.k - first * kStepK;
+    int load_left = total, k_left = g.k - first * kStepK;
     __amdgpu_buffer_rsrc_t ra, rb;
     auto mask = [&]() __attribute__((always_inline)) {
         if (k_left < kStepK) {
@@ -301,12 +286,10 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
             lb.mask(k_left);
         }
     };
-    auto tile_a = [&]() __attribute__((always_inline)) { ra = la.tile(seg_a(seg, g.segments), load_left <= 0); };
-    auto tile_b = [&]() __attribute__((always_inline)) { rb = lb.tile(seg_b(seg, g.segments), load_left <= 0); };
+    auto tile_a = [&]() __attribute__((always_inline)) { ra = la.tile(load_left <= 0); };
+    auto tile_b = [&]() __attribute__((always_inline)) { rb = lb.tile(load_left <= 0); };
     auto advance = [&]() __attribute__((always_inline)) {
         --load_left;
-        if (++seg < g.segments) return;
-        seg = 0;
         la.advance();
         lb.advance();
         k_left -= kStepK;

@@ -19,8 +19,10 @@
 // 16-byte pieces.
 #include <hip/hip_runtime.h>
 
-#include "head_gemm.h"
 #include "head_internal.h"
+
+#include "head_gemm.h"
+#include "head_gemm32.h"
 
 namespace ge {
 namespace head {
@@ -184,14 +186,6 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* stats, int ld, 
     }
 }
 
-// hi + mid + lo = x to 24 bits; a non-finite x keeps its value in hi alone.
-__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
-    p[0] = to_bf16(x);
-    const float r = x - to_f32(p[0]);
-    p[1] = to_bf16(r);
-    p[2] = to_bf16(r - to_f32(p[1]));
-}
-
 // The largest finite |grad| of the rows that carry a loss, 1 if there is none. The
 // logits' gradient is held in units of it: where all rows weigh the same, as in
 // a mean, the factor's own rounding to 8 bits would scale whole gradients.
@@ -212,16 +206,17 @@ __global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, cons
     *unit = m > 0.f ? m : 1.f;
 }
 
-template <bool kFast, int kPlanes>
+template <typename T>
 struct GradEpi {
+    static constexpr bool kFast = sizeof(T) == 2;
     Softcap sc;
     int v0, rows, vocab_all;
     const int32_t* targets;
     const float* lse;
     const float* grad;
     const float* unit;
-    uint16_t* out;  // kPlanes x [rows_pad][ld]
-    int64_t ld, plane;
+    T* out;  // [rows_pad][ld]
+    int64_t ld;
 
     // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is that of base 2, `g` four times it
     // with a softcap, whose slope is 4 (r - r^2) and whose l is cap - 2 cap r.
@@ -287,27 +282,22 @@ struct GradEpi {
                 for (int e = 0; e < kMt * 4; ++e)
                     if (at == e) d[e] = x;
             }
-            uint16_t* o = out + static_cast<int64_t>(n_first + j * 16) * ld + row0 + (lane >> 4) * 8;
+            T* o = out + static_cast<int64_t>(n_first + j * 16) * ld + row0 + (lane >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < kMt; i += 2) {
-                u32x4 pack[kPlanes];
+                constexpr int kWords = 2 * sizeof(T);
+                uint32_t pack[kWords];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float a = d[i * 4 + 2 * q], b = d[i * 4 + 2 * q + 1];
-                    if (kPlanes == 1) {
-                        pack[0][q] = to_bf16(a, b);
-                    } else {
-                        uint16_t x[3], y[3];
-                        split3(a, x);
-                        split3(b, y);
-#pragma unroll
-                        for (int k = 0; k < kPlanes; ++k) pack[k][q] = x[k] | static_cast<uint32_t>(y[k]) << 16;
-                    }
-#pragma unroll
-                    for (int k = 0; k < kPlanes; ++k) pack[k][q] = t[j] < 0 ? 0u : pack[k][q];  // no loss: nothing, not NaN either
+                for (int q = 0; q < kWords; ++q) {
+                    if constexpr (sizeof(T) == 2)
+                        pack[q] = to_bf16(d[i * 4 + 2 * q], d[i * 4 + 2 * q + 1]);
+                    else
+                        pack[q] = __builtin_bit_cast(uint32_t, d[i * 4 + q]);
+                    if (t[j] < 0) pack[q] = 0;  // no loss: nothing, not NaN either
                 }
 #pragma unroll
-                for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<u32x4*>(o + k * plane + i * 16) = pack[k];
+                for (int q = 0; q < kWords; q += 4)
+                    *reinterpret_cast<u32x4*>(o + i * 16 + q * 4 / sizeof(T)) = u32x4{pack[q], pack[q + 1], pack[q + 2], pack[q + 3]};
             }
         }
     }
@@ -391,21 +381,13 @@ __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int
     out[r * out_ld + d] = from_f32<T>(s * *unit);
 }
 
-// Rows of T into bf16 planes whose rows are `kpad` long, zeros behind `dim`.
+// Rows into rows that are `kpad` long, zeros behind `dim`.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, int dim, int kpad, uint16_t* out, int64_t plane) {
+__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, int dim, int kpad, T* out) {
     const int d = blockIdx.x * 256 + threadIdx.x;
     if (d >= kpad) return;
     const int64_t r = blockIdx.y;
-    const int64_t o = r * kpad + d;
-    const T x = d < dim ? in[r * ld + d] : T(0);
-    if constexpr (sizeof(T) == 4) {
-        uint16_t s[3];
-        split3(x, s);
-        for (int k = 0; k < 3; ++k) out[k * plane + o] = s[k];
-    } else {
-        out[o] = x;
-    }
+    out[r * kpad + d] = d < dim ? in[r * ld + d] : T(0);
 }
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, int64_t ld, int dim) {
@@ -420,10 +402,10 @@ void for_rows(int64_t rows, F launch) {
 }
 
 template <typename T>
-void pack(const T* in, int64_t ld, int64_t rows, int dim, int64_t kpad, uint16_t* out, int64_t plane, hipStream_t st) {
+void pack(const T* in, int64_t ld, int64_t rows, int dim, int64_t kpad, T* out, hipStream_t st) {
     for_rows(rows, [&](int64_t r, unsigned n) {
         pack_kernel<T><<<dim3(static_cast<unsigned>((kpad + 255) / 256), n), 256, 0, st>>>(in + r * ld, ld, dim, static_cast<int>(kpad),
-                                                                                out + r * kpad, plane);
+                                                                                out + r * kpad);
     });
 }
 
@@ -433,61 +415,59 @@ struct Call {
     const LossPlan& plan;
     const Buffers& b;
     hipStream_t st;
-    static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
-    static constexpr int kSegments = sizeof(T) == 4 ? kMaxSegments : 1;
     static constexpr bool kFast = sizeof(T) == 2;
 
+    Operand operand(const T* p, int64_t ld, int64_t rows, bool packed, void* to) const {
+        if (!packed) return Operand{p, ld, (rows - 1) * ld + x.dim};
+        pack(p, ld, rows, x.dim, plan.kpad, static_cast<T*>(to), st);
+        return Operand{to, plan.kpad, rows * plan.kpad};
+    }
     Operand hidden() const {
-        if (plan.pack_h) {
-            const int64_t plane = x.rows * plan.kpad;
-            pack(static_cast<const T*>(x.hidden), x.hidden_stride, x.rows, x.dim, plan.kpad, b.hpack, plane, st);
-            return Operand{b.hpack, plan.kpad, plane, plane};
-        }
-        const int64_t ld = x.rows > 1 ? x.hidden_stride : x.dim;
-        return Operand{static_cast<const uint16_t*>(x.hidden), ld, (x.rows - 1) * ld + x.dim, 0};
+        return operand(static_cast<const T*>(x.hidden), x.rows > 1 ? x.hidden_stride : x.dim, x.rows, plan.pack_h, b.hpack);
     }
     // Rows v0 .. v0 + n of the weights.
     Operand weights(int v0, int n) const {
         const int64_t ld = x.vocab > 1 ? x.weight_stride : x.dim;
-        if (plan.pack_w) {
-            const int64_t plane = n * plan.kpad;
-            pack(static_cast<const T*>(x.weight) + v0 * ld, ld, n, x.dim, plan.kpad, b.wpack, plane, st);
-            return Operand{b.wpack, plan.kpad, plane, plane};
-        }
-        return Operand{static_cast<const uint16_t*>(x.weight) + v0 * ld, ld, (n - 1) * ld + x.dim, 0};
+        return operand(static_cast<const T*>(x.weight) + v0 * ld, ld, n, plan.pack_w, b.wpack);
     }
     Softcap softcap() const {
         if (!(x.softcap > 0.f)) return Softcap{0.f, 0.f, 0.f};
         return Softcap{x.softcap, 1.0f / x.softcap, 2.0f * kLog2e / x.softcap};
     }
-    GemmArgs gemm(const Operand& a, const Operand& bb, int64_t k, int m, int n, int bm, int bn, int splits) const {
+    template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
+    void run(const Operand& a, const Operand& bb, int64_t k, int m, int n, int splits, int group, const Epi& e) const {
+        constexpr int kStep = sizeof(T) == 4 ? kStepK32 : kStepK;
         GemmArgs g{};
         g.a = a;
         g.b = bb;
         g.k = static_cast<int>(k);
-        g.segments = kSegments;
-        g.tiles_m = (m + bm - 1) / bm;
-        g.tiles_n = (n + bn - 1) / bn;
-        const int steps = (g.k + kStepK - 1) / kStepK;
-        g.steps_per_split = (steps + splits - 1) / splits;
+        g.tiles_m = (m + kBm - 1) / kBm;
+        g.tiles_n = (n + kBn - 1) / kBn;
+        g.steps_per_split = ((g.k + kStep - 1) / kStep + splits - 1) / splits;
         g.splits = splits;
-        g.group_m = 4;
-        return g;
-    }
-    template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
-    void run(const GemmArgs& g, const Epi& e) const {
+        g.group_m = group;
         const unsigned blocks = static_cast<unsigned>(g.tiles_m) * g.tiles_n * g.splits;
-        gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 64 * kWm * kWn, 0, st>>>(g, e);
+        if constexpr (sizeof(T) == 4)
+            gemm32_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 256, 0, st>>>(g, e);
+        else
+            gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 256, 0, st>>>(g, e);
     }
     template <typename Epi>
     void logits(const Operand& w, const Operand& h, int n, const Epi& e) const {
         // A packed row's padding is zeros on both sides; a direct row ends at dim.
         const int64_t k = plan.pack_w && plan.pack_h ? plan.kpad : x.dim;
-        const GemmArgs g = gemm(w, h, k, n, x.rows, plan.tile_m, plan.tile_n, 1);
-        if (plan.small)
-            run<kSmallTileM, kSmallTileN, 4, 1, true, true>(g, e);
-        else
-            run<256, 256, 2, 2, true, true>(g, e);
+        if constexpr (sizeof(T) == 4) {
+            if (plan.tile_n == 32)
+                run<128, 32, 4, 1, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else if (plan.tile_n == 96)
+                run<128, 96, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else
+                run<128, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
+        } else if (plan.tile_n == kSmallTileN) {
+            run<kSmallTileM, kSmallTileN, 4, 1, true, true>(w, h, k, n, x.rows, 1, 4, e);
+        } else {
+            run<256, 256, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
+        }
     }
     void forward() const {
         const Operand h = hidden();
@@ -504,7 +484,8 @@ struct Call {
         T* dh = static_cast<T*>(x.dhidden);
         const int64_t dw_ld = x.vocab > 1 ? x.dweight_stride : x.dim, dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
         const Operand h = hidden();
-        const int64_t ld = plan.dz_ld, dlp = ld * plan.rows_pad;
+        const int64_t ld = plan.dz_ld;
+        constexpr int kTile = sizeof(T) == 4 ? 128 : 256;
         float* unit = b.row;
         grad_unit_kernel<<<1, 1024, 0, st>>>(x.grad, x.targets, x.rows, x.vocab, unit);
         const int64_t hld = (x.dim + 3) / 4 * 4;
@@ -513,20 +494,18 @@ struct Call {
         for (int v0 = 0; v0 < x.vocab; v0 += plan.piece) {
             const int n = std::min(plan.piece, x.vocab - v0);
             const Operand w = weights(v0, n);
-            GradEpi<kFast, kPlanes> e{softcap(), v0, x.rows, x.vocab, x.targets, x.lse, x.grad, unit, b.dlogits, ld, dlp};
+            GradEpi<T> e{softcap(), v0, x.rows, x.vocab, x.targets, x.lse, x.grad, unit, reinterpret_cast<T*>(b.dlogits), ld};
             logits(w, h, n, e);
             // Rows past the batch read as zeros: they are no rows of the hidden states either.
-            const Operand dz{b.dlogits, ld, x.rows * ld, dlp};
+            const Operand dz{b.dlogits, ld, x.rows * ld};
             if (dh) {
-                GemmArgs g = gemm(w, dz, n, x.dim, x.rows, 256, 256, splits);
                 HiddenEpi he{b.dhidden, hld, split, x.dim, x.rows, v0 > 0};
-                run<256, 256, 2, 2, false, true>(g, he);
+                run<kTile, kTile, 2, 2, false, true>(w, dz, n, x.dim, x.rows, splits, 6, he);
             }
             if (dw) {
-                GemmArgs g = gemm(h, dz, x.rows, x.dim, n, 256, 256, 1);
                 WeightEpi<T> we{dw + v0 * dw_ld, dw_ld, x.dim, n, false, unit};
                 we.vec = aligned_to(we.out, 4 * sizeof(T)) && (x.vocab <= 1 || dw_ld % 4 == 0);
-                run<256, 256, 2, 2, false, false>(g, we);
+                run<kTile, kTile, 2, 2, false, false>(h, dz, x.rows, x.dim, n, 1, 4, we);
             }
         }
         if (dh) {

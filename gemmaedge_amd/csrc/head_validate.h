@@ -15,16 +15,17 @@ namespace ge {
 namespace head {
 
 constexpr int kTileM = 256;       // vocabulary (or channels) of a large tile
+constexpr int kTile32 = 128;      // of a tile of float32 operands
 constexpr int kSmallRows = 64;    // batches up to this take the small tiles
 constexpr int kSmallTileM = 128;
 constexpr int kSmallTileN = 32;
-constexpr int kPadK = 64;         // packed planes' rows are padded to this
+constexpr int kPadK = 64;         // packed rows are padded to this
 constexpr int kPadDz = 64;        // and the logits' gradient's by this: rows a power of two apart share their memory channels
 constexpr int kNormParts = 512;   // workgroups of the norm's backward pass, whose weight gradients are summed last
 constexpr int kNormBlocks = 1280; // and of the forward pass, at most
 
 inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-inline int planes_of(int dtype) { return dtype == GE_DTYPE_F32 ? 3 : 1; }
+inline int planes_of(int dtype) { return dtype == GE_DTYPE_F32 ? 2 : 1; }  // of two bytes
 inline int elem_size(int dtype) { return dtype == GE_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == GE_DTYPE_F32 || dtype == GE_DTYPE_BF16; }
 
@@ -35,8 +36,8 @@ struct Capacity {
     bool train;
     int64_t stats;    // float2 per row and vocabulary tile
     int64_t row;      // floats per row: target logits, norm's row sums
-    int64_t hpack;    // hidden states as padded bf16 planes
-    int64_t wpack;    // a piece of the weights as padded bf16 planes
+    int64_t hpack;    // hidden states in padded rows
+    int64_t wpack;    // a piece of the weights in padded rows
     int64_t dlogits;  // the logits' gradient of a piece of the vocabulary
     int64_t dhidden;  // float32 parts of the hidden states' gradient
     int64_t norm;     // float32 parts of the norm weights' gradients
@@ -45,11 +46,12 @@ struct Capacity {
 // Workspace of a handle. Pieces of the vocabulary are as large as fits 512 MB
 // of logits' gradient: each piece adds to the hidden states' float32 gradient and
 // ends three launches (4,096 rows of 2,816 channels: 0.3 ms for 256 MB). A packed
-// piece of weights takes at most 64 MB a plane.
+// piece of weights takes at most 64 MB (bf16).
 inline void size_workspace(Capacity& c) {
     const int64_t rows = c.max_rows, dim = round_up(c.max_dim, kPadK), vocab = round_up(c.max_vocab, kTileM);
     const int64_t planes = planes_of(c.dtype), rows_pad = round_up(rows, 256);
-    c.stats = 8 * std::max(rows * (vocab / kTileM), std::min<int64_t>(rows, kSmallRows) * (vocab / kSmallTileM));
+    c.stats = 8 * std::max(rows * (vocab / (c.dtype == GE_DTYPE_F32 ? kTile32 : kTileM)),
+                           std::min<int64_t>(rows, kSmallRows) * (vocab / kSmallTileM));
     c.row = 8 * rows;
     c.hpack = 2 * planes * rows * dim;
     const int64_t cols = std::min(vocab, std::max<int64_t>(kTileM, ((64LL << 20) / (2 * dim)) / kTileM * kTileM));
@@ -57,7 +59,7 @@ inline void size_workspace(Capacity& c) {
     c.dlogits = c.dhidden = c.norm = 0;
     if (!c.train) return;
     const int64_t per_col = 2 * planes * rows_pad;
-    c.dlogits = std::min(per_col * (vocab + kPadDz), std::max<int64_t>(per_col * (kTileM + kPadDz), 512LL << 20));
+    c.dlogits = std::min(per_col * (vocab + kPadDz), std::max<int64_t>(per_col * kTileM, 512LL << 20) + per_col * kPadDz);
     const int64_t tiles = (rows_pad / 256) * ((dim + 255) / 256);
     c.dhidden = 4LL * 256 * 256 * std::max<int64_t>(tiles, 1024);
     c.norm = 4LL * 2 * kNormParts * c.max_dim;
@@ -116,10 +118,9 @@ inline int check_norm(const Capacity& c, const ge_norm_args& x, bool backward, c
 
 // How a loss call runs.
 struct LossPlan {
-    bool pack_h, pack_w;  // operands copied into padded bf16 planes first
-    int planes;           // 1 or 3
-    int64_t kpad;         // packed planes' row length
-    int small;            // small tiles (few rows)
+    bool pack_h, pack_w;  // operands copied into padded rows first
+    int planes;           // of two bytes: 1 or 2
+    int64_t kpad;         // packed rows' length
     int tile_m, tile_n;   // of the logits' product
     int rows_pad;         // rows of the logits' gradient
     int piece;            // vocabulary per piece of the backward (a multiple of kTileM)
@@ -156,35 +157,48 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
         return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a tensor is not aligned to its elements");
 
     plan.planes = planes_of(c.dtype);
-    // Tiles are fetched 16 bytes a lane: other rows are packed first.
+    // bf16 tiles are fetched 16 bytes a lane into LDS: other rows are packed first.
+    // float32 ones pass registers and need no alignment. Offsets in a tile have 31 bits.
     auto direct = [&](const void* p, int64_t stride, int rows) {
-        return c.dtype == GE_DTYPE_BF16 && aligned_to(p, 16) && (rows <= 1 || stride % 8 == 0) && x.dim % 8 == 0 &&
-               stride <= (1 << 21);
+        if (rows > 1 && stride > (1 << 21)) return false;
+        return c.dtype == GE_DTYPE_F32 || (aligned_to(p, 16) && (rows <= 1 || stride % 8 == 0) && x.dim % 8 == 0);
     };
     plan.pack_h = !direct(x.hidden, x.hidden_stride, x.rows);
     plan.pack_w = !direct(x.weight, x.weight_stride, x.vocab);
     plan.kpad = round_up(x.dim, kPadK);
-    plan.small = x.rows <= kSmallRows;
-    plan.tile_m = plan.small ? kSmallTileM : kTileM;
-    plan.tile_n = plan.small ? kSmallTileN : 256;
-    plan.rows_pad = static_cast<int>(round_up(std::max(x.rows, 1), 256));
+    if (c.dtype == GE_DTYPE_F32) {
+        // The tile that pads the rows least, a little in favour of wide ones: 128,
+        // 96 (300 rows: 384 either way, 96 rows: 96 against 128) or 32 for few rows.
+        plan.tile_m = kTile32;
+        plan.tile_n = x.rows <= 32 ? 32 : round_up(x.rows, 96) + 16 < round_up(x.rows, 128) ? 96 : 128;
+    } else {
+        const bool small = x.rows <= kSmallRows;
+        plan.tile_m = small ? kSmallTileM : kTileM;
+        plan.tile_n = small ? kSmallTileN : 256;
+    }
+    plan.rows_pad = static_cast<int>(round_up(std::max(x.rows, 1), 256));  // whole tiles of any width that is chosen
     const int64_t vpad = round_up(x.vocab, kTileM);
     const int64_t pack_cols = c.wpack / (2 * plan.planes * plan.kpad) / kTileM * kTileM;
     plan.pack_piece = static_cast<int>(plan.pack_w ? std::min(vpad, pack_cols) : vpad);
     if (backward) {
         const int64_t cols = (c.dlogits / (2LL * plan.planes * plan.rows_pad) - kPadDz) / kTileM * kTileM;
-        plan.piece = static_cast<int>(std::min<int64_t>(std::min<int64_t>(vpad, cols), plan.pack_piece));
+        // as few pieces as fit, all of about the same size
+        const int64_t most = std::min<int64_t>(std::min<int64_t>(vpad, cols), plan.pack_piece);
+        const int64_t pieces = (vpad + most - 1) / most;
+        plan.piece = static_cast<int>(std::min(most, round_up((vpad + pieces - 1) / pieces, kTileM)));
         plan.dz_ld = plan.piece + kPadDz;
-        // Parts of the sum over the piece: tiles of 256 x 256 run a compute unit
-        // each, 256 at a time; a part costs its steps and about 12 more for its
-        // beginning and for adding what it has.
-        const int64_t tiles = static_cast<int64_t>(plan.rows_pad / 256) * ((x.dim + 255) / 256);
+        // Parts of the sum over the piece: 256 tiles run at a time, one on each compute
+        // unit (512 of float32, two on each); a part costs its steps and about 12 more
+        // for its beginning and for adding what it has.
+        const int64_t tile = c.dtype == GE_DTYPE_F32 ? kTile32 : 256, slots = c.dtype == GE_DTYPE_F32 ? 512 : 256;
+        const int64_t tiles = (x.rows + tile - 1) / tile * ((x.dim + tile - 1) / tile);
         const int64_t steps = plan.piece / 64;
-        const int64_t fit = std::min<int64_t>(std::min<int64_t>(32, steps), c.dhidden / (4LL * 256 * 256 * tiles));
+        const int64_t most_bytes = 4 * std::max<int64_t>(x.rows, 1) * round_up(x.dim, 4);
+        const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(32, steps), c.dhidden / most_bytes));
         int64_t best = INT64_MAX;
         plan.splits = 1;
         for (int64_t s = 1; s <= fit; ++s) {
-            const int64_t cost = (tiles * s + 255) / 256 * ((steps + s - 1) / s + 12);
+            const int64_t cost = (tiles * s + slots - 1) / slots * ((steps + s - 1) / s + 12);
             if (cost < best) {
                 best = cost;
                 plan.splits = static_cast<int>(s);
