@@ -27,21 +27,23 @@ namespace ge {
 namespace head {
 namespace {
 
-constexpr int kVec = 8;              // channels of a vector
+// Channels of a vector: 16 bytes, so that neighbouring lanes' loads are neighbours.
+template <typename T>
+constexpr int vec_of = 16 / sizeof(T);
 constexpr int kNormThreads = 512;    // most threads of a workgroup
 constexpr int kGroupDim = 1024;      // longest row of a lane group
 constexpr int kRegisterDim = 8192;   // longest row that stays in registers
 
-template <typename T>
+template <typename T, int kVec>
 struct Vec {
     T v[kVec];
 };
 
-// Channels i .. i + 7 of a row of `dim`, zeros behind its end. Rows need no
+// kVec channels of a row of `dim` from i on, zeros behind its end. Rows need no
 // alignment beyond their elements': the loads are 16 bytes wide at any address.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int i, int dim) {
-    Vec<T> r;
+template <int kVec, typename T>
+__device__ __forceinline__ Vec<T, kVec> load_vec(const T* row, int i, int dim) {
+    Vec<T, kVec> r;
     if (i + kVec <= dim) {
         __builtin_memcpy(&r, row + i, sizeof(r));
     } else {
@@ -50,9 +52,9 @@ __device__ __forceinline__ Vec<T> load_vec(const T* row, int i, int dim) {
     }
     return r;
 }
-template <typename T>
+template <typename T, int kVec>
 __device__ __forceinline__ void store_vec(T* row, int i, int dim, const float (&x)[kVec]) {
-    Vec<T> r;
+    Vec<T, kVec> r;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) r.v[e] = from_f32<T>(x[e]);
     if (i + kVec <= dim) {
@@ -64,34 +66,65 @@ __device__ __forceinline__ void store_vec(T* row, int i, int dim, const float (&
     }
 }
 
+// Sum over groups of kLanes lanes, the same in each of them. Steps within 16 lanes
+// are modifiers of the addition, the others swap rows of lanes between registers:
+// nothing passes LDS, whose six round trips a sum took longer than a row's loads.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+    auto dpp = [&](auto ctrl) {
+        const int w = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true);
+        v += __builtin_bit_cast(float, w);
+    };
+    dpp(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    dpp(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    dpp(std::integral_constant<int, 0x141>{});  // mirrored in 8
+    if (kLanes >= 16) dpp(std::integral_constant<int, 0x140>{});  // mirrored in 16
+    if (kLanes >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const uint32_t a = r[0], b = r[1];
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    if (kLanes >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t a = r[0], b = r[1];
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    return v;
+}
+
 // The threads of one row: kGroup lanes of a wave, or (0) the whole workgroup.
+constexpr int kMostWaves = kNormThreads / 64;
 template <int kGroup>
 struct Team {
     int lane, slot, lanes, slots;
-    float2* red;  // [2][kNormThreads / 64]
+    float2* red;  // [2][kMostWaves]
     int turn = 0;
     __device__ __forceinline__ explicit Team(float2* lds) : red(lds) {
         lanes = kGroup ? kGroup : blockDim.x;
         lane = kGroup ? threadIdx.x % (kGroup ? kGroup : 1) : threadIdx.x;
         slot = kGroup ? threadIdx.x / (kGroup ? kGroup : 1) : 0;
         slots = kGroup ? blockDim.x / (kGroup ? kGroup : 1) : 1;
+        if (!kGroup) {  // waves that are not there add nothing
+            if (threadIdx.x < 2 * kMostWaves) red[threadIdx.x] = make_float2(0.f, 0.f);
+            __syncthreads();
+        }
     }
     // Sums of two values over the team, the same in every thread. Two buffers in
     // turn: a wave writes one again only after a barrier that every wave reaches
     // when it has read it.
     __device__ __forceinline__ float2 sum(float2 v) {
-#pragma unroll
-        for (int o = (kGroup ? kGroup : 64) / 2; o > 0; o >>= 1) {
-            v.x += __shfl_xor(v.x, o);
-            v.y += __shfl_xor(v.y, o);
-        }
+        v.x = lanes_sum<kGroup ? kGroup : 64>(v.x);
+        v.y = lanes_sum<kGroup ? kGroup : 64>(v.y);
         if (kGroup) return v;
-        float2* buf = red + turn * (kNormThreads / 64);
+        float2* buf = red + turn * kMostWaves;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
         float2 s = buf[0];
-        for (int i = 1; i < lanes / 64; ++i) {
+#pragma unroll
+        for (int i = 1; i < kMostWaves; ++i) {
             s.x += buf[i].x;
             s.y += buf[i].y;
         }
@@ -101,7 +134,8 @@ struct Team {
 
 template <typename T, typename W, int kGroup, int kVecs>
 __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
-    __shared__ float2 red[2 * (kNormThreads / 64)];
+    __shared__ __align__(16) float2 red[2 * kMostWaves];
+    constexpr int kVec = vec_of<T>;
     Team<kGroup> team(red);
     const int dim = x.dim;
     const float n = static_cast<float>(dim);
@@ -110,9 +144,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
         at[j] = (j * team.lanes + team.lane) * kVec;
-        const Vec<W> vw = load_vec(static_cast<const W*>(x.weight), at[j], dim);
-        Vec<W> vb{};
-        if (x.bias) vb = load_vec(static_cast<const W*>(x.bias), at[j], dim);
+        const Vec<W, kVec> vw = load_vec<kVec>(static_cast<const W*>(x.weight), at[j], dim);
+        Vec<W, kVec> vb{};
+        if (x.bias) vb = load_vec<kVec>(static_cast<const W*>(x.bias), at[j], dim);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
             w[j][e] = to_f32(vw.v[e]);
@@ -123,9 +157,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     int64_t r = static_cast<int64_t>(blockIdx.x) * team.slots + team.slot;
     if (r >= x.rows) return;  // a lane group of its own; a workgroup's first row is there
     const T* in = static_cast<const T*>(x.x);
-    Vec<T> next[kVecs];
+    Vec<T, kVec> next[kVecs];
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) next[j] = load_vec(in + r * x.x_stride, at[j], dim);
+    for (int j = 0; j < kVecs; ++j) next[j] = load_vec<kVec>(in + r * x.x_stride, at[j], dim);
     for (; r < x.rows; r += step) {
         float h[kVecs][kVec];
         float2 s{0.f, 0.f};
@@ -138,7 +172,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
             }
         if (r + step < x.rows) {
 #pragma unroll
-            for (int j = 0; j < kVecs; ++j) next[j] = load_vec(in + (r + step) * x.x_stride, at[j], dim);
+            for (int j = 0; j < kVecs; ++j) next[j] = load_vec<kVec>(in + (r + step) * x.x_stride, at[j], dim);
         }
         const float mean = x.center ? team.sum(s).x / n : 0.f;
         float2 q{0.f, 0.f};
@@ -168,7 +202,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
 // dx, and with kWeight a workgroup's part of the weights' gradients.
 template <typename T, typename W, int kGroup, int kVecs, bool kWeight>
 __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_args x, float* parts) {
-    __shared__ float2 red[2 * (kNormThreads / 64)];
+    __shared__ __align__(16) float2 red[2 * kMostWaves];
+    constexpr int kVec = vec_of<T>;
     __shared__ float over[kWeight && kGroup ? kNormThreads * kVec : 1];
     Team<kGroup> team(red);
     const int dim = x.dim;
@@ -178,7 +213,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
         at[j] = (j * team.lanes + team.lane) * kVec;
-        const Vec<W> vw = load_vec(static_cast<const W*>(x.weight), at[j], dim);
+        const Vec<W, kVec> vw = load_vec<kVec>(static_cast<const W*>(x.weight), at[j], dim);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
             w[j][e] = to_f32(vw.v[e]);
@@ -189,28 +224,37 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
     int64_t r = static_cast<int64_t>(blockIdx.x) * team.slots + team.slot;
     const T* in = static_cast<const T*>(x.x);
     const T* dy = static_cast<const T*>(x.dy);
-    Vec<T> nx[kVecs], ny[kVecs];
-    float nmean = 0.f, nrstd = 0.f;
+    struct Row {
+        Vec<T, kVec> x[kVecs], y[kVecs];
+        float mean, rstd;
+    };
+    Row next{};
+    // A row's statistics by vector loads, which are waited for where they are used:
+    // scalar ones would be waited for with the next sum's LDS, a memory's latency a row.
+    int lane_zero;
+    asm volatile("v_mov_b32 %0, 0" : "=v"(lane_zero));
+    const float *mean_of = x.mean + lane_zero, *rstd_of = x.rstd + lane_zero;
     auto fetch = [&](int64_t row) {
+        if (row >= x.rows) return;
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
-            nx[j] = load_vec(in + row * x.x_stride, at[j], dim);
-            ny[j] = load_vec(dy + row * x.dy_stride, at[j], dim);
+            next.x[j] = load_vec<kVec>(in + row * x.x_stride, at[j], dim);
+            next.y[j] = load_vec<kVec>(dy + row * x.dy_stride, at[j], dim);
         }
-        nmean = x.center ? x.mean[row] : 0.f;
-        nrstd = x.rstd[row];
+        next.mean = x.center ? mean_of[row] : 0.f;
+        next.rstd = rstd_of[row];
     };
-    if (r < x.rows) fetch(r);
+    fetch(r);
     for (; r < x.rows; r += step) {
-        const float mean = nmean, rstd = nrstd;
+        const float mean = next.mean, rstd = next.rstd;
         float h[kVecs][kVec], a[kVecs][kVec];
         float2 s{0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-                const float g = to_f32(ny[j].v[e]);
-                h[j][e] = (to_f32(nx[j].v[e]) - mean) * rstd;
+                const float g = to_f32(next.y[j].v[e]);
+                h[j][e] = (to_f32(next.x[j].v[e]) - mean) * rstd;
                 a[j][e] = g * w[j][e];
                 s.x += a[j][e];
                 s.y = fmaf(a[j][e], h[j][e], s.y);
@@ -219,7 +263,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
                     sb[j][e] += g;
                 }
             }
-        if (r + step < x.rows) fetch(r + step);
+        fetch(r + step);
         if (!x.dx) continue;
         s = team.sum(s);
         const float sa = x.center ? s.x * inv : 0.f, sx = s.y * inv;
@@ -381,34 +425,39 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dw_kernel(ge_norm_args
 struct NormPlan {
     int group, vecs, threads, slots;
 };
-NormPlan norm_plan(int dim) {
-    const int vectors = (dim + kVec - 1) / kVec;
+NormPlan norm_plan(int dim, int vec) {
+    const int vectors = (dim + vec - 1) / vec;
     NormPlan p{0, 1, 0, 1};
     if (dim <= kGroupDim) {
-        p.vecs = vectors > 64 ? 2 : 1;
+        while (p.vecs * 64 < vectors) p.vecs *= 2;
         p.group = 8;
         while (p.group * p.vecs < vectors) p.group *= 2;
         p.threads = kNormThreads;
         p.slots = p.threads / p.group;
         return p;
     }
-    p.vecs = vectors > kNormThreads ? 2 : 1;
+    while (p.vecs * kNormThreads < vectors) p.vecs *= 2;
     p.threads = ((vectors + p.vecs - 1) / p.vecs + 63) / 64 * 64;
     return p;
 }
 
 // Calls f with the plan's group and vectors as constants.
-template <typename F>
+template <typename T, typename F>
 void with_plan(const NormPlan& p, F f) {
     using std::integral_constant;
-    auto one = integral_constant<int, 1>{};
-    auto two = integral_constant<int, 2>{};
+    constexpr integral_constant<int, 1> one{};
+    constexpr integral_constant<int, 2> two{};
+    constexpr integral_constant<int, 4> four{};
     if (p.group == 8) return f(integral_constant<int, 8>{}, one);
     if (p.group == 16) return f(integral_constant<int, 16>{}, one);
     if (p.group == 32) return f(integral_constant<int, 32>{}, one);
-    if (p.group == 64) return p.vecs == 1 ? f(integral_constant<int, 64>{}, one) : f(integral_constant<int, 64>{}, two);
-    auto all = integral_constant<int, 0>{};
-    return p.vecs == 1 ? f(all, one) : f(all, two);
+    auto by_vecs = [&](auto group) {
+        if (p.vecs == 1) return f(group, one);
+        if (sizeof(T) == 2 || p.vecs == 2) return f(group, two);
+        if constexpr (sizeof(T) == 4) f(group, four);
+    };
+    if (p.group == 64) return by_vecs(integral_constant<int, 64>{});
+    by_vecs(integral_constant<int, 0>{});
 }
 
 template <typename T, typename W>
@@ -417,9 +466,9 @@ void norm_forward(const ge_norm_args& x, hipStream_t st) {
         norm_long_kernel<T, W><<<x.rows, kLongThreads, 0, st>>>(x);
         return;
     }
-    const NormPlan p = norm_plan(x.dim);
+    const NormPlan p = norm_plan(x.dim, vec_of<T>);
     const unsigned blocks = std::min((x.rows + p.slots - 1) / p.slots, kNormBlocks);
-    with_plan(p, [&](auto group, auto vecs) {
+    with_plan<T>(p, [&](auto group, auto vecs) {
         norm_kernel<T, W, decltype(group)::value, decltype(vecs)::value><<<blocks, p.threads, 0, st>>>(x);
     });
 }
@@ -436,9 +485,9 @@ void norm_backward(const ge_norm_args& x, const Buffers& b, hipStream_t st) {
         }
         if (x.dx && x.rows > 0) norm_long_dx_kernel<T, W><<<x.rows, kLongThreads, 0, st>>>(x);
     } else if (x.rows > 0) {
-        const NormPlan p = norm_plan(x.dim);
+        const NormPlan p = norm_plan(x.dim, vec_of<T>);
         parts = std::min((x.rows + p.slots - 1) / p.slots, kNormParts);
-        with_plan(p, [&](auto group, auto vecs) {
+        with_plan<T>(p, [&](auto group, auto vecs) {
             constexpr int g = decltype(group)::value, v = decltype(vecs)::value;
             if (weight)
                 norm_backward_kernel<T, W, g, v, true><<<parts, p.threads, 0, st>>>(x, b.norm);
