@@ -53,8 +53,6 @@ struct Tile32 {
     const char* base;
     int64_t left;
     int64_t step;
-    int64_t span;             // bytes from `base` to the end of the tile
-    bool whole;               // the operand ends between two 16-byte loads
     u32x4 raw[kPerThread];
 
     __device__ __forceinline__ void init(const Operand& o, int row0, int first) {
@@ -62,8 +60,6 @@ struct Tile32 {
         const int64_t skip = (kAlong ? static_cast<int64_t>(row0) * o.ld : row0) * 4 + step * first;
         base = static_cast<const char*>(o.p) + skip;
         left = o.end * 4 - skip;
-        span = ((kAlong ? kRows : kStepK32) - 1) * o.ld * 4 + (kAlong ? kStepK32 : kRows) * 4;
-        whole = o.ld % 4 == 0 && left % 16 == 0;
         kpos = (threadIdx.x & 7) * 4;
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
@@ -83,15 +79,9 @@ struct Tile32 {
     __device__ __forceinline__ void load(int k_left) {
         const int64_t n = left < 0 ? 0 : left > 0x7ffffff0 ? 0x7ffffff0 : left;
         __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(n), 0x00027000);
-        if (whole || left >= span) {
+        // bounds are checked element by element
 #pragma unroll
-            for (int i = 0; i < kPerThread; ++i) raw[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(voff[i]), 0, 0));
-        } else {  // a load that runs over the end gives zeros alone: the last ones in single elements
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) raw[i][e] = __builtin_amdgcn_raw_buffer_load_b32(rs, static_cast<int>(voff[i]) + e * 4, 0, 0);
-        }
+        for (int i = 0; i < kPerThread; ++i) raw[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(voff[i]), 0, 0));
         base += step;
         left -= step;
         if (kAlong && k_left < kStepK32) {

@@ -16,7 +16,8 @@
 // on the order in which workgroups run.
 //
 // Both passes are bound by memory. 16,384 rows of 2,816 bf16 channels: forward
-// 41 us (4.5 TB/s), backward 89 us (3.1 TB/s) + 4 us for the second launch.
+// 39 us (4.7 TB/s), backward 65 us (4.3 TB/s) + 4 us for the second launch; a large
+// copy moves 4.8 TB/s. Two or three rows ahead, or more workgroups, are no faster.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -66,6 +67,43 @@ __device__ __forceinline__ void store_vec(T* row, int i, int dim, const float (&
     }
 }
 
+// The vectors of a row at at[0], at[1], ... kWhole: by buffer loads and stores of
+// the row, whose bounds are checked by the hardware four bytes at a time; without
+// branches the compiler knows how many are in flight, and the next row's loads are
+// not waited for together with this row's stores. The row is then the same in the
+// whole wave, and its length a multiple of four bytes.
+template <bool kWhole, int kVec, int kVecs, typename T>
+__device__ __forceinline__ void load_row(const T* p, int64_t stride, int64_t r, int64_t rows, int dim, const int (&at)[kVecs],
+                                         Vec<T, kVec> (&to)[kVecs]) {
+    if constexpr (kWhole) {
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p + r * stride), 0,
+                                                                      r < rows ? dim * static_cast<int>(sizeof(T)) : 0, 0x00027000);
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j)
+            to[j] = __builtin_bit_cast(Vec<T, kVec>, __builtin_amdgcn_raw_buffer_load_b128(rs, at[j] * static_cast<int>(sizeof(T)), 0, 0));
+    } else if (r < rows) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) to[j] = load_vec<kVec>(p + r * stride, at[j], dim);
+    }
+}
+template <bool kWhole, int kVec, int kVecs, typename T>
+__device__ __forceinline__ void store_row(T* p, int64_t stride, int64_t r, int dim, const int (&at)[kVecs], const float (&x)[kVecs][kVec]) {
+    if constexpr (kWhole) {
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(p + r * stride, 0, dim * static_cast<int>(sizeof(T)), 0x00027000);
+        using Words = decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0));
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            Vec<T, kVec> v;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v.v[e] = from_f32<T>(x[j][e]);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, v), rs, at[j] * static_cast<int>(sizeof(T)), 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) store_vec(p + r * stride, at[j], dim, x[j]);
+    }
+}
+
 // Sum over groups of kLanes lanes, the same in each of them. Steps within 16 lanes
 // are modifiers of the addition, the others swap rows of lanes between registers:
 // nothing passes LDS, whose six round trips a sum took longer than a row's loads.
@@ -105,6 +143,7 @@ struct Team {
         lanes = kGroup ? kGroup : blockDim.x;
         lane = kGroup ? threadIdx.x % (kGroup ? kGroup : 1) : threadIdx.x;
         slot = kGroup ? threadIdx.x / (kGroup ? kGroup : 1) : 0;
+        if (kGroup == 64) slot = __builtin_amdgcn_readfirstlane(slot);
         slots = kGroup ? blockDim.x / (kGroup ? kGroup : 1) : 1;
         if (!kGroup) {  // waves that are not there add nothing
             if (threadIdx.x < 2 * kMostWaves) red[threadIdx.x] = make_float2(0.f, 0.f);
@@ -132,7 +171,7 @@ struct Team {
     }
 };
 
-template <typename T, typename W, int kGroup, int kVecs>
+template <typename T, typename W, int kGroup, int kVecs, bool kWhole>
 __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     __shared__ __align__(16) float2 red[2 * kMostWaves];
     constexpr int kVec = vec_of<T>;
@@ -158,8 +197,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     if (r >= x.rows) return;  // a lane group of its own; a workgroup's first row is there
     const T* in = static_cast<const T*>(x.x);
     Vec<T, kVec> next[kVecs];
-#pragma unroll
-    for (int j = 0; j < kVecs; ++j) next[j] = load_vec<kVec>(in + r * x.x_stride, at[j], dim);
+    load_row<kWhole>(in, x.x_stride, r, x.rows, dim, at, next);
     for (; r < x.rows; r += step) {
         float h[kVecs][kVec];
         float2 s{0.f, 0.f};
@@ -170,10 +208,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
                 h[j][e] = to_f32(next[j].v[e]);
                 s.x += h[j][e];
             }
-        if (r + step < x.rows) {
-#pragma unroll
-            for (int j = 0; j < kVecs; ++j) next[j] = load_vec<kVec>(in + (r + step) * x.x_stride, at[j], dim);
-        }
+        load_row<kWhole>(in, x.x_stride, r + step, x.rows, dim, at, next);
         const float mean = x.center ? team.sum(s).x / n : 0.f;
         float2 q{0.f, 0.f};
 #pragma unroll
@@ -184,14 +219,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
                 if (at[j] + e < dim) q.x = fmaf(h[j][e], h[j][e], q.x);
             }
         const float rstd = 1.0f / sqrtf(team.sum(q).x / n + x.eps);
-        T* out = static_cast<T*>(x.y) + r * x.y_stride;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            float y[kVec];
+        for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) y[e] = fmaf(h[j][e] * rstd, w[j][e], b[j][e]);
-            store_vec(out, at[j], dim, y);
-        }
+            for (int e = 0; e < kVec; ++e) h[j][e] = fmaf(h[j][e] * rstd, w[j][e], b[j][e]);
+        store_row<kWhole>(static_cast<T*>(x.y), x.y_stride, r, dim, at, h);
         if (team.lane == 0) {
             x.rstd[r] = rstd;
             if (x.mean) x.mean[r] = mean;
@@ -200,7 +232,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
 }
 
 // dx, and with kWeight a workgroup's part of the weights' gradients.
-template <typename T, typename W, int kGroup, int kVecs, bool kWeight>
+template <typename T, typename W, int kGroup, int kVecs, bool kWhole, bool kWeight>
 __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_args x, float* parts) {
     __shared__ __align__(16) float2 red[2 * kMostWaves];
     constexpr int kVec = vec_of<T>;
@@ -234,15 +266,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
     int lane_zero;
     asm volatile("v_mov_b32 %0, 0" : "=v"(lane_zero));
     const float *mean_of = x.mean + lane_zero, *rstd_of = x.rstd + lane_zero;
-    auto fetch = [&](int64_t row) {
-        if (row >= x.rows) return;
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            next.x[j] = load_vec<kVec>(in + row * x.x_stride, at[j], dim);
-            next.y[j] = load_vec<kVec>(dy + row * x.dy_stride, at[j], dim);
-        }
-        next.mean = x.center ? mean_of[row] : 0.f;
-        next.rstd = rstd_of[row];
+    auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+        load_row<kWhole>(in, x.x_stride, row, x.rows, dim, at, next.x);
+        load_row<kWhole>(dy, x.dy_stride, row, x.rows, dim, at, next.y);
+        const int64_t last = min(row, static_cast<int64_t>(x.rows) - 1);
+        next.mean = x.center ? mean_of[last] : 0.f;
+        next.rstd = rstd_of[last];
     };
     fetch(r);
     for (; r < x.rows; r += step) {
@@ -267,14 +296,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
         if (!x.dx) continue;
         s = team.sum(s);
         const float sa = x.center ? s.x * inv : 0.f, sx = s.y * inv;
-        T* dx = static_cast<T*>(x.dx) + r * x.dx_stride;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            float o[kVec];
+        for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) o[e] = rstd * (a[j][e] - sa - h[j][e] * sx);
-            store_vec(dx, at[j], dim, o);
-        }
+            for (int e = 0; e < kVec; ++e) a[j][e] = rstd * (a[j][e] - sa - h[j][e] * sx);
+        store_row<kWhole>(static_cast<T*>(x.dx), x.dx_stride, r, dim, at, a);
     }
     if constexpr (kWeight) {
         float* p = parts + static_cast<int64_t>(blockIdx.x) * 2 * dim;
@@ -441,23 +467,27 @@ NormPlan norm_plan(int dim, int vec) {
     return p;
 }
 
-// Calls f with the plan's group and vectors as constants.
+// Calls f with the plan's group and vectors and whether rows are whole as constants.
 template <typename T, typename F>
-void with_plan(const NormPlan& p, F f) {
+void with_plan(const NormPlan& p, int dim, F f) {
     using std::integral_constant;
+    constexpr std::false_type no{};
     constexpr integral_constant<int, 1> one{};
-    constexpr integral_constant<int, 2> two{};
-    constexpr integral_constant<int, 4> four{};
-    if (p.group == 8) return f(integral_constant<int, 8>{}, one);
-    if (p.group == 16) return f(integral_constant<int, 16>{}, one);
-    if (p.group == 32) return f(integral_constant<int, 32>{}, one);
-    auto by_vecs = [&](auto group) {
-        if (p.vecs == 1) return f(group, one);
-        if (sizeof(T) == 2 || p.vecs == 2) return f(group, two);
-        if constexpr (sizeof(T) == 4) f(group, four);
+    if (p.group == 8) return f(integral_constant<int, 8>{}, one, no);
+    if (p.group == 16) return f(integral_constant<int, 16>{}, one, no);
+    if (p.group == 32) return f(integral_constant<int, 32>{}, one, no);
+    auto by_vecs = [&](auto group, auto whole) {
+        if (p.vecs == 1) return f(group, one, whole);
+        if (sizeof(T) == 2 || p.vecs == 2) return f(group, integral_constant<int, 2>{}, whole);
+        if constexpr (sizeof(T) == 4) f(group, integral_constant<int, 4>{}, whole);
     };
-    if (p.group == 64) return by_vecs(integral_constant<int, 64>{});
-    by_vecs(integral_constant<int, 0>{});
+    auto by_group = [&](auto whole) {
+        if (p.group == 64) return by_vecs(integral_constant<int, 64>{}, whole);
+        by_vecs(integral_constant<int, 0>{}, whole);
+    };
+    if constexpr (sizeof(T) == 4) return by_group(std::true_type{});
+    if (dim % 2 == 0) return by_group(std::true_type{});
+    by_group(no);
 }
 
 template <typename T, typename W>
@@ -468,8 +498,8 @@ void norm_forward(const ge_norm_args& x, hipStream_t st) {
     }
     const NormPlan p = norm_plan(x.dim, vec_of<T>);
     const unsigned blocks = std::min((x.rows + p.slots - 1) / p.slots, kNormBlocks);
-    with_plan<T>(p, [&](auto group, auto vecs) {
-        norm_kernel<T, W, decltype(group)::value, decltype(vecs)::value><<<blocks, p.threads, 0, st>>>(x);
+    with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto whole) {
+        norm_kernel<T, W, decltype(group)::value, decltype(vecs)::value, decltype(whole)::value><<<blocks, p.threads, 0, st>>>(x);
     });
 }
 
@@ -487,12 +517,13 @@ void norm_backward(const ge_norm_args& x, const Buffers& b, hipStream_t st) {
     } else if (x.rows > 0) {
         const NormPlan p = norm_plan(x.dim, vec_of<T>);
         parts = std::min((x.rows + p.slots - 1) / p.slots, kNormParts);
-        with_plan<T>(p, [&](auto group, auto vecs) {
+        with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto whole) {
             constexpr int g = decltype(group)::value, v = decltype(vecs)::value;
+            constexpr bool w = decltype(whole)::value;
             if (weight)
-                norm_backward_kernel<T, W, g, v, true><<<parts, p.threads, 0, st>>>(x, b.norm);
+                norm_backward_kernel<T, W, g, v, w, true><<<parts, p.threads, 0, st>>>(x, b.norm);
             else if (x.dx)
-                norm_backward_kernel<T, W, g, v, false><<<parts, p.threads, 0, st>>>(x, b.norm);
+                norm_backward_kernel<T, W, g, v, w, false><<<parts, p.threads, 0, st>>>(x, b.norm);
         });
     }
     if (weight) {
