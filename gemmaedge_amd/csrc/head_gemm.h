@@ -234,7 +234,7 @@ __device__ __forceinline__ void product(f32x4& c, bf16x8 a, bf16x8 b) {
 // One workgroup's tile of kBm x kBn, kWavesM x kWavesN waves. Epi: see the callers;
 // it gets acc[mt][nt], whose element j is row epi_row(mt, 4 * (lane / 16) + j)
 // (A along k) or mt * 16 + 4 * (lane / 16) + j (across k) of the wave's rows and
-// column nt * 16 + lane % 16 of its columns.
+// column nt * 16 + lane % 16 of its columns. `prepare` loads what it needs of them.
 template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, bool kBAlong, typename Epi>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g, Epi epi) {
     constexpr int kWaves = kWavesM * kWavesN;
@@ -247,27 +247,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const TilePlace place = tile_place(g, blockIdx.x, gridDim.x);
-    const int m0 = place.m * kBm, n0 = place.n * kBn;
     const int wm = wave % kWavesM, wn = wave / kWavesM;
-
-    const int steps = (g.k + kStepK - 1) / kStepK;
-    const int first = place.split * g.steps_per_split;
-    const int last = min(steps, first + g.steps_per_split);
-    const int total = max(0, last - first);
     using LoaderA = TileLoader<kBm, kAAlong, true, kWaves>;
     using LoaderB = TileLoader<kBn, kBAlong, false, kWaves>;
     LoaderA la;
     LoaderB lb;
-    la.init(g.a, m0, first, wave, lane);
-    lb.init(g.b, n0, first, wave, lane);
-
     f32x4 acc[kMt][kNt];
-#pragma unroll
-    for (int i = 0; i < kMt; ++i)
-#pragma unroll
-        for (int j = 0; j < kNt; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     typename std::conditional<kAAlong, FragAlong<true>, FragAcross<kBm, kMt>>::type fra;
     typename std::conditional<kBAlong, FragAlong<false>, FragAcross<kBn, kNt>>::type frb;
     fra.init(wm * kWm, lane);
@@ -278,7 +263,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
     constexpr int kProducts = kMt * kNt;
     constexpr bool kInPlace = kProducts >= 32;
     // Loads of steps past the end bring zeros, whose products change nothing.
-    int load_left = total, k_left = g.k - first * kStepK;
+    int load_left, k_left;
     __amdgpu_buffer_rsrc_t ra, rb;
     auto mask = [&]() __attribute__((always_inline)) {
         if (k_left < kStepK) {
@@ -358,8 +343,20 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
         arrive();
         half(upper, stage, next);
     };
+    const TilePlace place = tile_place(g, blockIdx.x, gridDim.x);
+    const int m0 = place.m * kBm, n0 = place.n * kBn;
+    const int first = place.split * g.steps_per_split;
+    const int total = max(0, min((g.k + kStepK - 1) / kStepK, first + g.steps_per_split) - first);
+    load_left = total;
+    k_left = g.k - first * kStepK;
+    la.init(g.a, m0, first, wave, lane);
+    lb.init(g.b, n0, first, wave, lane);
     load_all(s0);
     load_all(s1);
+#pragma unroll
+    for (int i = 0; i < kMt; ++i)
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     arrive();
 #pragma unroll
     for (int i = 0; i < kMt + kNt; ++i) fetch(i, 0, s0);
@@ -372,10 +369,10 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
         // done (16 cycles); what reads the accumulators comes behind the loop.
         if (kInPlace) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
     }
-    // The epilogue may use LDS: nothing is on its way there any more.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    epi.template finish<kBm, kBn, kWavesM, kWavesN, kAAlong>(acc, m0, n0, place, wm, wn, lane, wave, reinterpret_cast<char*>(s0));
+    // Every wave is done with the stages, and nothing is on its way there any more.
+    arrive();
+    auto state = epi.template prepare<kWm, kNt>(m0 + wm * kWm, n0 + wn * kWn, lane);
+    epi.template finish<kBm, kBn, kWavesM, kWavesN, kAAlong>(acc, state, m0, n0, place, wm, wn, lane, reinterpret_cast<float2*>(s0));
 }
 
 }  // namespace head

@@ -184,7 +184,8 @@ __global__ __launch_bounds__(256, 2) void gemm32_kernel(GemmArgs g, Epi epi) {
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[kPairs[s][0]][i], fb[kPairs[s][1]][j], acc[i][j], 0, 0, 0);
         __syncthreads();
     }
-    epi.template finish<kBm, kBn, kWavesM, kWavesN, kAAlong>(acc, m0, n0, place, wm, wn, lane, wave, reinterpret_cast<char*>(lds));
+    auto state = epi.template prepare<kWm, kNt>(m0 + wm * kWm, n0 + wn * kWn, lane);
+    epi.template finish<kBm, kBn, kWavesM, kWavesN, kAAlong>(acc, state, m0, n0, place, wm, wn, lane, reinterpret_cast<float2*>(lds));
 }
 
 }  // namespace head

@@ -74,15 +74,23 @@ struct StatsEpi {
     float2* stats;   // [rows][ld]
     int ld, tile0;
 
+    template <int kNt>
+    struct State {
+        int t[kNt];
+    };
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State<kNt> prepare(int, int col0, int lane) const {
+        State<kNt> s;
+        load_targets(targets, col0 + (lane & 15), rows, v0, vocab, s.t);
+        return s;
+    }
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
-                                           int wave, char* lds) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State<kNt>& s, int m0, int n0, TilePlace place, int wm, int wn,
+                                           int lane, float2* part) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
-        float2* part = reinterpret_cast<float2*>(lds);  // [kWavesM][kBn]
         const int row0 = m0 + wm * kWm;
         const int n_first = n0 + wn * kWn + (lane & 15);
-        int t[kNt];
-        load_targets(targets, n_first, rows, v0, vocab, t);
+        const int(&t)[kNt] = s.t;
         const bool tail = row0 + kWm > vocab;
         const bool simple = kFast && sc.bounded() && !tail;
         if (!simple && sc.cap > 0.f) {
@@ -232,35 +240,44 @@ struct GradEpi {
         return (exp2_fast((l - lse) * kLog2e) - one) * fmaf(-y, y, 1.0f) * g;
     }
 
+    template <int kNt>
+    struct State {
+        int t[kNt];
+        float lse[kNt], grad[kNt], unit;
+    };
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State<kNt> prepare(int, int col0, int lane) const {
+        State<kNt> s;
+        load_targets(targets, col0 + (lane & 15), rows, 0, vocab_all, s.t);
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            const int n = min(col0 + (lane & 15) + j * 16, rows - 1);
+            s.lse[j] = lse[n];
+            s.grad[j] = grad[n];
+        }
+        s.unit = *unit;
+        return s;
+    }
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
-                                           int wave, char* lds) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State<kNt>& s, int m0, int n0, TilePlace place, int wm, int wn,
+                                           int lane, float2* part) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm;
         const int n_first = n0 + wn * kWn + (lane & 15);
-        int t[kNt];
         float ls[kNt], gr[kNt];
-        load_targets(targets, n_first, rows, 0, vocab_all, t);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
-            const int n = min(n_first + j * 16, rows - 1);
-            ls[j] = lse[n];
-            gr[j] = grad[n];
-        }
-        const float u = *unit;
-#pragma unroll
-        for (int j = 0; j < kNt; ++j) {
-            float g = gr[j] / u;
+            ls[j] = s.lse[j];
+            gr[j] = s.grad[j] / s.unit;
             if (kFast) {
                 ls[j] = sc.cap > 0.f ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
-                if (sc.cap > 0.f) g *= 4.0f;
+                if (sc.cap > 0.f) gr[j] *= 4.0f;
             }
-            gr[j] = g;
         }
         if (sc.cap > 0.f)
-            store<kWm, true>(acc, row0, n_first, lane, t, ls, gr);
+            store<kWm, true>(acc, row0, n_first, lane, s.t, ls, gr);
         else
-            store<kWm, false>(acc, row0, n_first, lane, t, ls, gr);
+            store<kWm, false>(acc, row0, n_first, lane, s.t, ls, gr);
     }
     template <int kWm, bool kCap, int kMt, int kNt>
     __device__ __forceinline__ void store(f32x4 (&acc)[kMt][kNt], int row0, int n_first, int lane, const int (&t)[kNt],
@@ -310,21 +327,28 @@ struct HiddenEpi {
     int dim, rows;
     bool add;
 
+    struct State {};
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State prepare(int, int, int) const { return {}; }
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
-                                           int wave, char* lds) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State& s, int m0, int n0, TilePlace place, int wm, int wn,
+                                           int lane, float2* part) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             const int n = n0 + wn * kWn + j * 16 + (lane & 15);
             if (n >= rows) continue;
+            float* o = out + place.split * split + n * ld;
+            const int d0 = m0 + wm * kWm + 4 * (lane >> 4);
+            f32x4 sum[kMt];
 #pragma unroll
-            for (int i = 0; i < kMt; ++i) {
-                const int d = m0 + wm * kWm + i * 16 + 4 * (lane >> 4);
-                if (d >= dim) continue;  // ld is a multiple of 4 above dim
-                f32x4* o = reinterpret_cast<f32x4*>(out + place.split * split + n * ld + d);
-                *o = add ? *o + acc[i][j] : acc[i][j];
+            for (int i = 0; i < kMt; ++i) {  // ld is a multiple of 4 above dim
+                sum[i] = acc[i][j];
+                if (add && d0 + i * 16 < dim) sum[i] += *reinterpret_cast<const f32x4*>(o + d0 + i * 16);
             }
+#pragma unroll
+            for (int i = 0; i < kMt; ++i)
+                if (d0 + i * 16 < dim) *reinterpret_cast<f32x4*>(o + d0 + i * 16) = sum[i];
         }
     }
 };
@@ -337,11 +361,16 @@ struct WeightEpi {
     bool vec;  // rows take 4-element stores
     const float* unit;
 
+    struct State {
+        float unit;
+    };
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State prepare(int, int, int) const { return {*unit}; }
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
-    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], int m0, int n0, TilePlace place, int wm, int wn, int lane,
-                                           int wave, char* lds) const {
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State& s, int m0, int n0, TilePlace place, int wm, int wn,
+                                           int lane, float2* part) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
-        const float u = *unit;
+        const float u = s.unit;
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             const int v = n0 + wn * kWn + j * 16 + (lane & 15);
@@ -446,11 +475,11 @@ struct Call {
         g.steps_per_split = ((g.k + kStep - 1) / kStep + splits - 1) / splits;
         g.splits = splits;
         g.group_m = group;
-        const unsigned blocks = static_cast<unsigned>(g.tiles_m) * g.tiles_n * g.splits;
+        const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
         if constexpr (sizeof(T) == 4)
-            gemm32_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 256, 0, st>>>(g, e);
+            gemm32_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<static_cast<unsigned>(tiles), 256, 0, st>>>(g, e);
         else
-            gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<blocks, 256, 0, st>>>(g, e);
+            gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<static_cast<unsigned>(tiles), 256, 0, st>>>(g, e);
     }
     template <typename Epi>
     void logits(const Operand& w, const Operand& h, int n, const Epi& e) const {

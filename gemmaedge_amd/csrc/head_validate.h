@@ -14,6 +14,7 @@
 namespace ge {
 namespace head {
 
+constexpr int kUnits = 256;       // compute units
 constexpr int kTileM = 256;       // vocabulary (or channels) of a large tile
 constexpr int kTile32 = 128;      // of a tile of float32 operands
 constexpr int kSmallRows = 64;    // batches up to this take the small tiles
@@ -190,7 +191,7 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
         // Parts of the sum over the piece: 256 tiles run at a time, one on each compute
         // unit (512 of float32, two on each); a part costs its steps and about 12 more
         // for its beginning and for adding what it has.
-        const int64_t tile = c.dtype == GE_DTYPE_F32 ? kTile32 : 256, slots = c.dtype == GE_DTYPE_F32 ? 512 : 256;
+        const int64_t tile = c.dtype == GE_DTYPE_F32 ? kTile32 : 256, slots = c.dtype == GE_DTYPE_F32 ? 2 * kUnits : kUnits;
         const int64_t tiles = (x.rows + tile - 1) / tile * ((x.dim + tile - 1) / tile);
         const int64_t steps = plan.piece / 64;
         const int64_t most_bytes = 4 * std::max<int64_t>(x.rows, 1) * round_up(x.dim, 4);
