@@ -488,6 +488,8 @@ struct Call {
         if constexpr (sizeof(T) == 4) {
             if (plan.tile_n == 32)
                 run<128, 32, 4, 1, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else if (plan.tile_n == 64)
+                run<128, 64, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
             else if (plan.tile_n == 96)
                 run<128, 96, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
             else
