@@ -410,13 +410,23 @@ __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int
     out[r * out_ld + d] = from_f32<T>(s * *unit);
 }
 
-// Rows into rows that are `kpad` long, zeros behind `dim`.
+// Rows into rows that are `kpad` long (a multiple of 8), zeros behind `dim`: 8
+// elements a thread, read at any address, written aligned.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, int dim, int kpad, T* out) {
-    const int d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= kpad) return;
-    const int64_t r = blockIdx.y;
-    out[r * kpad + d] = d < dim ? in[r * ld + d] : T(0);
+__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, unsigned rows, int dim, int kpad, T* out) {
+    const int d = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    const int64_t r = blockIdx.y * blockDim.y + threadIdx.y;
+    if (d >= kpad || r >= rows) return;
+    struct Vec {
+        T v[8];
+    } x;
+    if (d + 8 <= dim) {
+        __builtin_memcpy(&x, in + r * ld + d, sizeof(x));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] = d + e < dim ? in[r * ld + d + e] : T(0);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(out + r * kpad + d, 16), &x, sizeof(x));
 }
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, int64_t ld, int dim) {
@@ -432,9 +442,13 @@ void for_rows(int64_t rows, F launch) {
 
 template <typename T>
 void pack(const T* in, int64_t ld, int64_t rows, int dim, int64_t kpad, T* out, hipStream_t st) {
+    const unsigned units = static_cast<unsigned>(kpad / 8);
+    unsigned tx = 8;
+    while (tx < units && tx < 256) tx *= 2;
+    const unsigned ty = 256 / tx;
     for_rows(rows, [&](int64_t r, unsigned n) {
-        pack_kernel<T><<<dim3(static_cast<unsigned>((kpad + 255) / 256), n), 256, 0, st>>>(in + r * ld, ld, dim, static_cast<int>(kpad),
-                                                                                out + r * kpad);
+        pack_kernel<T><<<dim3((units + tx - 1) / tx, (n + ty - 1) / ty), dim3(tx, ty), 0, st>>>(in + r * ld, ld, n, dim, static_cast<int>(kpad),
+                                                                                               out + r * kpad);
     });
 }
 
@@ -496,6 +510,8 @@ struct Call {
                 run<128, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
         } else if (plan.tile_n == kSmallTileN) {
             run<kSmallTileM, kSmallTileN, 4, 1, true, true>(w, h, k, n, x.rows, 1, 4, e);
+        } else if (plan.tile_n == 128) {
+            run<256, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
         } else {
             run<256, 256, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
         }
@@ -531,7 +547,10 @@ struct Call {
             const Operand dz{b.dlogits, ld, x.rows * ld};
             if (dh) {
                 HiddenEpi he{b.dhidden, hld, split, x.dim, x.rows, v0 > 0};
-                run<kTile, kTile, 2, 2, false, true>(w, dz, n, x.dim, x.rows, splits, 6, he);
+                if (sizeof(T) == 2 && x.rows <= 128)
+                    run<kTile, 128, 2, 2, false, true>(w, dz, n, x.dim, x.rows, splits, 6, he);
+                else
+                    run<kTile, kTile, 2, 2, false, true>(w, dz, n, x.dim, x.rows, splits, 6, he);
             }
             if (dw) {
                 WeightEpi<T> we{dw + v0 * dw_ld, dw_ld, x.dim, n, false, unit};
