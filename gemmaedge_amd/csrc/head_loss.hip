@@ -194,9 +194,9 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* stats, int ld, 
     }
 }
 
-// The largest finite |grad| of the rows that carry a loss, 1 if there is none. The
-// logits' gradient is held in units of it: where all rows weigh the same, as in
-// a mean, the factor's own rounding to 8 bits would scale whole gradients.
+// The mantissa of the largest finite |grad| of the rows that carry a loss, 1 if there
+// is none. The logits' gradient is held in units of it: where all rows weigh the
+// same, as in a mean, the weight's own rounding to 8 bits would scale whole gradients.
 __global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, const int32_t* targets, int rows, int vocab, float* unit) {
     __shared__ float red[16];
     float m = 0.f;
@@ -211,7 +211,8 @@ __global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, cons
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
-    *unit = m > 0.f ? m : 1.f;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, m);
+    *unit = m >= 0x1p-126f ? __builtin_bit_cast(float, (bits & 0x007fffffu) | 0x3f800000u) : 1.f;
 }
 
 template <typename T>
