@@ -11,6 +11,11 @@
 // (Planes written to memory by a launch before cost 3 bytes more an element than the
 // operand has, and each fragment was read twice.) Two workgroups share a compute unit: one splits and
 // waits while the other multiplies, so one stage of LDS is enough.
+//
+// 1,000 rows, width 1,000, vocabulary 50,257: 187 TFLOP/s of float32 products, 1.15
+// PFLOP/s of the matrix cores; 300 rows, width 768: 140 with the rows that pad its
+// tiles. Keeping the hidden states and the logits' gradient as planes in memory,
+// which takes half of the splitting out, was no faster (1,000 rows: 3 % slower).
 #pragma once
 
 #include "head_gemm.h"

@@ -1,5 +1,5 @@
 // Cross entropy over the vocabulary and its gradients without the logits
-// (include/gemmaedge_head.h), on the matrix product of head_gemm.h.
+// (include/gemmaedge_head.h), on the matrix products of head_gemm.h and head_gemm32.h.
 //
 // Forward: a tile of vocabulary x rows of logits stays in the accumulators; its
 // epilogue leaves, for each row, the tile's largest logit and the sum of
@@ -10,13 +10,22 @@
 // epilogue makes dz = g (exp(l - lse) - [target]) (1 - (l / c)^2) and stores it
 // for the piece; dhidden += dz . weights (the piece's sum in parts, each added
 // to its own float32 array, joined at the end in a fixed order); dweight rows
-// of the piece = dz^T . hidden.
+// of the piece = dz^T . hidden. bf16 operands: dz is rounded once to bf16.
 //
 // The vocabulary is the tile's M side: a lane of the accumulators then holds 4
 // logits of one row per 16 x 16 product, and, with the rows of a wave's tile
-// dealt out by epi_row, a contiguous run of the vocabulary: sums over the
+// dealt out by epi_row, 8 neighbours in every two products: sums over the
 // vocabulary are mostly sums over a lane's own registers, and dz is stored in
-// 16-byte pieces.
+// 16-byte pieces. The epilogues have one wave a SIMD and nothing to hide behind:
+// no branch an element, the target's element apart, and with a softcap two
+// exponentials and a reciprocal an element, which are most of their 8 us a tile.
+//
+// 4,096 rows, width 2,816, vocabulary 262,144 in bf16: forward 4.7 ms (1,280
+// TFLOP/s), backward 14.4 ms: logits again 4.9 (1,230), dhidden 4.9 (1,230),
+// dweight 4.5 (1,330); a plain product of this size by the library reaches 1,480.
+// Bound by the matrix cores (54 to 65 % of their cycles at the 2.0 to 2.1 GHz that
+// the card holds under them) and the loads that feed them. One row: the weights'
+// bytes, 5.9 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "head_internal.h"
@@ -138,11 +147,11 @@ struct StatsEpi {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 // A wave whose rows all lie past the vocabulary has nothing to add.
-                const float ref = top == -__builtin_inff() ? 0.f : top * kLog2e;
+                const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
                 for (int i = 0; i < kMt; ++i)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) sum += exp2_fast(fmaf(acc[i][j][q], kLog2e, -ref));
+                    for (int q = 0; q < 4; ++q) sum += exp2_fast((acc[i][j][q] - ref) * kLog2e);  // the difference is exact where it counts
             }
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);

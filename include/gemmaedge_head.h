@@ -36,8 +36,8 @@ typedef struct ge_head ge_head;
 /* Create a head on `device` for up to max_rows hidden states of up to max_dim
  * channels and a vocabulary of up to max_vocab, elements of type `dtype`.
  * Allocates every workspace now. train != 0 adds what the backward calls need
- * (about 0.5 to 1 GiB for the loss of large batches; the gradient of the
- * logits is held for a piece of the vocabulary at a time). */
+ * (about 1 GiB for the loss of large batches; the gradient of the logits is
+ * held for a piece of the vocabulary at a time, 512 MiB at most). */
 int ge_head_create(int device, int max_rows, int max_dim, int max_vocab, int dtype, int train, ge_head** out);
 
 void ge_head_destroy(ge_head* head);
@@ -90,10 +90,11 @@ int ge_head_norm_backward(ge_head* head, void* stream, const ge_norm_args* args)
  *   dz_v = grad * (exp(l_v - lse) - [v = target]) * (1 - (l_v / softcap)^2),
  *   dhidden = sum over v of dz_v * weight_v, dweight_v = sum over rows of dz_v * hidden.
  * It computes the logits again, a piece of the vocabulary at a time, and holds
- * dz in the operands' type (bf16: each value rounded once to 8 bits of
- * mantissa before the two products, whose sums are float32; float32 operands
- * are multiplied in three bf16 planes each, 24 bits). A non-finite element
- * makes the rows it takes part in NaN. */
+ * dz in the operands' type (bf16: each value rounded once to 8 bits of mantissa,
+ * in units of the largest grad's mantissa, before the two products, whose sums
+ * are float32; float32 operands are multiplied in three bf16 planes each, 24
+ * bits). A NaN makes the rows it takes part in NaN; so does an infinity in
+ * float32, and in bf16 where the formula gives no number. */
 typedef struct ge_loss_args {
     const void* hidden;       /* [rows][dim], hidden_stride elements apart */
     int64_t hidden_stride;
@@ -120,7 +121,8 @@ int ge_head_loss_backward(ge_head* head, void* stream, const ge_loss_args* args)
 /* One AdamW step over any number of tensors in one launch:
  *   g = grad * grad_scale, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g g,
  *   p = p (1 - lr weight_decay) - (lr / (1 - beta1^step)) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * in float32, each operation rounded by itself. p is the master where there is
+ * in float32, each operation rounded by itself (with 8-bit states the square root
+ * and the quotient are within 1 ulp each). p is the master where there is
  * one (the parameter is then the master rounded), else the parameter.
  *
  * state_bits 32: m and v are float32. state_bits 8: blocks of GE_ADAMW_BLOCK
