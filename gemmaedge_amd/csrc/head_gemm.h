@@ -357,7 +357,11 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g
     for (int i = 0; i < kMt; ++i)
 #pragma unroll
         for (int j = 0; j < kNt; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    arrive();
+    // The first stage has arrived; a wave has at least this many loads of the second.
+    constexpr int kSecond = LoaderA::kInstr / kWaves + LoaderB::kInstr / kWaves;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kSecond) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kMt + kNt; ++i) fetch(i, 0, s0);
     // Steps in pairs: an odd one's partner multiplies zeros. One way out of the loop

@@ -12,6 +12,8 @@ from __future__ import annotations
 import ctypes
 from typing import Optional, Sequence
 
+import torch
+
 from . import sampler as S
 
 GE_ADAMW_BLOCK = 256
@@ -98,8 +100,6 @@ def _check(rc: int) -> None:
 
 
 def _dtype(t, what: str) -> int:
-    import torch
-
     if t.dtype == torch.float32:
         return S.GE_DTYPE_F32
     if t.dtype == torch.bfloat16:
@@ -133,28 +133,25 @@ def _on_gpu(t, what: str):
     return t.device
 
 
-class _Stream:
-    """The stream of a call: ``handle`` for the launch, and a context for the
-    outputs it allocates. The current stream, the usual case, needs no switch."""
+def _stream(stream, device):
+    """(handle for the launch, context for the outputs it allocates). The current
+    stream, the usual case, needs no context."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index), None
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    return stream.cuda_stream, torch.cuda.stream(stream)
 
-    def __init__(self, stream, device):
-        import torch
 
-        self._switch = None
-        if stream is None:
-            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
-        else:
-            stream = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
-            self.handle = stream.cuda_stream
-            self._switch = torch.cuda.stream(stream)
-
-    def __enter__(self):
-        if self._switch is not None:
-            self._switch.__enter__()
-
-    def __exit__(self, *exc):
-        if self._switch is not None:
-            self._switch.__exit__(*exc)
+def _output(t, what: str, dtype, shape, device, switch):
+    """The given output, checked, or a new one of the call's stream."""
+    if t is not None:
+        _want(t, what, dtype, shape, device)
+        return t
+    if switch is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with switch:
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 class Head:
@@ -164,8 +161,6 @@ class Head:
     A handle must not be used by two streams at once."""
 
     def __init__(self, max_rows: int, max_dim: int, max_vocab: int, dtype=None, train: bool = False, device: int = 0):
-        import torch
-
         self._h = None
         self.dtype = torch.bfloat16 if dtype is None else dtype
         if self.dtype not in (torch.float32, torch.bfloat16):
@@ -203,31 +198,22 @@ class Head:
         """y = (x - mean) * rstd * weight + bias over the last axis of [rows, dim];
         without ``center`` the mean is left at 0 (root-mean-square norm) and None is
         returned for it. Returns (y, mean, rstd)."""
-        import torch
-
         rows, dim = self._rows(x, "x")
         a = NormArgs()
         a.weight_dtype = _dtype(weight, "weight")
         _want(weight, "weight", weight.dtype, (dim,), self.device)
         if bias is not None:
             _want(bias, "bias", weight.dtype, (dim,), self.device)
-        stream = _Stream(stream, self.device)
-        with stream:
-            if y is None:
-                y = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
-            if mean is None and center:
-                mean = torch.empty(rows, dtype=torch.float32, device=self.device)
-            if rstd is None:
-                rstd = torch.empty(rows, dtype=torch.float32, device=self.device)
-        _want(y, "y", self.dtype, (rows, dim), self.device)
-        for t, what in ((mean, "mean"), (rstd, "rstd")):
-            if t is not None:
-                _want(t, what, torch.float32, (rows,), self.device)
+        handle, switch = _stream(stream, self.device)
+        y = _output(y, "y", self.dtype, (rows, dim), self.device, switch)
+        rstd = _output(rstd, "rstd", torch.float32, (rows,), self.device, switch)
+        if center or mean is not None:
+            mean = _output(mean, "mean", torch.float32, (rows,), self.device, switch)
         a.x, a.x_stride, a.rows, a.dim = x.data_ptr(), _stride(x), rows, dim
         a.center, a.eps = int(center), eps
         a.weight, a.bias = weight.data_ptr(), S._ptr(bias)
         a.y, a.y_stride, a.mean, a.rstd = y.data_ptr(), _stride(y), S._ptr(mean), rstd.data_ptr()
-        _check(_library().ge_head_norm(self._h, stream.handle, ctypes.byref(a)))
+        _check(_library().ge_head_norm(self._h, handle, ctypes.byref(a)))
         return y, mean, rstd
 
     def norm_backward(self, grad, x, weight, mean, rstd, bias: bool = False, dx=None, dweight=None, dbias=None,
@@ -235,8 +221,6 @@ class Head:
         """Gradients of ``norm`` for the gradient ``grad`` of its y, with the mean
         (None: not centred) and rstd it returned. Returns (dx, dweight, dbias), None
         for what is not wanted (``need_input``, ``need_weight``, ``bias``)."""
-        import torch
-
         rows, dim = self._rows(x, "x")
         a = NormArgs()
         a.weight_dtype = _dtype(weight, "weight")
@@ -245,31 +229,23 @@ class Head:
         _want(rstd, "rstd", torch.float32, (rows,), self.device)
         if mean is not None:
             _want(mean, "mean", torch.float32, (rows,), self.device)
-        stream = _Stream(stream, self.device)
-        with stream:
-            if dx is None and need_input:
-                dx = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
-            if dweight is None and need_weight:
-                dweight = torch.empty(dim, dtype=weight.dtype, device=self.device)
-            if dbias is None and bias:
-                dbias = torch.empty(dim, dtype=weight.dtype, device=self.device)
-        if dx is not None:
-            _want(dx, "dx", self.dtype, (rows, dim), self.device)
+        handle, switch = _stream(stream, self.device)
+        if need_input or dx is not None:
+            dx = _output(dx, "dx", self.dtype, (rows, dim), self.device, switch)
             a.dx_stride = _stride(dx)
-        for t, what in ((dweight, "dweight"), (dbias, "dbias")):
-            if t is not None:
-                _want(t, what, weight.dtype, (dim,), self.device)
+        if need_weight or dweight is not None:
+            dweight = _output(dweight, "dweight", weight.dtype, (dim,), self.device, switch)
+        if bias or dbias is not None:
+            dbias = _output(dbias, "dbias", weight.dtype, (dim,), self.device, switch)
         a.x, a.x_stride, a.rows, a.dim = x.data_ptr(), _stride(x), rows, dim
         a.center = int(mean is not None)
         a.weight, a.mean, a.rstd = weight.data_ptr(), S._ptr(mean), rstd.data_ptr()
         a.dy, a.dy_stride, a.dx = grad.data_ptr(), _stride(grad), S._ptr(dx)
         a.dweight, a.dbias = S._ptr(dweight), S._ptr(dbias)
-        _check(_library().ge_head_norm_backward(self._h, stream.handle, ctypes.byref(a)))
+        _check(_library().ge_head_norm_backward(self._h, handle, ctypes.byref(a)))
         return dx, dweight, dbias
 
     def _loss_args(self, hidden, weight, targets, softcap):
-        import torch
-
         rows, dim = self._rows(hidden, "hidden")
         if weight.dim() != 2:
             raise ValueError(f"weight has shape {tuple(weight.shape)}: [vocab, dim] is wanted")
@@ -285,17 +261,12 @@ class Head:
         """Cross entropy of [rows, dim] hidden states against their ``targets``
         (int32 [rows]; outside [0, vocab): no loss) over [vocab, dim] weights.
         -loss is the target's log-probability. Returns (loss, lse), float32 [rows]."""
-        import torch
-
         a, rows, _, _ = self._loss_args(hidden, weight, targets, softcap)
-        stream = _Stream(stream, self.device)
-        with stream:
-            loss = torch.empty(rows, dtype=torch.float32, device=self.device) if loss is None else loss
-            lse = torch.empty(rows, dtype=torch.float32, device=self.device) if lse is None else lse
-        _want(loss, "loss", torch.float32, (rows,), self.device)
-        _want(lse, "lse", torch.float32, (rows,), self.device)
+        handle, switch = _stream(stream, self.device)
+        loss = _output(loss, "loss", torch.float32, (rows,), self.device, switch)
+        lse = _output(lse, "lse", torch.float32, (rows,), self.device, switch)
         a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-        _check(_library().ge_head_loss(self._h, stream.handle, ctypes.byref(a)))
+        _check(_library().ge_head_loss(self._h, handle, ctypes.byref(a)))
         return loss, lse
 
     def loss_backward(self, grad, hidden, weight, targets, lse, softcap: float = 0.0, dhidden=None, dweight=None,
@@ -303,25 +274,18 @@ class Head:
         """Gradients of ``loss`` for ``grad`` (float32 [rows], the objective's
         derivative by each row's loss) and the lse it returned. Returns (dhidden,
         dweight), None for what is not wanted."""
-        import torch
-
         a, rows, dim, vocab = self._loss_args(hidden, weight, targets, softcap)
         _want(grad, "grad", torch.float32, (rows,), self.device)
         _want(lse, "lse", torch.float32, (rows,), self.device)
-        stream = _Stream(stream, self.device)
-        with stream:
-            if dhidden is None and need_hidden:
-                dhidden = torch.empty(rows, dim, dtype=self.dtype, device=self.device)
-            if dweight is None and need_weight:
-                dweight = torch.empty(vocab, dim, dtype=self.dtype, device=self.device)
-        if dhidden is not None:
-            _want(dhidden, "dhidden", self.dtype, (rows, dim), self.device)
+        handle, switch = _stream(stream, self.device)
+        if need_hidden or dhidden is not None:
+            dhidden = _output(dhidden, "dhidden", self.dtype, (rows, dim), self.device, switch)
             a.dhidden, a.dhidden_stride = dhidden.data_ptr(), _stride(dhidden)
-        if dweight is not None:
-            _want(dweight, "dweight", self.dtype, (vocab, dim), self.device)
+        if need_weight or dweight is not None:
+            dweight = _output(dweight, "dweight", self.dtype, (vocab, dim), self.device, switch)
             a.dweight, a.dweight_stride = dweight.data_ptr(), _stride(dweight)
         a.grad, a.lse = grad.data_ptr(), lse.data_ptr()
-        _check(_library().ge_head_loss_backward(self._h, stream.handle, ctypes.byref(a)))
+        _check(_library().ge_head_loss_backward(self._h, handle, ctypes.byref(a)))
         return dhidden, dweight
 
 
@@ -341,8 +305,6 @@ class AdamW:
     def __init__(self, params: Sequence, grads: Sequence, masters: Optional[Sequence] = None, lr: float = 1e-3,
                  beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, seed: int = 0, m=None, v=None, m_scale=None, v_scale=None):
-        import torch
-
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits {state_bits}: 8 or 32 is wanted")
         params, grads = list(params), list(grads)
@@ -402,8 +364,6 @@ class AdamW:
     def device_params(self, lr: Optional[float] = None, grad_scale: float = 1.0, out=None):
         """The next step's parameters as a uint8 device tensor (``out`` is overwritten
         if given), and counts the step."""
-        import torch
-
         self.steps += 1
         host = torch.frombuffer(bytearray(self._params(self.steps, lr, grad_scale)), dtype=torch.uint8)
         return host.to(self.device) if out is None else out.copy_(host)
@@ -411,8 +371,6 @@ class AdamW:
     def step(self, lr: Optional[float] = None, grad_scale: float = 1.0, stream=None, device_params=None):
         """One step with the gradients in ``grads``, each times ``grad_scale``. With
         ``device_params`` (see there) the launch reads those and counts nothing."""
-        import torch
-
         a = self._args
         if device_params is None:
             a.params = self._params(self.steps + 1, lr, grad_scale)
@@ -420,12 +378,12 @@ class AdamW:
         else:
             _want(device_params, "device_params", torch.uint8, (ctypes.sizeof(AdamwParams),), self.device)
             a.device_params = device_params.data_ptr()
-        stream = _Stream(stream, self.device)
+        handle, _ = _stream(stream, self.device)
         if torch.cuda.current_device() == self.device.index:
-            rc = _library().ge_adamw_step(stream.handle, ctypes.byref(a))
+            rc = _library().ge_adamw_step(handle, ctypes.byref(a))
         else:
             with torch.cuda.device(self.device):
-                rc = _library().ge_adamw_step(stream.handle, ctypes.byref(a))
+                rc = _library().ge_adamw_step(handle, ctypes.byref(a))
         _check(rc)
         if device_params is None:
             self.steps += 1
