@@ -67,40 +67,92 @@ __device__ __forceinline__ void store_vec(T* row, int i, int dim, const float (&
     }
 }
 
-// The vectors of a row at at[0], at[1], ... kWhole: by buffer loads and stores of
-// the row, whose bounds are checked by the hardware four bytes at a time; without
-// branches the compiler knows how many are in flight, and the next row's loads are
-// not waited for together with this row's stores. The row is then the same in the
-// whole wave, and its length a multiple of four bytes.
-template <bool kWhole, int kVec, int kVecs, typename T>
-__device__ __forceinline__ void load_row(const T* p, int64_t stride, int64_t r, int64_t rows, int dim, const int (&at)[kVecs],
-                                         Vec<T, kVec> (&to)[kVecs]) {
-    if constexpr (kWhole) {
-        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p + r * stride), 0,
-                                                                      r < rows ? dim * static_cast<int>(sizeof(T)) : 0, 0x00027000);
+// How a row is read and written. kWhole: by buffer loads and stores of the row,
+// whose bounds the hardware checks four bytes at a time; without branches the
+// compiler knows how many are in flight, and the next row's loads are not waited
+// for together with this row's stores. The row is then the same in the whole wave.
+// kOdd: the same for rows of an odd number of bf16 channels, the last one apart.
+// kBranches: rows of lane groups within a wave.
+enum Mode { kBranches, kWhole, kOdd };
+
+// A thread's channels of a row, the vectors at at[0], at[1], ..., and how it reads them.
+template <Mode kMode, int kVec, int kVecs>
+struct Place {
+    int dim;
+    int at[kVecs];
+    int last_vec, last_off;  // kOdd: the thread's vector with the last channel, and the channel's bytes from the row
+    __device__ __forceinline__ void init(int d, int lane, int lanes) {
+        dim = d;
+        last_vec = -1;
+        last_off = 0x7ffffff0;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            at[j] = (j * lanes + lane) * kVec;
+            if (kMode == kOdd && d - 1 - at[j] >= 0 && d - 1 - at[j] < kVec) {
+                last_vec = j;
+                last_off = (d - 1) * 2;
+            }
+        }
+    }
+    __device__ __forceinline__ bool is_last(int j, int e) const { return kMode == kOdd && j == last_vec && e == (dim - 1) % kVec; }
+};
+
+// A row's values in a thread.
+template <typename T, Mode kMode, int kVec, int kVecs>
+struct RowOf {
+    Vec<T, kVec> v[kVecs];
+    T last;
+    __device__ __forceinline__ float get(const Place<kMode, kVec, kVecs>& p, int j, int e) const {
+        return to_f32(p.is_last(j, e) ? last : v[j].v[e]);
+    }
+};
+
+template <typename T, Mode kMode, int kVec, int kVecs>
+__device__ __forceinline__ void load_row(const T* p, int64_t stride, int64_t r, int64_t rows, const Place<kMode, kVec, kVecs>& pl,
+                                         RowOf<T, kMode, kVec, kVecs>& to) {
+    if constexpr (kMode != kBranches) {
+        constexpr int kSize = sizeof(T);
+        T* const row = const_cast<T*>(p + r * stride);
+        const int bytes = r < rows ? pl.dim * kSize : 0;
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(row, 0, kMode == kOdd && bytes ? bytes - kSize : bytes, 0x00027000);
 #pragma unroll
         for (int j = 0; j < kVecs; ++j)
-            to[j] = __builtin_bit_cast(Vec<T, kVec>, __builtin_amdgcn_raw_buffer_load_b128(rs, at[j] * static_cast<int>(sizeof(T)), 0, 0));
+            to.v[j] = __builtin_bit_cast(Vec<T, kVec>, __builtin_amdgcn_raw_buffer_load_b128(rs, pl.at[j] * kSize, 0, 0));
+        if constexpr (kMode == kOdd) {
+            rs = __builtin_amdgcn_make_buffer_rsrc(row, 0, bytes, 0x00027000);
+            to.last = __builtin_amdgcn_raw_buffer_load_b16(rs, pl.last_off, 0, 0);
+        }
     } else if (r < rows) {
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) to[j] = load_vec<kVec>(p + r * stride, at[j], dim);
+        for (int j = 0; j < kVecs; ++j) to.v[j] = load_vec<kVec>(p + r * stride, pl.at[j], pl.dim);
     }
 }
-template <bool kWhole, int kVec, int kVecs, typename T>
-__device__ __forceinline__ void store_row(T* p, int64_t stride, int64_t r, int dim, const int (&at)[kVecs], const float (&x)[kVecs][kVec]) {
-    if constexpr (kWhole) {
-        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(p + r * stride, 0, dim * static_cast<int>(sizeof(T)), 0x00027000);
+template <Mode kMode, int kVec, int kVecs, typename T>
+__device__ __forceinline__ void store_row(T* p, int64_t stride, int64_t r, const Place<kMode, kVec, kVecs>& pl, const float (&x)[kVecs][kVec]) {
+    if constexpr (kMode != kBranches) {
+        constexpr int kSize = sizeof(T);
+        T* const row = p + r * stride;
+        const int bytes = pl.dim * kSize;
+        __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(row, 0, kMode == kOdd ? bytes - kSize : bytes, 0x00027000);
         using Words = decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0));
+        T last = T(0);
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
             Vec<T, kVec> v;
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) v.v[e] = from_f32<T>(x[j][e]);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, v), rs, at[j] * static_cast<int>(sizeof(T)), 0, 0);
+            for (int e = 0; e < kVec; ++e) {
+                v.v[e] = from_f32<T>(x[j][e]);
+                if (pl.is_last(j, e)) last = v.v[e];
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, v), rs, pl.at[j] * kSize, 0, 0);
+        }
+        if constexpr (kMode == kOdd) {
+            rs = __builtin_amdgcn_make_buffer_rsrc(row, 0, bytes, 0x00027000);
+            __builtin_amdgcn_raw_buffer_store_b16(last, rs, pl.last_off, 0, 0);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) store_vec(p + r * stride, at[j], dim, x[j]);
+        for (int j = 0; j < kVecs; ++j) store_vec(p + r * stride, pl.at[j], pl.dim, x[j]);
     }
 }
 
@@ -171,7 +223,7 @@ struct Team {
     }
 };
 
-template <typename T, typename W, int kGroup, int kVecs, bool kWhole>
+template <typename T, typename W, int kGroup, int kVecs, Mode kMode>
 __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     __shared__ __align__(16) float2 red[2 * kMostWaves];
     constexpr int kVec = vec_of<T>;
@@ -179,10 +231,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     const int dim = x.dim;
     const float n = static_cast<float>(dim);
     float w[kVecs][kVec], b[kVecs][kVec];
-    int at[kVecs];
+    Place<kMode, kVec, kVecs> place;
+    place.init(dim, team.lane, team.lanes);
+    const int(&at)[kVecs] = place.at;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
-        at[j] = (j * team.lanes + team.lane) * kVec;
         const Vec<W, kVec> vw = load_vec<kVec>(static_cast<const W*>(x.weight), at[j], dim);
         Vec<W, kVec> vb{};
         if (x.bias) vb = load_vec<kVec>(static_cast<const W*>(x.bias), at[j], dim);
@@ -196,8 +249,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
     int64_t r = static_cast<int64_t>(blockIdx.x) * team.slots + team.slot;
     if (r >= x.rows) return;  // a lane group of its own; a workgroup's first row is there
     const T* in = static_cast<const T*>(x.x);
-    Vec<T, kVec> next[kVecs];
-    load_row<kWhole>(in, x.x_stride, r, x.rows, dim, at, next);
+    RowOf<T, kMode, kVec, kVecs> next;
+    load_row(in, x.x_stride, r, x.rows, place, next);
     for (; r < x.rows; r += step) {
         float h[kVecs][kVec];
         float2 s{0.f, 0.f};
@@ -205,10 +258,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-                h[j][e] = to_f32(next[j].v[e]);
+                h[j][e] = next.get(place, j, e);
                 s.x += h[j][e];
             }
-        load_row<kWhole>(in, x.x_stride, r + step, x.rows, dim, at, next);
+        load_row(in, x.x_stride, r + step, x.rows, place, next);
         const float mean = x.center ? team.sum(s).x / n : 0.f;
         float2 q{0.f, 0.f};
 #pragma unroll
@@ -223,7 +276,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < kVec; ++e) h[j][e] = fmaf(h[j][e] * rstd, w[j][e], b[j][e]);
-        store_row<kWhole>(static_cast<T*>(x.y), x.y_stride, r, dim, at, h);
+        store_row(static_cast<T*>(x.y), x.y_stride, r, place, h);
         if (team.lane == 0) {
             x.rstd[r] = rstd;
             if (x.mean) x.mean[r] = mean;
@@ -232,7 +285,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(ge_norm_args x) {
 }
 
 // dx, and with kWeight a workgroup's part of the weights' gradients.
-template <typename T, typename W, int kGroup, int kVecs, bool kWhole, bool kWeight>
+template <typename T, typename W, int kGroup, int kVecs, Mode kMode, bool kWeight>
 __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_args x, float* parts) {
     __shared__ __align__(16) float2 red[2 * kMostWaves];
     constexpr int kVec = vec_of<T>;
@@ -241,10 +294,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
     const int dim = x.dim;
     const float inv = 1.0f / static_cast<float>(dim);
     float w[kVecs][kVec], sw[kVecs][kVec], sb[kVecs][kVec];
-    int at[kVecs];
+    Place<kMode, kVec, kVecs> place;
+    place.init(dim, team.lane, team.lanes);
+    const int(&at)[kVecs] = place.at;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
-        at[j] = (j * team.lanes + team.lane) * kVec;
         const Vec<W, kVec> vw = load_vec<kVec>(static_cast<const W*>(x.weight), at[j], dim);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
@@ -257,7 +311,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
     const T* in = static_cast<const T*>(x.x);
     const T* dy = static_cast<const T*>(x.dy);
     struct Row {
-        Vec<T, kVec> x[kVecs], y[kVecs];
+        RowOf<T, kMode, kVec, kVecs> x, y;
         float mean, rstd;
     };
     Row next{};
@@ -267,8 +321,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
     asm volatile("v_mov_b32 %0, 0" : "=v"(lane_zero));
     const float *mean_of = x.mean + lane_zero, *rstd_of = x.rstd + lane_zero;
     auto fetch = [&](int64_t row) __attribute__((always_inline)) {
-        load_row<kWhole>(in, x.x_stride, row, x.rows, dim, at, next.x);
-        load_row<kWhole>(dy, x.dy_stride, row, x.rows, dim, at, next.y);
+        load_row(in, x.x_stride, row, x.rows, place, next.x);
+        load_row(dy, x.dy_stride, row, x.rows, place, next.y);
         const int64_t last = min(row, static_cast<int64_t>(x.rows) - 1);
         next.mean = x.center ? mean_of[last] : 0.f;
         next.rstd = rstd_of[last];
@@ -282,8 +336,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-                const float g = to_f32(next.y[j].v[e]);
-                h[j][e] = (to_f32(next.x[j].v[e]) - mean) * rstd;
+                const float g = next.y.get(place, j, e);
+                h[j][e] = (next.x.get(place, j, e) - mean) * rstd;
                 a[j][e] = g * w[j][e];
                 s.x += a[j][e];
                 s.y = fmaf(a[j][e], h[j][e], s.y);
@@ -300,7 +354,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(ge_norm_arg
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < kVec; ++e) a[j][e] = rstd * (a[j][e] - sa - h[j][e] * sx);
-        store_row<kWhole>(static_cast<T*>(x.dx), x.dx_stride, r, dim, at, a);
+        store_row(static_cast<T*>(x.dx), x.dx_stride, r, place, a);
     }
     if constexpr (kWeight) {
         float* p = parts + static_cast<int64_t>(blockIdx.x) * 2 * dim;
@@ -467,27 +521,28 @@ NormPlan norm_plan(int dim, int vec) {
     return p;
 }
 
-// Calls f with the plan's group and vectors and whether rows are whole as constants.
+// Calls f with the plan's group and vectors and the rows' mode as constants.
 template <typename T, typename F>
 void with_plan(const NormPlan& p, int dim, F f) {
     using std::integral_constant;
-    constexpr std::false_type no{};
+    constexpr integral_constant<Mode, kBranches> branches{};
     constexpr integral_constant<int, 1> one{};
-    if (p.group == 8) return f(integral_constant<int, 8>{}, one, no);
-    if (p.group == 16) return f(integral_constant<int, 16>{}, one, no);
-    if (p.group == 32) return f(integral_constant<int, 32>{}, one, no);
-    auto by_vecs = [&](auto group, auto whole) {
-        if (p.vecs == 1) return f(group, one, whole);
-        if (sizeof(T) == 2 || p.vecs == 2) return f(group, integral_constant<int, 2>{}, whole);
-        if constexpr (sizeof(T) == 4) f(group, integral_constant<int, 4>{}, whole);
+    if (p.group == 8) return f(integral_constant<int, 8>{}, one, branches);
+    if (p.group == 16) return f(integral_constant<int, 16>{}, one, branches);
+    if (p.group == 32) return f(integral_constant<int, 32>{}, one, branches);
+    auto by_vecs = [&](auto group, auto mode) {
+        if (p.vecs == 1) return f(group, one, mode);
+        if (sizeof(T) == 2 || p.vecs == 2) return f(group, integral_constant<int, 2>{}, mode);
+        if constexpr (sizeof(T) == 4) f(group, integral_constant<int, 4>{}, mode);
     };
-    auto by_group = [&](auto whole) {
-        if (p.group == 64) return by_vecs(integral_constant<int, 64>{}, whole);
-        by_vecs(integral_constant<int, 0>{}, whole);
+    auto by_group = [&](auto mode) {
+        if (p.group == 64) return by_vecs(integral_constant<int, 64>{}, mode);
+        by_vecs(integral_constant<int, 0>{}, mode);
     };
-    if constexpr (sizeof(T) == 4) return by_group(std::true_type{});
-    if (dim % 2 == 0) return by_group(std::true_type{});
-    by_group(no);
+    if constexpr (sizeof(T) == 2) {
+        if (dim % 2 != 0) return by_group(integral_constant<Mode, kOdd>{});
+    }
+    by_group(integral_constant<Mode, kWhole>{});
 }
 
 template <typename T, typename W>
@@ -498,8 +553,8 @@ void norm_forward(const ge_norm_args& x, hipStream_t st) {
     }
     const NormPlan p = norm_plan(x.dim, vec_of<T>);
     const unsigned blocks = std::min((x.rows + p.slots - 1) / p.slots, kNormBlocks);
-    with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto whole) {
-        norm_kernel<T, W, decltype(group)::value, decltype(vecs)::value, decltype(whole)::value><<<blocks, p.threads, 0, st>>>(x);
+    with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto mode) {
+        norm_kernel<T, W, decltype(group)::value, decltype(vecs)::value, decltype(mode)::value><<<blocks, p.threads, 0, st>>>(x);
     });
 }
 
@@ -517,13 +572,13 @@ void norm_backward(const ge_norm_args& x, const Buffers& b, hipStream_t st) {
     } else if (x.rows > 0) {
         const NormPlan p = norm_plan(x.dim, vec_of<T>);
         parts = std::min((x.rows + p.slots - 1) / p.slots, kNormParts);
-        with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto whole) {
+        with_plan<T>(p, x.dim, [&](auto group, auto vecs, auto mode) {
             constexpr int g = decltype(group)::value, v = decltype(vecs)::value;
-            constexpr bool w = decltype(whole)::value;
+            constexpr Mode m = decltype(mode)::value;
             if (weight)
-                norm_backward_kernel<T, W, g, v, w, true><<<parts, p.threads, 0, st>>>(x, b.norm);
+                norm_backward_kernel<T, W, g, v, m, true><<<parts, p.threads, 0, st>>>(x, b.norm);
             else if (x.dx)
-                norm_backward_kernel<T, W, g, v, w, false><<<parts, p.threads, 0, st>>>(x, b.norm);
+                norm_backward_kernel<T, W, g, v, m, false><<<parts, p.threads, 0, st>>>(x, b.norm);
         });
     }
     if (weight) {
