@@ -229,6 +229,7 @@ struct GradEpi {
     static constexpr bool kFast = sizeof(T) == 2;
     Softcap sc;
     int v0, rows, vocab_all;
+    int piece;  // words of the vocabulary from v0 on in this product
     const int32_t* targets;
     const float* lse;
     const float* grad;
@@ -293,6 +294,9 @@ struct GradEpi {
     __device__ __forceinline__ void store(f32x4 (&acc)[kMt][kNt], int row0, int n_first, int lane, const int (&t)[kNt],
                                           const float (&ls)[kNt], const float (&gr)[kNt]) const {
         __builtin_assume(kCap ? sc.cap > 0.f : !(sc.cap > 0.f));
+        // Words past the vocabulary have logits of 0, and exp(-lse) may be infinite: the
+        // product over the words, which reads up to 7 of them, gets zeros instead.
+        const bool tail = row0 + kWm > piece;
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             float d[kMt * 4];
@@ -308,6 +312,10 @@ struct GradEpi {
 #pragma unroll
                 for (int e = 0; e < kMt * 4; ++e)
                     if (at == e) d[e] = x;
+            }
+            if (tail) {
+#pragma unroll
+                for (int e = 0; e < kMt * 4; ++e) d[e] = row0 + epi_row(e >> 2, 4 * (lane >> 4) + (e & 3)) < piece ? d[e] : 0.f;
             }
             T* o = out + static_cast<int64_t>(n_first + j * 16) * ld + row0 + (lane >> 4) * 8;
 #pragma unroll
@@ -551,7 +559,7 @@ struct Call {
         for (int v0 = 0; v0 < x.vocab; v0 += plan.piece) {
             const int n = std::min(plan.piece, x.vocab - v0);
             const Operand w = weights(v0, n);
-            GradEpi<T> e{softcap(), v0, x.rows, x.vocab, x.targets, x.lse, x.grad, unit, reinterpret_cast<T*>(b.dlogits), ld};
+            GradEpi<T> e{softcap(), v0, x.rows, x.vocab, n, x.targets, x.lse, x.grad, unit, reinterpret_cast<T*>(b.dlogits), ld};
             logits(w, h, n, e);
             // Rows past the batch read as zeros: they are no rows of the hidden states either.
             const Operand dz{b.dlogits, ld, x.rows * ld};
