@@ -41,16 +41,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// softcap * tanh(z / softcap). bf16 operands: tanh = 1 - 2 r with r = 1 / (exp(2 x) + 1)
-// of the hardware's exp2 and reciprocal, 3e-7 of the cap off at most, far below
-// what the operands' 8 bits leave of z; float32 operands: tanhf.
+// How logits are capped. kBounded: bf16 operands and caps up to 40; kWide: larger caps, and float32 operands.
+enum Cap { kNone, kBounded, kWide };
+
+// softcap * tanh(z / softcap). bf16 operands, caps up to 40: tanh = 1 - 2 r with
+// r = 1 / (exp(2 x) + 1) of the hardware's exp2 and reciprocal, 4e-7 of the cap off at
+// most, far below what the operands' 8 bits leave of z. Above 40 that error would
+// reach the logits, which may be small against the cap: below x = 1 / 4 a series, whose
+// first term is z itself, so that it is 1e-6 of the logit off at most. float32 operands:
+// tanhf, and z itself where x^2 / 3 < u (x has lost bits there if 1 / cap is subnormal).
 struct Softcap {
     float cap, inv, two;  // cap <= 0: none; two = 2 log2(e) / cap
     __device__ __forceinline__ float r(float z) const { return __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f); }
-    template <bool kFast>
-    __device__ __forceinline__ float apply(float z) const {
-        return kFast ? fmaf(r(z), -2.0f * cap, cap) : cap * tanhf(z * inv);
+    __device__ __forceinline__ float bounded_logit(float z) const { return fmaf(r(z), -2.0f * cap, cap); }
+    // `z` and its r
+    __device__ __forceinline__ float wide_logit(float z, float r) const {
+        const float x = z * inv, q = x * x;
+        const float s = fmaf(fmaf(fmaf(62.0f / 2835.0f, q, -17.0f / 315.0f), q, 2.0f / 15.0f), q, -1.0f / 3.0f);
+        return q < 0.0625f ? fmaf(z, s * q, z) : fmaf(r, -2.0f * cap, cap);
     }
+    __device__ __forceinline__ float exact_logit(float z, float tanh) const { return fabsf(z * inv) < 0x1p-12f ? z : cap * tanh; }
     // exp(-2 cap) is a normal number: sums of exp(l - cap) need no largest logit.
     __device__ __forceinline__ bool bounded() const { return cap > 0.f && cap <= 40.f; }
 };
@@ -70,6 +80,16 @@ __device__ __forceinline__ void load_targets(const int32_t* targets, int n_first
     for (int j = 0; j < kNt; ++j) t[j] = targets[min(n_first + j * 16, rows - 1)];
 #pragma unroll
     for (int j = 0; j < kNt; ++j) t[j] = n_first + j * 16 < rows && t[j] >= v0 && t[j] - v0 < vocab ? t[j] - v0 : -1;
+}
+
+// Column j's accumulators stay where they are until here: the compiler otherwise reads all
+// of a large tile's into registers first, which do not hold them.
+template <int kMt, int kNt>
+__device__ __forceinline__ void hold(f32x4 (&acc)[kMt][kNt], int j) {
+    if constexpr (kMt * kNt >= 32) {
+#pragma unroll
+        for (int i = 0; i < kMt; ++i) asm volatile("" : "+a"(acc[i][j]));
+    }
 }
 
 template <bool kFast>
@@ -93,70 +113,89 @@ struct StatsEpi {
         load_targets(targets, col0 + (lane & 15), rows, v0, vocab, s.t);
         return s;
     }
+    template <Cap kCap>
+    __device__ __forceinline__ float logit(float z) const {
+        if (kCap == kNone) return z;
+        if (!kFast) return sc.exact_logit(z, tanhf(z * sc.inv));
+        return kCap == kBounded ? sc.bounded_logit(z) : sc.wide_logit(z, sc.r(z));
+    }
+    // The largest logit, the sum and the target's logit of the wave's columns.
+    template <int kWm, Cap kCap, int kMt, int kNt>
+    __device__ __forceinline__ void columns(f32x4 (&acc)[kMt][kNt], const int (&t)[kNt], int row0, int n_first, int lane,
+                                            float2* part) const {
+        const bool tail = row0 + kWm > vocab;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            hold(acc, j);
+            float l[4 * kMt];
+#pragma unroll
+            for (int e = 0; e < 4 * kMt; ++e) l[e] = logit<kCap>(acc[e >> 2][j][e & 3]);
+            if (tail) {
+#pragma unroll
+                for (int e = 0; e < 4 * kMt; ++e)
+                    l[e] = row0 + epi_row(e >> 2, 4 * (lane >> 4) + (e & 3)) >= vocab ? -__builtin_inff() : l[e];
+            }
+            const int at = target_place<kWm>(t[j], row0, lane);
+            if (t[j] >= 0 && at >= 0) {
+                float x = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4 * kMt; ++e)
+                    if (at == e) x = l[e];
+                target_logit[n_first + j * 16] = x;
+            }
+            float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4 * kMt; ++e) top = fmaxf(top, l[e]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // A wave whose rows all lie past the vocabulary has nothing to add.
+            const float ref = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+            for (int e = 0; e < 4 * kMt; ++e) sum += exp2_fast((l[e] - ref) * kLog2e);  // the difference is exact where it counts
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane < 16) part[j * 16 + lane] = make_float2(top, sum);
+        }
+    }
+    // The same for caps up to 40 within the vocabulary: the cap stands for the largest logit.
+    template <int kWm, int kMt, int kNt>
+    __device__ __forceinline__ void bounded_columns(f32x4 (&acc)[kMt][kNt], const int (&t)[kNt], int row0, int n_first, int lane,
+                                                    float2* part) const {
+        const float k = -2.0f * kLog2e * sc.cap;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            hold(acc, j);
+            const int at = target_place<kWm>(t[j], row0, lane);
+            if (t[j] >= 0 && at >= 0) {
+                float x = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4 * kMt; ++e)
+                    if (at == e) x = acc[e >> 2][j][e & 3];
+                target_logit[n_first + j * 16] = sc.bounded_logit(x);
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4 * kMt; ++e) sum += exp2_fast(sc.r(acc[e >> 2][j][e & 3]) * k);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane < 16) part[j * 16 + lane] = make_float2(sc.cap, sum);
+        }
+    }
     template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
     __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State<kNt>& s, int m0, int n0, TilePlace place, int wm, int wn,
                                            int lane, float2* part) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm;
         const int n_first = n0 + wn * kWn + (lane & 15);
-        const int(&t)[kNt] = s.t;
-        const bool tail = row0 + kWm > vocab;
-        const bool simple = kFast && sc.bounded() && !tail;
-        if (!simple && sc.cap > 0.f) {
-#pragma unroll
-            for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                for (int j = 0; j < kNt; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[i][j][q] = sc.apply<kFast>(acc[i][j][q]);
-        }
-        if (tail) {
-#pragma unroll
-            for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const bool past = row0 + epi_row(i, 4 * (lane >> 4) + q) >= vocab;
-#pragma unroll
-                    for (int j = 0; j < kNt; ++j) acc[i][j][q] = past ? -__builtin_inff() : acc[i][j][q];
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < kNt; ++j) {
-            const int at = target_place<kWm>(t[j], row0, lane);
-            if (t[j] >= 0 && at >= 0) {
-                float l = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4 * kMt; ++e)
-                    if (at == e) l = acc[e >> 2][j][e & 3];
-                target_logit[n_first + j * 16] = simple ? sc.apply<kFast>(l) : l;
-            }
-            float top, sum = 0.f;
-            if (simple) {
-                top = sc.cap;
-                const float k = -2.0f * kLog2e * sc.cap;
-#pragma unroll
-                for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) sum += exp2_fast(sc.r(acc[i][j][q]) * k);
-            } else {
-                top = -__builtin_inff();
-#pragma unroll
-                for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) top = fmaxf(top, acc[i][j][q]);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                // A wave whose rows all lie past the vocabulary has nothing to add.
-                const float ref = top == -__builtin_inff() ? 0.f : top;
-#pragma unroll
-                for (int i = 0; i < kMt; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) sum += exp2_fast((acc[i][j][q] - ref) * kLog2e);  // the difference is exact where it counts
-            }
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (lane < 16) part[wm * kBn + wn * kWn + j * 16 + lane] = make_float2(top, sum);
-        }
+        float2* const to = part + wm * kBn + wn * kWn;
+        if (!(sc.cap > 0.f))
+            columns<kWm, kNone>(acc, s.t, row0, n_first, lane, to);
+        else if (!kFast || !sc.bounded())
+            columns<kWm, kWide>(acc, s.t, row0, n_first, lane, to);
+        else if (row0 + kWm > vocab)
+            columns<kWm, kBounded>(acc, s.t, row0, n_first, lane, to);
+        else
+            bounded_columns<kWm>(acc, s.t, row0, n_first, lane, to);
         __syncthreads();
         for (int c = threadIdx.x; c < kBn; c += 64 * kWavesM * kWavesN) {
             const int n = n0 + c;
@@ -237,17 +276,18 @@ struct GradEpi {
     T* out;  // [rows_pad][ld]
     int64_t ld;
 
-    // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is that of base 2, `g` four times it
-    // with a softcap, whose slope is 4 (r - r^2) and whose l is cap - 2 cap r.
+    // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is log2(e) times (-lse, or with kBounded,
+    // whose l is cap - 2 cap r, cap - lse), `g` with a cap four times g, since the slope is 4 (r - r^2).
+    template <Cap kCap>
     __device__ __forceinline__ float dz(float z, float lse, float g, float one) const {
-        if (kFast && sc.cap > 0.f) {
+        if (kFast) {
+            if (kCap == kNone) return (exp2_fast(fmaf(z, kLog2e, lse)) - one) * g;
             const float r = sc.r(z);
-            const float p = exp2_fast(fmaf(r, -2.0f * kLog2e * sc.cap, lse));
-            return (p - one) * fmaf(-r, r, r) * g;
+            const float e = kCap == kBounded ? fmaf(r, -2.0f * kLog2e * sc.cap, lse) : fmaf(sc.wide_logit(z, r), kLog2e, lse);
+            return (exp2_fast(e) - one) * fmaf(-r, r, r) * g;
         }
-        if (kFast) return (exp2_fast(fmaf(z, kLog2e, lse)) - one) * g;
-        const float l = sc.cap > 0.f ? sc.apply<false>(z) : z;
-        const float y = sc.cap > 0.f ? l * sc.inv : 0.f;
+        const float y = kCap == kNone ? 0.f : tanhf(z * sc.inv);
+        const float l = kCap == kNone ? z : sc.exact_logit(z, y);
         return (exp2_fast((l - lse) * kLog2e) - one) * fmaf(-y, y, 1.0f) * g;
     }
 
@@ -281,19 +321,20 @@ struct GradEpi {
             ls[j] = s.lse[j];
             gr[j] = s.grad[j] / s.unit;
             if (kFast) {
-                ls[j] = sc.cap > 0.f ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
+                ls[j] = sc.bounded() ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
                 if (sc.cap > 0.f) gr[j] *= 4.0f;
             }
         }
-        if (sc.cap > 0.f)
-            store<kWm, true>(acc, row0, n_first, lane, s.t, ls, gr);
+        if (!(sc.cap > 0.f))
+            store<kWm, kNone>(acc, row0, n_first, lane, s.t, ls, gr);
+        else if (kFast && sc.bounded())
+            store<kWm, kBounded>(acc, row0, n_first, lane, s.t, ls, gr);
         else
-            store<kWm, false>(acc, row0, n_first, lane, s.t, ls, gr);
+            store<kWm, kWide>(acc, row0, n_first, lane, s.t, ls, gr);
     }
-    template <int kWm, bool kCap, int kMt, int kNt>
+    template <int kWm, Cap kCap, int kMt, int kNt>
     __device__ __forceinline__ void store(f32x4 (&acc)[kMt][kNt], int row0, int n_first, int lane, const int (&t)[kNt],
                                           const float (&ls)[kNt], const float (&gr)[kNt]) const {
-        __builtin_assume(kCap ? sc.cap > 0.f : !(sc.cap > 0.f));
         // Words past the vocabulary have logits of 0, and exp(-lse) may be infinite: the
         // product over the words, which reads up to 7 of them, gets zeros instead.
         const bool tail = row0 + kWm > piece;
@@ -301,14 +342,14 @@ struct GradEpi {
         for (int j = 0; j < kNt; ++j) {
             float d[kMt * 4];
 #pragma unroll
-            for (int e = 0; e < kMt * 4; ++e) d[e] = dz(acc[e >> 2][j][e & 3], ls[j], gr[j], 0.f);
+            for (int e = 0; e < kMt * 4; ++e) d[e] = dz<kCap>(acc[e >> 2][j][e & 3], ls[j], gr[j], 0.f);
             const int at = t[j] < v0 ? -1 : target_place<kWm>(t[j] - v0, row0, lane);
             if (at >= 0) {
                 float z = 0.f;
 #pragma unroll
                 for (int e = 0; e < kMt * 4; ++e)
                     if (at == e) z = acc[e >> 2][j][e & 3];
-                const float x = dz(z, ls[j], gr[j], 1.0f);
+                const float x = dz<kCap>(z, ls[j], gr[j], 1.0f);
 #pragma unroll
                 for (int e = 0; e < kMt * 4; ++e)
                     if (at == e) d[e] = x;
