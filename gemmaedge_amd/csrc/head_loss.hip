@@ -28,6 +28,8 @@
 // bytes, 5.9 TB/s.
 #include <hip/hip_runtime.h>
 
+#include <limits>
+
 #include "head_internal.h"
 
 #include "head_gemm.h"
@@ -534,7 +536,9 @@ struct Call {
     }
     Softcap softcap() const {
         if (!(x.softcap > 0.f)) return Softcap{0.f, 0.f, 0.f};
-        return Softcap{x.softcap, 1.0f / x.softcap, 2.0f * kLog2e / x.softcap};
+        // Finite for subnormal caps too: a logit of 0 times infinity would be NaN.
+        constexpr float kMost = std::numeric_limits<float>::max();
+        return Softcap{x.softcap, std::min(1.0f / x.softcap, kMost), std::min(2.0f * kLog2e / x.softcap, kMost)};
     }
     template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
     void run(const Operand& a, const Operand& bb, int64_t k, int m, int n, int splits, int group, const Epi& e) const {
