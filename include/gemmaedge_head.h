@@ -83,8 +83,9 @@ int ge_head_norm_backward(ge_head* head, void* stream, const ge_norm_args* args)
  * vocabulary, without storing the logits:
  *   z_v = hidden . weight_v, l_v = softcap * tanh(z_v / softcap) (l = z if softcap <= 0),
  *   lse = log(sum(exp(l_v))), loss = lse - l_target.
- * A row whose target lies outside [0, vocab) carries no loss: its loss is 0
- * and it adds nothing to a gradient; its lse is computed all the same.
+ * A row whose target lies outside [0, vocab) carries no loss: its loss and its
+ * dhidden are 0 and it adds nothing to dweight, whatever the row and the weights
+ * hold; its lse is computed all the same.
  * The backward call takes grad[r] = d(objective) / d(loss[r]) and the lse of
  * the forward call on the same inputs, and writes
  *   dz_v = grad * (exp(l_v - lse) - [v = target]) * (1 - (l_v / softcap)^2),
