@@ -20,6 +20,9 @@ namespace {
 struct AdamCoeff {
     float beta1, rest1, beta2, rest2, eps, decay, size, root, grad_scale;
     uint32_t seed_mul, step_mul;
+    // The hardware's square root takes a subnormal v for 0. That stays below half an ulp
+    // of sqrt(v) root + eps where eps is at least 2^24 times the root of 2^-126.
+    __host__ __device__ bool fast() const { return eps >= root * 0x1p-39f; }
 };
 
 __host__ __device__ inline double power(double b, uint32_t n) {
@@ -242,8 +245,14 @@ __device__ __forceinline__ void step8(const AdamCoeff& c, const Chunk& ch) {
                 // Elements behind the tensor's end are zeros and no largest value.
                 mbig = max(mbig, __builtin_bit_cast(uint32_t, m[e]) & 0x7fffffffu);
                 vbig = max(vbig, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
-                q[e] = updated<true>(c, m[e], v[e], to_f32(p[u][e]));
             }
+        }
+        if (c.fast()) {
+#pragma unroll
+            for (int e = 0; e < kN; ++e) q[e] = updated<true>(c, m[e], v[e], to_f32(p[u][e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < kN; ++e) q[e] = updated<false>(c, m[e], v[e], to_f32(p[u][e]));
         }
         store_param<kFull>(t, i, count[u], q);
         mbig = half_wave_max(mbig);

@@ -125,7 +125,8 @@ int ge_head_loss_backward(ge_head* head, void* stream, const ge_loss_args* args)
  *   g = grad * grad_scale, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g g,
  *   p = p (1 - lr weight_decay) - (lr / (1 - beta1^step)) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * in float32, each operation rounded by itself (with 8-bit states the square root
- * and the quotient are within 1 ulp each). p is the master where there is
+ * and the quotient are within 1 ulp each, unless eps is below 2^-39 / sqrt(1 - beta2^step):
+ * then they are rounded correctly). p is the master where there is
  * one (the parameter is then the master rounded), else the parameter.
  *
  * state_bits 32: m and v are float32. state_bits 8: blocks of GE_ADAMW_BLOCK
