@@ -196,8 +196,9 @@ class Head:
 
     def norm(self, x, weight, bias=None, eps: float = 1e-6, center: bool = True, y=None, mean=None, rstd=None, stream=None):
         """y = (x - mean) * rstd * weight + bias over the last axis of [rows, dim];
-        without ``center`` the mean is left at 0 (root-mean-square norm) and None is
-        returned for it. Returns (y, mean, rstd)."""
+        without ``center`` the mean is left at 0 (root-mean-square norm), a ``mean``
+        that is passed in is filled with zeros, and None is returned for it, which is
+        what ``norm_backward`` knows the norm by. Returns (y, mean, rstd)."""
         rows, dim = self._rows(x, "x")
         a = NormArgs()
         a.weight_dtype = _dtype(weight, "weight")
@@ -214,7 +215,7 @@ class Head:
         a.weight, a.bias = weight.data_ptr(), S._ptr(bias)
         a.y, a.y_stride, a.mean, a.rstd = y.data_ptr(), _stride(y), S._ptr(mean), rstd.data_ptr()
         _check(_library().ge_head_norm(self._h, handle, ctypes.byref(a)))
-        return y, mean, rstd
+        return y, mean if center else None, rstd
 
     def norm_backward(self, grad, x, weight, mean, rstd, bias: bool = False, dx=None, dweight=None, dbias=None,
                       need_input: bool = True, need_weight: bool = True, stream=None):
