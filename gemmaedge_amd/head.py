@@ -5,7 +5,11 @@ with its gradients, and the AdamW step: ctypes over the same library as
 ``sampler``; torch supplies device memory and streams. There is no CPU path.
 
 Calls run on the current torch stream of the tensors' device unless ``stream``
-is given, and outputs that are not passed in are allocated on it.
+is given, and outputs that are not passed in are allocated on it. Ordering that
+stream after the work that fills the inputs is the caller's. A torch.cuda.Stream
+other than the current one is recorded on every tensor of the call, so tensors may
+be dropped right after it; with a raw handle or an ExternalStream the caller keeps
+them until the stream has passed the call.
 """
 from __future__ import annotations
 
@@ -134,23 +138,33 @@ def _on_gpu(t, what: str):
 
 
 def _stream(stream, device):
-    """(handle for the launch, context for the outputs it allocates). The current
-    stream, the usual case, needs no context."""
+    """(handle for the launch, the stream itself if it is not the current one)."""
+    current = torch._C._cuda_getCurrentRawStream(device.index)
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device.index), None
+        return current, None
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=device)
-    return stream.cuda_stream, torch.cuda.stream(stream)
+    return stream.cuda_stream, stream if stream.cuda_stream != current else None
 
 
-def _output(t, what: str, dtype, shape, device, switch):
+def _used(side, *tensors):
+    """Notes that work on ``side`` uses the tensors, so that their memory is not handed
+    out again before it is done. Streams that torch does not own may be gone by the
+    time a tensor is freed: there the caller keeps the tensors."""
+    if side is not None and not isinstance(side, torch.cuda.ExternalStream):
+        for t in tensors:
+            if t is not None:
+                t.record_stream(side)
+
+
+def _output(t, what: str, dtype, shape, device, side):
     """The given output, checked, or a new one of the call's stream."""
     if t is not None:
         _want(t, what, dtype, shape, device)
         return t
-    if switch is None:
+    if side is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    with switch:
+    with torch.cuda.stream(side):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
@@ -205,16 +219,17 @@ class Head:
         _want(weight, "weight", weight.dtype, (dim,), self.device)
         if bias is not None:
             _want(bias, "bias", weight.dtype, (dim,), self.device)
-        handle, switch = _stream(stream, self.device)
-        y = _output(y, "y", self.dtype, (rows, dim), self.device, switch)
-        rstd = _output(rstd, "rstd", torch.float32, (rows,), self.device, switch)
+        handle, side = _stream(stream, self.device)
+        y = _output(y, "y", self.dtype, (rows, dim), self.device, side)
+        rstd = _output(rstd, "rstd", torch.float32, (rows,), self.device, side)
         if center or mean is not None:
-            mean = _output(mean, "mean", torch.float32, (rows,), self.device, switch)
+            mean = _output(mean, "mean", torch.float32, (rows,), self.device, side)
         a.x, a.x_stride, a.rows, a.dim = x.data_ptr(), _stride(x), rows, dim
         a.center, a.eps = int(center), eps
         a.weight, a.bias = weight.data_ptr(), S._ptr(bias)
         a.y, a.y_stride, a.mean, a.rstd = y.data_ptr(), _stride(y), S._ptr(mean), rstd.data_ptr()
         _check(_library().ge_head_norm(self._h, handle, ctypes.byref(a)))
+        _used(side, x, weight, bias, y, mean, rstd)
         return y, mean if center else None, rstd
 
     def norm_backward(self, grad, x, weight, mean, rstd, bias: bool = False, dx=None, dweight=None, dbias=None,
@@ -230,20 +245,21 @@ class Head:
         _want(rstd, "rstd", torch.float32, (rows,), self.device)
         if mean is not None:
             _want(mean, "mean", torch.float32, (rows,), self.device)
-        handle, switch = _stream(stream, self.device)
+        handle, side = _stream(stream, self.device)
         if need_input or dx is not None:
-            dx = _output(dx, "dx", self.dtype, (rows, dim), self.device, switch)
+            dx = _output(dx, "dx", self.dtype, (rows, dim), self.device, side)
             a.dx_stride = _stride(dx)
         if need_weight or dweight is not None:
-            dweight = _output(dweight, "dweight", weight.dtype, (dim,), self.device, switch)
+            dweight = _output(dweight, "dweight", weight.dtype, (dim,), self.device, side)
         if bias or dbias is not None:
-            dbias = _output(dbias, "dbias", weight.dtype, (dim,), self.device, switch)
+            dbias = _output(dbias, "dbias", weight.dtype, (dim,), self.device, side)
         a.x, a.x_stride, a.rows, a.dim = x.data_ptr(), _stride(x), rows, dim
         a.center = int(mean is not None)
         a.weight, a.mean, a.rstd = weight.data_ptr(), S._ptr(mean), rstd.data_ptr()
         a.dy, a.dy_stride, a.dx = grad.data_ptr(), _stride(grad), S._ptr(dx)
         a.dweight, a.dbias = S._ptr(dweight), S._ptr(dbias)
         _check(_library().ge_head_norm_backward(self._h, handle, ctypes.byref(a)))
+        _used(side, grad, x, weight, mean, rstd, dx, dweight, dbias)
         return dx, dweight, dbias
 
     def _loss_args(self, hidden, weight, targets, softcap):
@@ -263,11 +279,12 @@ class Head:
         (int32 [rows]; outside [0, vocab): no loss) over [vocab, dim] weights.
         -loss is the target's log-probability. Returns (loss, lse), float32 [rows]."""
         a, rows, _, _ = self._loss_args(hidden, weight, targets, softcap)
-        handle, switch = _stream(stream, self.device)
-        loss = _output(loss, "loss", torch.float32, (rows,), self.device, switch)
-        lse = _output(lse, "lse", torch.float32, (rows,), self.device, switch)
+        handle, side = _stream(stream, self.device)
+        loss = _output(loss, "loss", torch.float32, (rows,), self.device, side)
+        lse = _output(lse, "lse", torch.float32, (rows,), self.device, side)
         a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
         _check(_library().ge_head_loss(self._h, handle, ctypes.byref(a)))
+        _used(side, hidden, weight, targets, loss, lse)
         return loss, lse
 
     def loss_backward(self, grad, hidden, weight, targets, lse, softcap: float = 0.0, dhidden=None, dweight=None,
@@ -278,15 +295,16 @@ class Head:
         a, rows, dim, vocab = self._loss_args(hidden, weight, targets, softcap)
         _want(grad, "grad", torch.float32, (rows,), self.device)
         _want(lse, "lse", torch.float32, (rows,), self.device)
-        handle, switch = _stream(stream, self.device)
+        handle, side = _stream(stream, self.device)
         if need_hidden or dhidden is not None:
-            dhidden = _output(dhidden, "dhidden", self.dtype, (rows, dim), self.device, switch)
+            dhidden = _output(dhidden, "dhidden", self.dtype, (rows, dim), self.device, side)
             a.dhidden, a.dhidden_stride = dhidden.data_ptr(), _stride(dhidden)
         if need_weight or dweight is not None:
-            dweight = _output(dweight, "dweight", self.dtype, (vocab, dim), self.device, switch)
+            dweight = _output(dweight, "dweight", self.dtype, (vocab, dim), self.device, side)
             a.dweight, a.dweight_stride = dweight.data_ptr(), _stride(dweight)
         a.grad, a.lse = grad.data_ptr(), lse.data_ptr()
         _check(_library().ge_head_loss_backward(self._h, handle, ctypes.byref(a)))
+        _used(side, grad, hidden, weight, targets, lse, dhidden, dweight)
         return dhidden, dweight
 
 
@@ -355,6 +373,7 @@ class AdamW:
         self._table = host.to(device)
         self._args = AdamwArgs(self._table.data_ptr(), size.value, len(params), state_bits)
         self.params, self.grads, self.masters, self.device = params, grads, masters, device
+        self._streams = set()
         self.state_bits, self.seed, self.steps = state_bits, seed, 0
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
 
@@ -379,12 +398,17 @@ class AdamW:
         else:
             _want(device_params, "device_params", torch.uint8, (ctypes.sizeof(AdamwParams),), self.device)
             a.device_params = device_params.data_ptr()
-        handle, _ = _stream(stream, self.device)
+        handle, side = _stream(stream, self.device)
         if torch.cuda.current_device() == self.device.index:
             rc = _library().ge_adamw_step(handle, ctypes.byref(a))
         else:
             with torch.cuda.device(self.device):
                 rc = _library().ge_adamw_step(handle, ctypes.byref(a))
         _check(rc)
+        if side is not None:
+            _used(side, device_params)
+            if handle not in self._streams:  # the list's tensors stay what they are: once a stream
+                self._streams.add(handle)
+                _used(side, self._table, *self.params, *self.grads, *self.masters, *self.m, *self.v, *self.m_scale, *self.v_scale)
         if device_params is None:
             self.steps += 1
