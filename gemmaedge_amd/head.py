@@ -308,12 +308,26 @@ class Head:
         return dhidden, dweight
 
 
+def _disjoint(spans):
+    """Refuses memory that a step writes and that another of its tensors shares.
+    ``spans``: (first byte, end, what it is, whether it is written)."""
+    written, any_ = (0, ""), (0, "")
+    for start, end, what, writes in sorted(spans):
+        for other, name in (written, any_ if writes else written):
+            if start < other:
+                raise ValueError(f"{what} shares memory with {name}")
+        if writes:
+            written = max(written, (end, what))
+        any_ = max(any_, (end, what))
+
+
 class AdamW:
     """AdamW over a list of parameters, one launch a step (ge_adamw_step).
 
     ``params`` and ``grads`` are contiguous float32 or bfloat16 GPU tensors that
     stay where they are (gradients are written into the same buffers before each
-    step); ``masters`` gives float32 copies of some or all parameters (None: none).
+    step) and share no memory with one another: a tied parameter is listed once, with
+    the sum of its gradients. ``masters`` gives float32 copies of some or all parameters (None: none).
     ``state_bits`` is 32 or 8. States are created as zeros unless given: ``m`` and
     ``v`` float32, or float8_e4m3fn and float8_e5m2 with ``m_scale`` and ``v_scale``
     (float32, one for each 256 elements). ``steps`` counts the steps taken.
@@ -347,24 +361,31 @@ class AdamW:
         if any(len(x) != len(params) for x in lists):
             raise ValueError("params, grads, masters and states differ in number")
 
-        def flat(t, what, n, dtype=None):
+        spans = []
+
+        def flat(t, what, n, dtype=None, writes=True):
             if t.device != device or not t.is_contiguous() or t.numel() != n:
                 raise ValueError(f"{what}: {n} contiguous elements on {device} are wanted")
             if dtype is not None and t.dtype != dtype:
                 raise ValueError(f"{what} has dtype {t.dtype}: {dtype} is wanted")
+            if n:
+                spans.append((t.data_ptr(), t.data_ptr() + n * t.element_size(), what, writes))
             return t.data_ptr()
 
         table = (AdamwTensor * len(params))()
         for i, p in enumerate(params):
             t, n = table[i], sizes[i]
             t.param, t.param_dtype, t.n = flat(p, f"params[{i}]", n), _dtype(p, f"params[{i}]"), n
-            t.grad, t.grad_dtype = flat(grads[i], f"grads[{i}]", n), _dtype(grads[i], f"grads[{i}]")
+            t.grad, t.grad_dtype = flat(grads[i], f"grads[{i}]", n, writes=False), _dtype(grads[i], f"grads[{i}]")
             if masters[i] is not None:
                 t.master = flat(masters[i], f"masters[{i}]", n, torch.float32)
+                if t.master == t.param:  # a float32 parameter that is its own master
+                    spans.pop()
             t.m, t.v = flat(self.m[i], f"m[{i}]", n, mt), flat(self.v[i], f"v[{i}]", n, vt)
             if state_bits == 8:
                 t.m_scale = flat(self.m_scale[i], f"m_scale[{i}]", blocks[i], torch.float32)
                 t.v_scale = flat(self.v_scale[i], f"v_scale[{i}]", blocks[i], torch.float32)
+        _disjoint(spans)
         L = _library()
         size = _I64()
         _check(L.ge_adamw_table_bytes(table, len(params), state_bits, ctypes.byref(size)))

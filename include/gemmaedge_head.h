@@ -140,7 +140,10 @@ int ge_head_loss_backward(ge_head* head, void* stream, const ge_loss_args* args)
  * exactly. Values of m below the smallest normal code become that code or 0,
  * likewise at random; values of v below it become that code (a denominator
  * never shrinks). A block whose largest value is below 2^-100 is held as
- * zeros. A non-finite value makes its block NaN. */
+ * zeros. A non-finite value makes its block NaN.
+ *
+ * Memory that the step writes belongs to one tensor of the list and to nothing else
+ * of the call; a float32 parameter may be its own master. */
 #define GE_ADAMW_BLOCK 256
 
 typedef struct ge_adamw_tensor {
