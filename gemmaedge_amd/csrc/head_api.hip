@@ -190,6 +190,7 @@ int ge_adamw_step(void* stream, const ge_adamw_args* args) {
         (chunks > 0 && (!x.table || !ge::head::aligned_to(x.table, 16))))
         return ge::report(GE_ERR_INVALID_ARG, "table of another size than its count gives, NULL or not aligned to 16 bytes");
     if (x.state_bits != 8 && x.state_bits != 32) return ge::report(GE_ERR_INVALID_ARG, "state_bits is neither 8 nor 32");
+    if (!ge::head::aligned_to(x.device_params, 8)) return ge::report(GE_ERR_INVALID_ARG, "device_params is not aligned to 8 bytes");
     if (!x.device_params)
         if (const int rc = ge::head::check_adamw_params(x.params, msg, sizeof(msg))) return ge::report(rc, msg);
     const hipError_t e = ge::head::launch_adamw(x, chunks, static_cast<hipStream_t>(stream));
