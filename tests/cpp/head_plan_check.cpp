@@ -1,0 +1,92 @@
+// How the loss's calls are divided (gemmaedge_amd/csrc/head_validate.h), under the
+// address and undefined-behaviour sanitizers: that the sizes of the tests of several
+// pieces have several pieces, and that what the kernels write fits the workspaces.
+#include <cstdio>
+#include <cstdlib>
+
+#include "../../gemmaedge_amd/csrc/head_validate.h"
+
+using namespace ge::head;
+
+static int failures = 0;
+static char msg[256];
+#define CHECK(c)                                                  \
+    do {                                                          \
+        if (!(c)) {                                               \
+            std::printf("line %d: %s (%s)\n", __LINE__, #c, msg); \
+            if (++failures > 20) std::exit(1);                    \
+        }                                                         \
+    } while (0)
+
+static Capacity capacity(int rows, int dim, int vocab, int dtype) {
+    Capacity c{};
+    c.max_rows = rows;
+    c.max_dim = dim;
+    c.max_vocab = vocab;
+    c.dtype = dtype;
+    c.train = true;
+    size_workspace(c);
+    return c;
+}
+
+static void* at(uintptr_t a) { return reinterpret_cast<void*>(a); }
+
+static LossPlan plan_of(const Capacity& c, int rows, int dim, int vocab, int64_t weight_stride, uintptr_t weight = 4096) {
+    ge_loss_args x{};
+    x.hidden = x.dhidden = x.dweight = at(4096);
+    x.weight = at(weight);
+    x.targets = static_cast<int32_t*>(at(4096));
+    x.loss = x.lse = static_cast<float*>(at(4096));
+    x.grad = static_cast<float*>(at(4096));
+    x.hidden_stride = x.dhidden_stride = x.dweight_stride = dim;
+    x.weight_stride = weight_stride;
+    x.rows = rows;
+    x.dim = dim;
+    x.vocab = vocab;
+    LossPlan p{};
+    CHECK(check_loss(c, x, true, p, msg, sizeof(msg)) == GE_OK);
+    return p;
+}
+
+// What the kernels write and read of the logits' gradient and of its product with the weights.
+static void fits(const Capacity& c, const LossPlan& p, int rows, int dim, int vocab) {
+    const int64_t size = elem_size(c.dtype);
+    CHECK(size * p.rows_pad * p.dz_ld <= c.dlogits);
+    CHECK(p.dz_ld >= round_up(std::min(p.piece, vocab), p.tile_m) && p.rows_pad >= rows);
+    // the last byte of a tile: 256 rows of bf16, 128 of float32, along the vocabulary, 64 across it
+    CHECK((512 / size - 1) * p.dz_ld * size + 128 < 0x7ffffff0);
+    CHECK(4LL * p.splits * rows * round_up(dim, 4) <= c.dhidden);
+}
+
+static void pieces() {
+    struct Case {
+        int rows, dim, vocab, dtype;
+        int64_t weight_stride;
+        uintptr_t weight;
+        int pieces;
+        bool packed;
+    };
+    const Case cases[] = {
+        {4096, 64, 70001, GE_DTYPE_BF16, 64, 4096, 2, false},
+        {2000, 128, 131075, GE_DTYPE_BF16, 128, 4096, 2, false},
+        {4096, 64, 40001, GE_DTYPE_F32, 64, 4096, 2, false},
+        {3000, 33, 100003, GE_DTYPE_F32, 33, 4096, 3, false},
+        {5, 65536, 601, GE_DTYPE_F32, (1 << 21) + 8, 4096 + 12, 2, true},
+    };
+    for (const Case& k : cases) {
+        const Capacity c = capacity(k.rows, k.dim, k.vocab, k.dtype);
+        const LossPlan p = plan_of(c, k.rows, k.dim, k.vocab, k.weight_stride, k.weight);
+        CHECK((k.vocab + p.piece - 1) / p.piece == k.pieces);
+        CHECK(p.pack_w == k.packed);
+        if (k.packed) CHECK((k.vocab + p.pack_piece - 1) / p.pack_piece > 1);
+        if (k.dtype == GE_DTYPE_BF16) CHECK(p.tile_n == 256);
+        fits(c, p, k.rows, k.dim, k.vocab);
+    }
+}
+
+int main() {
+    pieces();
+    if (failures) return 1;
+    std::printf("head plans passed\n");
+    return 0;
+}
