@@ -20,6 +20,7 @@ constexpr int kTile32 = 128;      // of a tile of float32 operands
 constexpr int kSmallRows = 64;    // batches up to this take the small tiles
 constexpr int kSmallTileM = 128;
 constexpr int kSmallTileN = 32;
+constexpr int kMaxStride = 1 << 21;  // elements between rows that tiles are fetched from: 256 rows within 31 bits
 constexpr int kPadK = 64;         // packed rows are padded to this
 constexpr int kPadDz = 64;        // and the logits' gradient's by this: rows a power of two apart share their memory channels
 constexpr int kNormParts = 512;   // workgroups of the norm's backward pass, whose weight gradients are summed last
@@ -162,7 +163,7 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
     // into rows with zeros behind them. float32 ones pass registers and need no
     // alignment. Offsets in a tile have 31 bits.
     auto direct = [&](const void* p, int64_t stride, int rows) {
-        if (rows > 1 && stride > (1 << 21)) return false;
+        if (rows > 1 && stride > kMaxStride) return false;
         return c.dtype == GE_DTYPE_F32 || (aligned_to(p, 16) && (rows <= 1 || stride % 8 == 0) && x.dim % 8 == 0);
     };
     plan.pack_h = !direct(x.hidden, x.hidden_stride, x.rows);
@@ -193,7 +194,8 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
     const int64_t pack_cols = c.wpack / (2 * plan.planes * plan.kpad) / kTileM * kTileM;
     plan.pack_piece = static_cast<int>(plan.pack_w ? std::min(vpad, pack_cols) : vpad);
     if (backward) {
-        const int64_t cols = (c.dlogits / (2LL * plan.planes * plan.rows_pad) - kPadDz) / kTileM * kTileM;
+        // offsets in a tile of the gradient's rows have 31 bits, as in the operands
+        const int64_t cols = std::min<int64_t>(kMaxStride - kTileM, (c.dlogits / (2LL * plan.planes * plan.rows_pad) - kPadDz) / kTileM * kTileM);
         // as few pieces as fit, all of about the same size
         const int64_t most = std::min<int64_t>(std::min<int64_t>(vpad, cols), plan.pack_piece);
         const int64_t pieces = (vpad + most - 1) / most;

@@ -1,8 +1,11 @@
 // How the loss's calls are divided (gemmaedge_amd/csrc/head_validate.h), under the
 // address and undefined-behaviour sanitizers: that the sizes of the tests of several
-// pieces have several pieces, and that what the kernels write fits the workspaces.
+// pieces have several pieces, that what the kernels write fits the workspaces, and that
+// a handle holds no more than its calls can use.
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
+#include <random>
 
 #include "../../gemmaedge_amd/csrc/head_validate.h"
 
@@ -84,8 +87,34 @@ static void pieces() {
     }
 }
 
+static int spread(std::mt19937& r, int hi) {
+    const double u = std::uniform_real_distribution<double>(0.0, std::log(static_cast<double>(hi) + 0.999))(r);
+    return std::max(1, std::min(hi, static_cast<int>(std::exp(u))));
+}
+
+// Handles of every size that can be created, and calls within them.
+static void random_plans() {
+    std::mt19937 r(5);
+    for (int i = 0; i < 200000 && !failures; ++i) {
+        const Capacity c = capacity(spread(r, 1 << 22), spread(r, GE_HEAD_MAX_DIM), spread(r, 1 << 24), static_cast<int>(r() & 1));
+        const int rows = spread(r, c.max_rows), dim = spread(r, c.max_dim), vocab = spread(r, c.max_vocab);
+        const LossPlan p = plan_of(c, rows, dim, vocab, dim + static_cast<int64_t>(r() % 9));
+        fits(c, p, rows, dim, vocab);
+        if (failures)
+            std::printf("rows %d of %d, dim %d of %d, vocab %d of %d, dtype %d: rows of %lld\n", rows, c.max_rows, dim, c.max_dim, vocab,
+                        c.max_vocab, c.dtype, static_cast<long long>(p.dz_ld));
+    }
+    // few rows of a handle for very many, and the largest vocabulary
+    for (int dtype = 0; dtype < 2; ++dtype)
+        for (int rows : {1, 200, 256, 257, 512}) {
+            const Capacity c = capacity(1 << 22, 8, 1 << 24, dtype);
+            fits(c, plan_of(c, rows, 8, 1 << 24, 8), rows, 8, 1 << 24);
+        }
+}
+
 int main() {
     pieces();
+    random_plans();
     if (failures) return 1;
     std::printf("head plans passed\n");
     return 0;
