@@ -23,6 +23,7 @@ constexpr int kSmallTileN = 32;
 constexpr int kMaxStride = 1 << 21;  // elements between rows that tiles are fetched from: 256 rows within 31 bits
 constexpr int kPadK = 64;         // packed rows are padded to this
 constexpr int kPadDz = 64;        // and the logits' gradient's by this: rows a power of two apart share their memory channels
+constexpr int kMaxSplits = 32;    // parts of the vocabulary's sum in the hidden states' gradient
 constexpr int kNormParts = 512;   // workgroups of the norm's backward pass, whose weight gradients are summed last
 constexpr int kNormBlocks = 1280; // and of the forward pass, at most
 
@@ -63,7 +64,9 @@ inline void size_workspace(Capacity& c) {
     const int64_t per_col = 2 * planes * rows_pad;
     c.dlogits = std::min(per_col * (vocab + kPadDz), std::max<int64_t>(per_col * kTileM, 512LL << 20) + per_col * kPadDz);
     const int64_t tiles = (rows_pad / 256) * ((dim + 255) / 256);
-    c.dhidden = 4LL * 256 * 256 * std::max<int64_t>(tiles, 1024);
+    // no call splits its sum into more parts than steps, or 32
+    const int64_t parts = std::min<int64_t>(kMaxSplits, vocab / 64);
+    c.dhidden = 4 * std::min<int64_t>(256 * 256 * std::max<int64_t>(tiles, 1024), parts * rows * round_up(c.max_dim, 4));
     c.norm = 4LL * 2 * kNormParts * c.max_dim;
 }
 
@@ -208,7 +211,7 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
         const int64_t tiles = (x.rows + tile - 1) / tile * ((x.dim + tile - 1) / tile);
         const int64_t steps = plan.piece / 64;
         const int64_t most_bytes = 4 * std::max<int64_t>(x.rows, 1) * round_up(x.dim, 4);
-        const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(32, steps), c.dhidden / most_bytes));
+        const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, steps), c.dhidden / most_bytes));
         int64_t best = INT64_MAX;
         plan.splits = 1;
         for (int64_t s = 1; s <= fit; ++s) {

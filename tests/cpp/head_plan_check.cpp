@@ -112,9 +112,25 @@ static void random_plans() {
         }
 }
 
+// The parts of the hidden states' gradient take what the handle's calls can use, and their number does not depend on it.
+static void parts() {
+    CHECK(capacity(16, 64, 1, GE_DTYPE_BF16).dhidden == 4LL * 4 * 16 * 64);
+    CHECK(capacity(16, 64, 1000, GE_DTYPE_F32).dhidden == 4LL * 16 * 16 * 64);
+    std::mt19937 r(6);
+    for (int i = 0; i < 100000 && !failures; ++i) {
+        Capacity c = capacity(spread(r, 1 << 22), spread(r, GE_HEAD_MAX_DIM), spread(r, 1 << 24), static_cast<int>(r() & 1));
+        const int rows = spread(r, c.max_rows), dim = spread(r, c.max_dim), vocab = spread(r, c.max_vocab);
+        CHECK(c.dhidden <= 4LL * 32 * c.max_rows * round_up(c.max_dim, 4));
+        const int splits = plan_of(c, rows, dim, vocab, dim).splits;
+        c.dhidden = 4LL * 256 * 256 * std::max<int64_t>((c.max_rows + 255LL) / 256 * ((c.max_dim + 255) / 256), 1024);
+        CHECK(plan_of(c, rows, dim, vocab, dim).splits == splits);
+    }
+}
+
 int main() {
     pieces();
     random_plans();
+    parts();
     if (failures) return 1;
     std::printf("head plans passed\n");
     return 0;
