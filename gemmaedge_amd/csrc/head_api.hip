@@ -16,6 +16,7 @@ struct ge_head {
 namespace {
 
 int hip_error(hipError_t e, const char* what) {
+    (void)hipGetLastError();  // reported here: the next launch's check shall not find it
     char msg[256];
     ge::plan_fail(msg, sizeof(msg), 0, "%s: %s", what, hipGetErrorString(e));
     return ge::report(GE_ERR_DEVICE, msg);
