@@ -21,6 +21,7 @@ constexpr int kSmallRows = 64;    // batches up to this take the small tiles
 constexpr int kSmallTileM = 128;
 constexpr int kSmallTileN = 32;
 constexpr int kMaxStride = 1 << 21;  // elements between rows that tiles are fetched from: 256 rows within 31 bits
+constexpr int kMostTiles = (1 << 24) - 1;  // of one launch
 constexpr int kPadK = 64;         // packed rows are padded to this
 constexpr int kPadDz = 64;        // and the logits' gradient's by this: rows a power of two apart share their memory channels
 constexpr int kMaxSplits = 32;    // parts of the vocabulary's sum in the hidden states' gradient
@@ -129,7 +130,7 @@ struct LossPlan {
     int tile_m, tile_n;   // of the logits' product
     int rows_pad;         // rows of the logits' gradient
     int piece;            // vocabulary per piece of the backward (a multiple of kTileM)
-    int pack_piece;       // vocabulary per packed piece of the forward
+    int pack_piece;       // vocabulary per piece of the forward: packed weights, or tiles of a launch
     int splits;           // parts of the vocabulary's sum in dhidden
     int64_t dz_ld;        // elements from row to row of the logits' gradient
 };
@@ -195,7 +196,10 @@ inline int check_loss(const Capacity& c, const ge_loss_args& x, bool backward, L
     plan.rows_pad = static_cast<int>(round_up(std::max(x.rows, 1), 256));  // whole tiles of any width that is chosen
     const int64_t vpad = round_up(x.vocab, kTileM);
     const int64_t pack_cols = c.wpack / (2 * plan.planes * plan.kpad) / kTileM * kTileM;
-    plan.pack_piece = static_cast<int>(plan.pack_w ? std::min(vpad, pack_cols) : vpad);
+    // A launch has less than 2^32 threads, 256 for each tile.
+    const int64_t row_tiles = (std::max(x.rows, 1) + plan.tile_n - 1) / plan.tile_n;
+    const int64_t launch_cols = kMostTiles / row_tiles * plan.tile_m / kTileM * kTileM;
+    plan.pack_piece = static_cast<int>(std::min(std::min(vpad, launch_cols), plan.pack_w ? pack_cols : vpad));
     if (backward) {
         // offsets in a tile of the gradient's rows have 31 bits, as in the operands
         const int64_t cols = std::min<int64_t>(kMaxStride - kTileM, (c.dlogits / (2LL * plan.planes * plan.rows_pad) - kPadDz) / kTileM * kTileM);

@@ -59,6 +59,10 @@ static void fits(const Capacity& c, const LossPlan& p, int rows, int dim, int vo
     // the last byte of a tile: 256 rows of bf16, 128 of float32, along the vocabulary, 64 across it
     CHECK((512 / size - 1) * p.dz_ld * size + 128 < 0x7ffffff0);
     CHECK(4LL * p.splits * rows * round_up(dim, 4) <= c.dhidden);
+    // launches of less than 2^32 threads
+    const int64_t row_tiles = (rows + p.tile_n - 1) / p.tile_n;
+    CHECK(p.pack_piece >= kTileM && p.piece <= p.pack_piece);
+    CHECK(row_tiles * ((std::min(p.pack_piece, vocab) + p.tile_m - 1) / p.tile_m) * 256 < (1LL << 32));
 }
 
 static void pieces() {
