@@ -43,19 +43,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// How logits are capped. kBounded: bf16 operands and caps up to 40; kWide: larger caps, and float32 operands.
-enum Cap { kNone, kBounded, kWide };
+// How logits are capped. kSmall: bf16 operands and caps up to 64; kWide: larger caps, and float32 operands.
+enum Cap { kNone, kSmall, kWide };
 
-// softcap * tanh(z / softcap). bf16 operands, caps up to 40: tanh = 1 - 2 r with
+// softcap * tanh(z / softcap). bf16 operands, caps up to 64: tanh = 1 - 2 r with
 // r = 1 / (exp(2 x) + 1) of the hardware's exp2 and reciprocal, 4e-7 of the cap off at
-// most, far below what the operands' 8 bits leave of z. Above 40 that error would
+// most, far below what the operands' 8 bits leave of z. Above 64 that error would
 // reach the logits, which may be small against the cap: below x = 1 / 4 a series, whose
-// first term is z itself, so that it is 1e-6 of the logit off at most. float32 operands:
+// first term is z itself, so that it is 1e-6 of the logit off at most (a step's backward
+// pass 4 % slower). float32 operands:
 // tanhf, and z itself where x^2 / 3 < u (x has lost bits there if 1 / cap is subnormal).
 struct Softcap {
     float cap, inv, two;  // cap <= 0: none; two = 2 log2(e) / cap
     __device__ __forceinline__ float r(float z) const { return __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f); }
-    __device__ __forceinline__ float bounded_logit(float z) const { return fmaf(r(z), -2.0f * cap, cap); }
+    __device__ __forceinline__ float small_logit(float z) const { return fmaf(r(z), -2.0f * cap, cap); }
     // `z` and its r
     __device__ __forceinline__ float wide_logit(float z, float r) const {
         const float x = z * inv, q = x * x;
@@ -63,6 +64,7 @@ struct Softcap {
         return q < 0.0625f ? fmaf(z, s * q, z) : fmaf(r, -2.0f * cap, cap);
     }
     __device__ __forceinline__ float exact_logit(float z, float tanh) const { return fabsf(z * inv) < 0x1p-12f ? z : cap * tanh; }
+    __device__ __forceinline__ bool small() const { return cap > 0.f && cap <= 64.f; }
     // exp(-2 cap) is a normal number: sums of exp(l - cap) need no largest logit.
     __device__ __forceinline__ bool bounded() const { return cap > 0.f && cap <= 40.f; }
 };
@@ -119,7 +121,7 @@ struct StatsEpi {
     __device__ __forceinline__ float logit(float z) const {
         if (kCap == kNone) return z;
         if (!kFast) return sc.exact_logit(z, tanhf(z * sc.inv));
-        return kCap == kBounded ? sc.bounded_logit(z) : sc.wide_logit(z, sc.r(z));
+        return kCap == kSmall ? sc.small_logit(z) : sc.wide_logit(z, sc.r(z));
     }
     // The largest logit, the sum and the target's logit of the wave's columns.
     template <int kWm, Cap kCap, int kMt, int kNt>
@@ -173,7 +175,7 @@ struct StatsEpi {
 #pragma unroll
                 for (int e = 0; e < 4 * kMt; ++e)
                     if (at == e) x = acc[e >> 2][j][e & 3];
-                target_logit[n_first + j * 16] = sc.bounded_logit(x);
+                target_logit[n_first + j * 16] = sc.small_logit(x);
             }
             float sum = 0.f;
 #pragma unroll
@@ -192,10 +194,10 @@ struct StatsEpi {
         float2* const to = part + wm * kBn + wn * kWn;
         if (!(sc.cap > 0.f))
             columns<kWm, kNone>(acc, s.t, row0, n_first, lane, to);
-        else if (!kFast || !sc.bounded())
+        else if (!kFast || !sc.small())
             columns<kWm, kWide>(acc, s.t, row0, n_first, lane, to);
-        else if (row0 + kWm > vocab)
-            columns<kWm, kBounded>(acc, s.t, row0, n_first, lane, to);
+        else if (!sc.bounded() || row0 + kWm > vocab)
+            columns<kWm, kSmall>(acc, s.t, row0, n_first, lane, to);
         else
             bounded_columns<kWm>(acc, s.t, row0, n_first, lane, to);
         __syncthreads();
@@ -278,14 +280,14 @@ struct GradEpi {
     T* out;  // [rows_pad][ld]
     int64_t ld;
 
-    // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is log2(e) times (-lse, or with kBounded,
+    // (exp(l - lse) - one) (1 - (l / c)^2) g; fast: `lse` is log2(e) times (-lse, or with kSmall,
     // whose l is cap - 2 cap r, cap - lse), `g` with a cap four times g, since the slope is 4 (r - r^2).
     template <Cap kCap>
     __device__ __forceinline__ float dz(float z, float lse, float g, float one) const {
         if (kFast) {
             if (kCap == kNone) return (exp2_fast(fmaf(z, kLog2e, lse)) - one) * g;
             const float r = sc.r(z);
-            const float e = kCap == kBounded ? fmaf(r, -2.0f * kLog2e * sc.cap, lse) : fmaf(sc.wide_logit(z, r), kLog2e, lse);
+            const float e = kCap == kSmall ? fmaf(r, -2.0f * kLog2e * sc.cap, lse) : fmaf(sc.wide_logit(z, r), kLog2e, lse);
             return (exp2_fast(e) - one) * fmaf(-r, r, r) * g;
         }
         const float y = kCap == kNone ? 0.f : tanhf(z * sc.inv);
@@ -323,14 +325,14 @@ struct GradEpi {
             ls[j] = s.lse[j];
             gr[j] = s.grad[j] / s.unit;
             if (kFast) {
-                ls[j] = sc.bounded() ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
+                ls[j] = sc.small() ? (sc.cap - ls[j]) * kLog2e : -ls[j] * kLog2e;
                 if (sc.cap > 0.f) gr[j] *= 4.0f;
             }
         }
         if (!(sc.cap > 0.f))
             store<kWm, kNone>(acc, row0, n_first, lane, s.t, ls, gr);
-        else if (kFast && sc.bounded())
-            store<kWm, kBounded>(acc, row0, n_first, lane, s.t, ls, gr);
+        else if (kFast && sc.small())
+            store<kWm, kSmall>(acc, row0, n_first, lane, s.t, ls, gr);
         else
             store<kWm, kWide>(acc, row0, n_first, lane, s.t, ls, gr);
     }

@@ -95,7 +95,7 @@ int ge_head_norm_backward(ge_head* head, void* stream, const ge_norm_args* args)
  * in units of the largest grad's mantissa, before the two products, whose sums
  * are float32; float32 operands are multiplied in three bf16 planes each, 24
  * bits). With bf16 operands the softcap and the exponentials of both calls use the
- * hardware's exp2 and reciprocal: l is within 4e-7 of the cap for caps up to 40 and
+ * hardware's exp2 and reciprocal: l is within 4e-7 of the cap for caps up to 64 and
  * within 1e-6 of itself for larger ones, beside the products' own sums. A NaN makes the rows it takes part in NaN; so does an infinity in
  * float32, and in bf16 where the formula gives no number. */
 typedef struct ge_loss_args {
