@@ -249,22 +249,27 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* stats, int ld, 
 // The mantissa of the largest finite |grad| of the rows that carry a loss, 1 if there
 // is none. The logits' gradient is held in units of it: where all rows weigh the
 // same, as in a mean, the weight's own rounding to 8 bits would scale whole gradients.
-__global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, const int32_t* targets, int rows, int vocab, float* unit) {
-    __shared__ float red[16];
+template <int kThreads>
+__device__ __forceinline__ void grad_unit(const float* grad, const int32_t* targets, int rows, int vocab, float* unit, int thread) {
+    __shared__ float red[kThreads / 64];
     float m = 0.f;
-    for (int r = threadIdx.x; r < rows; r += 1024) {
+#pragma unroll 4
+    for (int r = thread; r < rows; r += kThreads) {
         const float g = fabsf(grad[r]);
         const int t = targets[r];
         if (t >= 0 && t < vocab && g < __builtin_inff()) m = fmaxf(m, g);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    if ((thread & 63) == 0) red[thread >> 6] = m;
     __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, red[i]);
+    if (thread != 0) return;
+    for (int i = 1; i < kThreads / 64; ++i) m = fmaxf(m, red[i]);
     const uint32_t bits = __builtin_bit_cast(uint32_t, m);
     *unit = m >= 0x1p-126f ? __builtin_bit_cast(float, (bits & 0x007fffffu) | 0x3f800000u) : 1.f;
+}
+__global__ __launch_bounds__(1024) void grad_unit_kernel(const float* grad, const int32_t* targets, int rows, int vocab, float* unit) {
+    grad_unit<1024>(grad, targets, rows, vocab, unit, threadIdx.x);
 }
 
 template <typename T>
@@ -476,16 +481,9 @@ __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int
 }
 
 // Rows into rows that are `kpad` long (a multiple of 8), zeros behind `dim`: 8
-// elements a thread, read at any address, written aligned. With `targets`, rows
-// without a loss are zeros.
+// elements a thread, read at any address, written aligned.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, unsigned rows, int dim, int kpad, T* out,
-                                                   const int32_t* targets, int vocab) {
-    const int d = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
-    const int64_t r = blockIdx.y * blockDim.y + threadIdx.y;
-    if (d >= kpad || r >= rows) return;
-    const int t = targets ? targets[r] : 0;
-    if (t < 0 || t >= vocab) dim = 0;
+__device__ __forceinline__ void pack_unit(const T* in, int64_t ld, int64_t r, int d, int dim, int kpad, T* out) {
     struct Vec {
         T v[8];
     } x;
@@ -497,28 +495,51 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, unsi
     }
     __builtin_memcpy(__builtin_assume_aligned(out + r * kpad + d, 16), &x, sizeof(x));
 }
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, unsigned rows, int dim, int kpad, T* out) {
+    const int d = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    const int64_t r = blockIdx.y * blockDim.y + threadIdx.y;
+    if (d >= kpad || r >= rows) return;
+    pack_unit(in, ld, r, d, dim, kpad, out);
+}
+
+// The same of hidden states, zeros for rows without a loss. The last row of workgroups of
+// a launch that gets `unit` finds the gradient's unit of all `all` rows meanwhile, which
+// takes as long as a launch of its own.
+template <typename T>
+__global__ __launch_bounds__(256) void keep_kernel(const T* in, int64_t ld, unsigned rows, int dim, int kpad, T* out, const int32_t* targets,
+                                                   int vocab, const float* grad, int all, float* unit) {
+    if (unit && blockIdx.y == gridDim.y - 1) {
+        if (blockIdx.x == 0) grad_unit<256>(grad, targets, all, vocab, unit, threadIdx.y * blockDim.x + threadIdx.x);
+        return;
+    }
+    const int d = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    const int64_t r = blockIdx.y * blockDim.y + threadIdx.y;
+    if (d >= kpad || r >= rows) return;
+    const int t = targets[r];
+    pack_unit(in, ld, r, d, t >= 0 && t < vocab ? dim : 0, kpad, out);
+}
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, int64_t ld, int dim) {
     const int d = blockIdx.x * 256 + threadIdx.x;
     if (d < dim) p[blockIdx.y * ld + d] = 0;
 }
 
-// Launches over rows on a grid's y, at most 65,535 at a time.
+// Launches over rows on a grid's y, of at most 65,535: one is left for another use.
 template <typename F>
 void for_rows(int64_t rows, F launch) {
-    for (int64_t r = 0; r < rows; r += 65535) launch(r, static_cast<unsigned>(rows - r < 65535 ? rows - r : 65535));
+    constexpr int64_t kMost = 65534;
+    for (int64_t r = 0; r < rows; r += kMost) launch(r, static_cast<unsigned>(std::min(rows - r, kMost)));
 }
 
-template <typename T>
-void pack(const T* in, int64_t ld, int64_t rows, int dim, int64_t kpad, T* out, const int32_t* targets, int vocab, hipStream_t st) {
+// launch(first row, rows, grid, workgroup) for rows of `kpad`, 8 elements a thread.
+template <typename F>
+void for_units(int64_t rows, int64_t kpad, F launch) {
     const unsigned units = static_cast<unsigned>(kpad / 8);
     unsigned tx = 8;
     while (tx < units && tx < 256) tx *= 2;
     const unsigned ty = 256 / tx;
-    for_rows(rows, [&](int64_t r, unsigned n) {
-        pack_kernel<T><<<dim3((units + tx - 1) / tx, (n + ty - 1) / ty), dim3(tx, ty), 0, st>>>(
-            in + r * ld, ld, n, dim, static_cast<int>(kpad), out + r * kpad, targets ? targets + r : nullptr, vocab);
-    });
+    for_rows(rows, [&](int64_t r, unsigned n) { launch(r, n, dim3((units + tx - 1) / tx, (n + ty - 1) / ty), dim3(tx, ty)); });
 }
 
 template <typename T>
@@ -529,17 +550,30 @@ struct Call {
     hipStream_t st;
     static constexpr bool kFast = sizeof(T) == 2;
 
-    Operand operand(const T* p, int64_t ld, int64_t rows, bool packed, void* to, const int32_t* targets = nullptr) const {
+    Operand operand(const T* p, int64_t ld, int64_t rows, bool packed, void* to) const {
         if (!packed) return Operand{p, ld, (rows - 1) * ld + x.dim};
-        pack(p, ld, rows, x.dim, plan.kpad, static_cast<T*>(to), targets, x.vocab, st);
+        T* const out = static_cast<T*>(to);
+        const int kpad = static_cast<int>(plan.kpad);
+        for_units(rows, plan.kpad, [&](int64_t r, unsigned n, dim3 grid, dim3 block) {
+            pack_kernel<T><<<grid, block, 0, st>>>(p + r * ld, ld, n, x.dim, kpad, out + r * plan.kpad);
+        });
         return Operand{to, plan.kpad, rows * plan.kpad};
     }
-    // kept: rows without a loss read as zeros. The weights' gradient multiplies them by
+    int64_t hidden_ld() const { return x.rows > 1 ? x.hidden_stride : x.dim; }
+    Operand hidden() const { return operand(static_cast<const T*>(x.hidden), hidden_ld(), x.rows, plan.pack_h, b.hpack); }
+    // Rows without a loss read as zeros, for the weights' gradient: it multiplies them by
     // zeros, and padding that is no number would be NaN in it all the same. The copy
     // takes 12 us for 4,096 rows of 2,816 channels, of 14 ms.
-    Operand hidden(bool kept) const {
-        return operand(static_cast<const T*>(x.hidden), x.rows > 1 ? x.hidden_stride : x.dim, x.rows, plan.pack_h || kept, b.hpack,
-                       kept ? x.targets : nullptr);
+    Operand kept_hidden(float* unit) const {
+        const T* const p = static_cast<const T*>(x.hidden);
+        T* const out = reinterpret_cast<T*>(b.hpack);
+        const int64_t ld = hidden_ld();
+        for_units(x.rows, plan.kpad, [&](int64_t r, unsigned n, dim3 grid, dim3 block) {
+            if (r == 0) ++grid.y;
+            keep_kernel<T><<<grid, block, 0, st>>>(p + r * ld, ld, n, x.dim, static_cast<int>(plan.kpad), out + r * plan.kpad, x.targets + r,
+                                                   x.vocab, x.grad, x.rows, r == 0 ? unit : nullptr);
+        });
+        return Operand{b.hpack, plan.kpad, x.rows * plan.kpad};
     }
     // Rows v0 .. v0 + n of the weights.
     Operand weights(int v0, int n) const {
@@ -592,7 +626,7 @@ struct Call {
         }
     }
     void forward() const {
-        const Operand h = hidden(false);
+        const Operand h = hidden();
         const int tiles = (x.vocab + plan.tile_m - 1) / plan.tile_m;
         for (int v0 = 0; v0 < x.vocab; v0 += plan.pack_piece) {
             const int n = std::min(plan.pack_piece, x.vocab - v0);
@@ -605,11 +639,11 @@ struct Call {
         T* dw = static_cast<T*>(x.dweight);
         T* dh = static_cast<T*>(x.dhidden);
         const int64_t dw_ld = x.vocab > 1 ? x.dweight_stride : x.dim, dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
-        const Operand h = hidden(dw != nullptr);
+        float* unit = b.row;
+        const Operand h = dw ? kept_hidden(unit) : hidden();
+        if (!dw) grad_unit_kernel<<<1, 1024, 0, st>>>(x.grad, x.targets, x.rows, x.vocab, unit);
         const int64_t ld = plan.dz_ld;
         constexpr int kTile = sizeof(T) == 4 ? 128 : 256;
-        float* unit = b.row;
-        grad_unit_kernel<<<1, 1024, 0, st>>>(x.grad, x.targets, x.rows, x.vocab, unit);
         const int64_t hld = (x.dim + 3) / 4 * 4;
         const int64_t split = x.rows * hld;
         int splits = plan.splits;

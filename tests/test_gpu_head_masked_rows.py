@@ -17,7 +17,8 @@ def rows_of(ref, at):
 @pytest.mark.parametrize("cap", (0.0, 30.0))
 @pytest.mark.parametrize("dt", ("bf16", "f32"))
 @pytest.mark.parametrize("rows,dim,vocab,pad", [(2, 64, 9, 0), (40, 64, 300, 0), (64, 33, 257, 0), (100, 72, 515, 8), (128, 1001, 130, 0),
-                                                (200, 64, 260, 0), (300, 136, 1005, 3), (513, 256, 700, 0)])
+                                                (200, 64, 260, 0), (300, 136, 1005, 3), (513, 256, 700, 0), (3, 33, 70001, 0),
+                                                (70001, 64, 9, 0)])
 def test_values_that_are_no_numbers_in_rows_without_a_loss(rows, dim, vocab, pad, dt, cap):
     from gemmaedge_amd import head as H
 
