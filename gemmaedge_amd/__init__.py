@@ -1,9 +1,10 @@
 """gemmaedge_amd — MI355X (gfx950) token-sampling path for GemmaEdge.
 
-The product is the HIP library lib/libgemmaedge_sampler.so with the C ABI in
-include/gemmaedge_sampler.h and the C++ drop-in in include/gemmaedge/sampling.h.
-This package is its Python binding (``sampler``) and the synthetic workloads of
-the benchmark configurations (``workloads``).
+The product is the HIP library lib/libgemmaedge_sampler.so with the C ABIs in
+include/gemmaedge_sampler.h (sampling) and include/gemmaedge_head.h (scoring and
+training the answer head) and the C++ drop-in in include/gemmaedge/sampling.h.
+This package is its Python bindings (``sampler``; ``head``, imported by itself) and
+the synthetic workloads of the benchmark configurations (``workloads``).
 """
 from .sampler import (  # noqa: F401
     GE_DTYPE_BF16,

@@ -20,10 +20,10 @@
 // no branch an element, the target's element apart, and with a softcap two
 // exponentials and a reciprocal an element, which are most of their 8 us a tile.
 //
-// 4,096 rows, width 2,816, vocabulary 262,144 in bf16: forward 4.7 ms (1,280
-// TFLOP/s), backward 14.4 ms: logits again 4.9 (1,230), dhidden 4.9 (1,230),
-// dweight 4.5 (1,330); a plain product of this size by the library reaches 1,480.
-// Bound by the matrix cores (54 to 65 % of their cycles at the 2.0 to 2.1 GHz that
+// 4,096 rows, width 2,816, vocabulary 262,144 in bf16: forward 4.7 ms (1,300
+// TFLOP/s), backward 14.3 ms: logits again 4.8 (1,250), dhidden 4.9 (1,240),
+// dweight 4.5 (1,350); a plain product of this size by the library reaches 1,480.
+// Bound by the matrix cores (53 to 66 % of their cycles at the 2.0 to 2.2 GHz that
 // the card holds under them) and the loads that feed them. One row: the weights'
 // bytes, 5.9 TB/s.
 #include <hip/hip_runtime.h>
@@ -50,9 +50,10 @@ enum Cap { kNone, kSmall, kWide };
 // r = 1 / (exp(2 x) + 1) of the hardware's exp2 and reciprocal, 4e-7 of the cap off at
 // most, far below what the operands' 8 bits leave of z. Above 64 that error would
 // reach the logits, which may be small against the cap: below x = 1 / 4 a series, whose
-// first term is z itself, so that it is 1e-6 of the logit off at most (a step's backward
-// pass 4 % slower). float32 operands:
-// tanhf, and z itself where x^2 / 3 < u (x has lost bits there if 1 / cap is subnormal).
+// first term is z itself, so that it is 1e-6 of the logit off at most (1,021 rows, width
+// 1,152, vocabulary 32,003: forward 84 us against 76, backward 284 against 272). float32
+// operands: tanhf, and z itself where x^2 / 3 < u (x has lost bits there if 1 / cap is
+// subnormal).
 struct Softcap {
     float cap, inv, two;  // cap <= 0: none; two = 2 log2(e) / cap
     __device__ __forceinline__ float r(float z) const { return __builtin_amdgcn_rcpf(exp2_fast(z * two) + 1.0f); }
@@ -390,7 +391,7 @@ struct GradEpi {
 
 // dhidden of a piece and part of it: float32, added to what earlier pieces left.
 struct HiddenEpi {
-    float* out;  // [splits][rows_pad][ld]
+    float* out;  // [splits][rows][ld]
     int64_t ld, split;
     int dim, rows;
     bool add;
@@ -563,7 +564,7 @@ struct Call {
     Operand hidden() const { return operand(static_cast<const T*>(x.hidden), hidden_ld(), x.rows, plan.pack_h, b.hpack); }
     // Rows without a loss read as zeros, for the weights' gradient: it multiplies them by
     // zeros, and padding that is no number would be NaN in it all the same. The copy
-    // takes 12 us for 4,096 rows of 2,816 channels, of 14 ms.
+    // takes 22 us for 4,096 rows of 2,816 channels, of 14.3 ms.
     Operand kept_hidden(float* unit) const {
         const T* const p = static_cast<const T*>(x.hidden);
         T* const out = reinterpret_cast<T*>(b.hpack);

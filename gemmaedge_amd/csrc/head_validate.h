@@ -39,7 +39,7 @@ struct Capacity {
     int dtype;
     bool train;
     int64_t stats;    // float2 per row and vocabulary tile
-    int64_t row;      // floats per row: target logits, norm's row sums
+    int64_t row;      // forward: the target's logit of each row; backward: the gradient's unit
     int64_t hpack;    // hidden states in padded rows
     int64_t wpack;    // a piece of the weights in padded rows
     int64_t dlogits;  // the logits' gradient of a piece of the vocabulary

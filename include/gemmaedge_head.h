@@ -35,9 +35,10 @@ typedef struct ge_head ge_head;
 
 /* Create a head on `device` for up to max_rows hidden states of up to max_dim
  * channels and a vocabulary of up to max_vocab, elements of type `dtype`.
- * Allocates every workspace now. train != 0 adds what the backward calls need
- * (about 1 GiB for the loss of large batches; the gradient of the logits is
- * held for a piece of the vocabulary at a time, 512 MiB at most). */
+ * Allocates every workspace now. train != 0 adds what the backward calls need: the
+ * gradient of the logits for a piece of the vocabulary at a time (about 512 MiB for
+ * large batches) and the hidden states' gradient in up to 32 parts (256 MiB, or one
+ * part if that is more); small handles take less. */
 int ge_head_create(int device, int max_rows, int max_dim, int max_vocab, int dtype, int train, ge_head** out);
 
 void ge_head_destroy(ge_head* head);
@@ -48,6 +49,7 @@ void ge_head_destroy(ge_head* head);
  *   with a = dy * weight: dx = rstd * (a - [sum(a) / D] - xhat * sum(a * xhat) / D)
  *   (the bracket with center only), dweight = sum over rows of dy * xhat,
  *   dbias = sum over rows of dy.
+ * The sums are float32: a row whose squares add up past 3.4e38 has an rstd of 0.
  * center = 1 is the layer norm, center = 0 the root-mean-square norm.
  * Rows may be any stride >= dim apart; channels are contiguous. x, y, dy and
  * dx have the handle's dtype; weight, bias, dweight and dbias weight_dtype. */
@@ -93,11 +95,13 @@ int ge_head_norm_backward(ge_head* head, void* stream, const ge_norm_args* args)
  * It computes the logits again, a piece of the vocabulary at a time, and holds
  * dz in the operands' type (bf16: each value rounded once to 8 bits of mantissa,
  * in units of the largest grad's mantissa, before the two products, whose sums
- * are float32; float32 operands are multiplied in three bf16 planes each, 24
- * bits). With bf16 operands the softcap and the exponentials of both calls use the
- * hardware's exp2 and reciprocal: l is within 4e-7 of the cap for caps up to 64 and
- * within 1e-6 of itself for larger ones, beside the products' own sums. A NaN makes the rows it takes part in NaN; so does an infinity in
- * float32, and in bf16 where the formula gives no number. */
+ * are float32; float32 operands are multiplied in three bf16 planes each, 24 bits
+ * of magnitudes from 2^-110 to 3.38e38, bf16's largest). With bf16 operands the
+ * softcap and the exponentials of both calls use the hardware's exp2 and
+ * reciprocal: l is within 4e-7 of the cap for caps up to 64 and within 1e-6 of
+ * itself for larger ones, beside the products' own sums. A NaN makes the rows it
+ * takes part in NaN; so does an infinity in float32, and in bf16 where a logit
+ * becomes +infinity or no number by it. */
 typedef struct ge_loss_args {
     const void* hidden;       /* [rows][dim], hidden_stride elements apart */
     int64_t hidden_stride;
@@ -125,9 +129,9 @@ int ge_head_loss_backward(ge_head* head, void* stream, const ge_loss_args* args)
  *   g = grad * grad_scale, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g g,
  *   p = p (1 - lr weight_decay) - (lr / (1 - beta1^step)) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * in float32, each operation rounded by itself (with 8-bit states the square root
- * and the quotient are within 1 ulp each, unless eps is below 2^-39 / sqrt(1 - beta2^step):
- * then they are rounded correctly). p is the master where there is
- * one (the parameter is then the master rounded), else the parameter.
+ * and the quotient are within 1 ulp each, unless eps is below
+ * 2^-39 / sqrt(1 - beta2^step): then they are rounded correctly). p is the master
+ * where there is one (the parameter is then the master rounded), else the parameter.
  *
  * state_bits 32: m and v are float32. state_bits 8: blocks of GE_ADAMW_BLOCK
  * elements share a float32 scale; m is held in e4m3 in units of its scale =
