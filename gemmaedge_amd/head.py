@@ -403,11 +403,17 @@ class AdamW:
                            step, self.seed)
 
     def device_params(self, lr: Optional[float] = None, grad_scale: float = 1.0, out=None):
-        """The next step's parameters as a uint8 device tensor (``out`` is overwritten
-        if given), and counts the step."""
+        """The next step's parameters, checked, as a uint8 device tensor (``out`` is
+        overwritten if given), and counts the step."""
+        if out is not None:
+            _want(out, "out", torch.uint8, (ctypes.sizeof(AdamwParams),), self.device)
+        params = self._params(self.steps + 1, lr, grad_scale)
+        # a step over no tensors: the checks alone
+        _check(_library().ge_adamw_step(None, ctypes.byref(AdamwArgs(None, 0, 0, self.state_bits, params))))
+        host = torch.frombuffer(bytearray(params), dtype=torch.uint8)
+        out = host.to(self.device) if out is None else out.copy_(host)
         self.steps += 1
-        host = torch.frombuffer(bytearray(self._params(self.steps, lr, grad_scale)), dtype=torch.uint8)
-        return host.to(self.device) if out is None else out.copy_(host)
+        return out
 
     def step(self, lr: Optional[float] = None, grad_scale: float = 1.0, stream=None, device_params=None):
         """One step with the gradients in ``grads``, each times ``grad_scale``. With

@@ -181,7 +181,8 @@ typedef struct ge_adamw_args {
     int32_t state_bits;       /* 32 or 8, as in ge_adamw_table */
     ge_adamw_params params;
     const ge_adamw_params* device_params; /* device memory, read by the launch instead of
-                                             params, for steps replayed from a graph; or NULL */
+                                             params, for steps replayed from a graph; or NULL.
+                                             8-byte aligned; the values are not checked */
 } ge_adamw_args;
 
 /* Checks `count` tensors and writes the size of their table to *bytes. */
