@@ -32,8 +32,7 @@
 
 #include "head_internal.h"
 
-#include "head_gemm.h"
-#include "head_gemm32.h"
+#include "head_tiles.h"
 
 namespace ge {
 namespace head {
@@ -481,30 +480,7 @@ __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int
     out[r * out_ld + d] = from_f32<T>(t >= 0 && t < vocab ? s * *unit : 0.f);
 }
 
-// Rows into rows that are `kpad` long (a multiple of 8), zeros behind `dim`: 8
-// elements a thread, read at any address, written aligned.
-template <typename T>
-__device__ __forceinline__ void pack_unit(const T* in, int64_t ld, int64_t r, int d, int dim, int kpad, T* out) {
-    struct Vec {
-        T v[8];
-    } x;
-    if (d + 8 <= dim) {
-        __builtin_memcpy(&x, in + r * ld + d, sizeof(x));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x.v[e] = d + e < dim ? in[r * ld + d + e] : T(0);
-    }
-    __builtin_memcpy(__builtin_assume_aligned(out + r * kpad + d, 16), &x, sizeof(x));
-}
-template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* in, int64_t ld, unsigned rows, int dim, int kpad, T* out) {
-    const int d = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
-    const int64_t r = blockIdx.y * blockDim.y + threadIdx.y;
-    if (d >= kpad || r >= rows) return;
-    pack_unit(in, ld, r, d, dim, kpad, out);
-}
-
-// The same of hidden states, zeros for rows without a loss. The last row of workgroups of
+// pack_kernel of hidden states, zeros for rows without a loss. The last row of workgroups of
 // a launch that gets `unit` finds the gradient's unit of all `all` rows meanwhile, which
 // takes as long as a launch of its own.
 template <typename T>
@@ -526,23 +502,6 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, int64_t ld,
     if (d < dim) p[blockIdx.y * ld + d] = 0;
 }
 
-// Launches over rows on a grid's y, of at most 65,535: one is left for another use.
-template <typename F>
-void for_rows(int64_t rows, F launch) {
-    constexpr int64_t kMost = 65534;
-    for (int64_t r = 0; r < rows; r += kMost) launch(r, static_cast<unsigned>(std::min(rows - r, kMost)));
-}
-
-// launch(first row, rows, grid, workgroup) for rows of `kpad`, 8 elements a thread.
-template <typename F>
-void for_units(int64_t rows, int64_t kpad, F launch) {
-    const unsigned units = static_cast<unsigned>(kpad / 8);
-    unsigned tx = 8;
-    while (tx < units && tx < 256) tx *= 2;
-    const unsigned ty = 256 / tx;
-    for_rows(rows, [&](int64_t r, unsigned n) { launch(r, n, dim3((units + tx - 1) / tx, (n + ty - 1) / ty), dim3(tx, ty)); });
-}
-
 template <typename T>
 struct Call {
     const ge_loss_args& x;
@@ -552,13 +511,7 @@ struct Call {
     static constexpr bool kFast = sizeof(T) == 2;
 
     Operand operand(const T* p, int64_t ld, int64_t rows, bool packed, void* to) const {
-        if (!packed) return Operand{p, ld, (rows - 1) * ld + x.dim};
-        T* const out = static_cast<T*>(to);
-        const int kpad = static_cast<int>(plan.kpad);
-        for_units(rows, plan.kpad, [&](int64_t r, unsigned n, dim3 grid, dim3 block) {
-            pack_kernel<T><<<grid, block, 0, st>>>(p + r * ld, ld, n, x.dim, kpad, out + r * plan.kpad);
-        });
-        return Operand{to, plan.kpad, rows * plan.kpad};
+        return packed ? packed_rows(p, ld, rows, x.dim, plan.kpad, to, st) : Operand{p, ld, (rows - 1) * ld + x.dim};
     }
     int64_t hidden_ld() const { return x.rows > 1 ? x.hidden_stride : x.dim; }
     Operand hidden() const { return operand(static_cast<const T*>(x.hidden), hidden_ld(), x.rows, plan.pack_h, b.hpack); }
@@ -589,21 +542,7 @@ struct Call {
     }
     template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
     void run(const Operand& a, const Operand& bb, int64_t k, int m, int n, int splits, int group, const Epi& e) const {
-        constexpr int kStep = sizeof(T) == 4 ? kStepK32 : kStepK;
-        GemmArgs g{};
-        g.a = a;
-        g.b = bb;
-        g.k = static_cast<int>(k);
-        g.tiles_m = (m + kBm - 1) / kBm;
-        g.tiles_n = (n + kBn - 1) / kBn;
-        g.steps_per_split = ((g.k + kStep - 1) / kStep + splits - 1) / splits;
-        g.splits = splits;
-        g.group_m = group;
-        const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
-        if constexpr (sizeof(T) == 4)
-            gemm32_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<static_cast<unsigned>(tiles), 256, 0, st>>>(g, e);
-        else
-            gemm_kernel<kBm, kBn, kWm, kWn, kA, kB, Epi><<<static_cast<unsigned>(tiles), 256, 0, st>>>(g, e);
+        run_tiles<T, kBm, kBn, kWm, kWn, kA, kB>(a, bb, k, m, n, splits, group, e, st);
     }
     template <typename Epi>
     void logits(const Operand& w, const Operand& h, int n, const Epi& e) const {

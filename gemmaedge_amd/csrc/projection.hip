@@ -1,0 +1,989 @@
+// A projection shared by all rows with a low-rank adapter for each row's request
+// (include/gemmaedge_projection.h), on the matrix products of head_gemm.h and
+// head_gemm32.h.
+//
+// Forward: u = scale A h of every row first; then the large product, whose
+// epilogue adds B u to the accumulators while they are still in registers: for
+// each adapter that the wave's rows have, in turn, the other rows' u count as
+// zeros. An adapter's rows of B are read once by each tile that needs them, and
+// rows of different requests need no sorting.
+//
+// Backward: dhidden = weight^T dout by the same product across the weights, with A^T
+// du added by the same epilogue (A is transposed first, which is small); du = scale
+// B^T dout and u as low-rank sums over all channels; dA and dB as sums over each
+// adapter's rows, which a launch lists in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <new>
+#include <type_traits>
+
+#include "head_tiles.h"
+#include "projection_validate.h"
+
+namespace ge {
+namespace projection {
+namespace {
+
+using head::bf16x8;
+using head::epi_row;
+using head::f32x4;
+using head::for_rows;
+using head::from_f32;
+using head::GemmArgs;
+using head::Operand;
+using head::s16x4;
+using head::TilePlace;
+using head::to_bf16;
+using head::to_f32;
+using head::u32x4;
+
+struct Buffers {
+    void* hpack;
+    void* wpack;
+    void* u;
+    void* du;
+    float* du_parts;
+    int32_t* order;
+    void* at;
+    void* dpack;
+    float* dhidden;
+};
+
+// ---- low-rank values ------------------------------------------------------------
+//
+// The rows' u and du, `pad` (rank_pad) values each, zeros behind the rank: float32
+// rows, or bf16 in two planes, the value rounded and what that left.
+template <typename T>
+struct Low {
+    T* p;
+    int64_t plane;  // elements from the first plane to the second (bf16)
+    int pad;
+};
+template <typename T>
+__device__ __forceinline__ void low_store(const Low<T>& u, int64_t row, int r, float x) {
+    T* const to = u.p + row * u.pad + r;
+    if constexpr (sizeof(T) == 4) {
+        *to = x;
+    } else {
+        const uint16_t hi = to_bf16(x);
+        to[0] = hi;
+        to[u.plane] = to_bf16(x - to_f32(hi));
+    }
+}
+
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The first n of 8 (or 4) elements, zeros for the others.
+__device__ __forceinline__ bf16x8 keep_below(u32x4 v, int n) {
+    if (n < 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = 2 * e + 1 < n ? v[e] : 2 * e < n ? v[e] & 0xffffu : 0u;
+    }
+    return __builtin_bit_cast(bf16x8, v);
+}
+__device__ __forceinline__ f32x4 keep_below4(u32x4 v, int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? v[e] : 0u;
+    return __builtin_bit_cast(f32x4, v);
+}
+
+// At most 2^31 - 16 bytes from p on, `left` of which are the operand's.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t left) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(max(int64_t{0}, min(left, int64_t{0x7ffffff0}))),
+                                             0x00027000);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(at), 0, 0));
+}
+// 8 bf16 elements. The hardware checks bounds four bytes at a time, so the last of an odd
+// number of elements has to be loaded by itself; `odd` where there can be one.
+__device__ __forceinline__ u32x4 load8(__amdgpu_buffer_rsrc_t rs, uint32_t at, bool odd) {
+    if (!odd) return load16(rs, at);
+    u32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint16_t lo = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(at + 4 * e), 0, 0);
+        const uint16_t hi = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(at + 4 * e + 2), 0, 0);
+        v[e] = lo | static_cast<uint32_t>(hi) << 16;
+    }
+    return v;
+}
+
+// Adapters' rows along the rank, one for each row of the large product's M side.
+template <typename T>
+struct Adapters {
+    const T* table;       // [adapters][m][rank]
+    int64_t m;
+    int rank, adapters;   // adapters 0: none
+    const int32_t* ids;   // [rows]
+    Low<T> u;
+};
+
+// Column j's accumulators stay where they are until here: see the products' kernel, whose
+// large tiles have no registers to read them all into. They are not written again:
+// with other values in them the compiler moves some between the product's steps,
+// whose instructions it knows nothing of.
+template <int kMt, int kNt>
+__device__ __forceinline__ void hold(f32x4 (&acc)[kMt][kNt], int j) {
+    if constexpr (kMt * kNt >= 32) {
+#pragma unroll
+        for (int t = 0; t < kMt; ++t) asm volatile("" : "+a"(acc[t][j]));
+    }
+}
+
+// Ranks that a fragment of an adapter's rows has, and of how many the registers keep them.
+template <typename T>
+constexpr int kFragRanks = sizeof(T) == 2 ? 32 : 16;
+constexpr int kKept = 2;
+
+// An adapter's rows of a wave, as the matrix instructions take them: kept while the
+// columns that follow have the same adapter.
+template <typename T, int kMt>
+struct TableRows {
+    typename std::conditional<sizeof(T) == 2, bf16x8, f32x4>::type f[kKept][kMt];
+    int k = -1, from = -1;
+    template <bool kAAlong>
+    __device__ __forceinline__ void load(const Adapters<T>& x, int64_t m0, int adapter, int r0, int lane) {
+        if (adapter == k && r0 == from) return;
+        k = adapter;
+        from = r0;
+        constexpr int kEach = sizeof(T) == 2 ? 8 : 4;  // ranks of a lane
+        const int i = lane & 15, g = lane >> 4;
+        const int64_t first = adapter * x.m + m0;
+        // Rows past the last lie behind the resource's end.
+        const auto rs = resource(x.table + first * x.rank, (x.m - m0) * x.rank * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+        for (int c = 0; c < kKept; ++c) {
+            const int r = r0 + c * kFragRanks<T> + kEach * g, left = x.rank - r;
+            if (r0 + c * kFragRanks<T> >= x.rank) break;
+#pragma unroll
+            for (int t = 0; t < kMt; ++t) {
+                const int row = kAAlong ? epi_row(t, i) : t * 16 + i;
+                const uint32_t at = left > 0 ? static_cast<uint32_t>(row * x.rank + r) * sizeof(T) : 0x80000000u;
+                if constexpr (sizeof(T) == 2)
+                    f[c][t] = keep_below(load8(rs, at, x.rank & 1), left);
+                else
+                    f[c][t] = keep_below4(load16(rs, at), left);
+            }
+        }
+    }
+};
+
+// Adds table[k] u to a column of accumulators, whose lanes i, i + 16, ... have row n = n0 + i of
+// adapter k = id, and whose first row along M is m0. An adapter's products with the rows that
+// are not its own are left out, not added as zeros: an infinity in one request's
+// adapter stays there.
+template <bool kAAlong, typename T, int kMt>
+__device__ __forceinline__ void add_adapters(const Adapters<T>& x, TableRows<T, kMt>& rows, f32x4 (&acc)[kMt], int64_t m0, int id, int64_t n,
+                                             int lane) {
+    constexpr int kStep = kFragRanks<T>;
+    const int g = lane >> 4;
+    uint64_t left = __ballot(id >= 0);
+    while (left) {
+        const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const bool mine = id == k;
+        left &= ~__ballot(mine);
+        const T* const u = x.u.p + n * x.u.pad + (kStep / 4) * g;
+        for (int r0 = 0; r0 < x.rank; r0 += kKept * kStep) {
+            u32x4 p[kKept][2];
+#pragma unroll
+            for (int c = 0; c < kKept; ++c) {
+                p[c][0] = p[c][1] = u32x4{0, 0, 0, 0};
+                const int r = r0 + c * kStep;
+                if (mine && r < x.rank) {
+                    p[c][0] = *reinterpret_cast<const u32x4*>(u + r);
+                    if constexpr (sizeof(T) == 2) p[c][1] = *reinterpret_cast<const u32x4*>(u + x.u.plane + r);
+                }
+            }
+            rows.template load<kAAlong>(x, m0, k, r0, lane);
+#pragma unroll
+            for (int c = 0; c < kKept; ++c) {
+                if (r0 + c * kStep >= x.rank) break;
+#pragma unroll
+                for (int t = 0; t < kMt; ++t) {
+                    f32x4 y{0.f, 0.f, 0.f, 0.f};
+                    if constexpr (sizeof(T) == 2) {
+                        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows.f[c][t], __builtin_bit_cast(bf16x8, p[c][1]), y, 0, 0, 0);
+                        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows.f[c][t], __builtin_bit_cast(bf16x8, p[c][0]), y, 0, 0, 0);
+                    } else {
+                        const f32x4 fu = __builtin_bit_cast(f32x4, p[c][0]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.f[c][t][e], fu[e], y, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][e] += mine ? y[e] : 0.f;
+                }
+            }
+        }
+    }
+}
+
+// The adapters of a lane's rows, -1: none.
+template <int kNt>
+__device__ __forceinline__ void load_ids(const int32_t* ids, int adapters, int64_t n_first, int rows, int (&id)[kNt]) {
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) {
+        id[j] = -1;
+        if (adapters && n_first + j * 16 < rows) id[j] = ids[n_first + j * 16];
+        if (id[j] >= adapters) id[j] = -1;
+    }
+}
+
+template <typename O, int kCount>
+__device__ __forceinline__ void store_out(O* o, const float (&x)[kCount], int n) {
+    struct Vec {
+        O v[kCount];
+    } q;
+#pragma unroll
+    for (int e = 0; e < kCount; ++e) q.v[e] = from_f32<O>(x[e]);
+    if (n >= kCount) {
+        __builtin_memcpy(o, &q, sizeof(q));
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e)
+            if (e < n) o[e] = q.v[e];
+    }
+}
+
+// The projection's outputs: a lane has 8 neighbours of a row in every two tiles.
+template <typename T, typename O>
+struct OutEpi {
+    Adapters<T> low;
+    int rows, m;   // m: outputs from the product's first row on
+    int v0;        // number of that row
+    O* out;        // of row 0 and output v0
+    int64_t ld;
+
+    template <int kNt>
+    struct State {
+        int id[kNt];
+    };
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State<kNt> prepare(int, int col0, int lane) const {
+        State<kNt> s;
+        load_ids(low.ids, low.adapters, col0 + (lane & 15), rows, s.id);
+        return s;
+    }
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State<kNt>& s, int m0, int n0, TilePlace, int wm, int wn, int lane,
+                                           float2*) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+        const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
+        TableRows<T, kMt> table;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            hold(acc, j);
+            const int n = col0 + j * 16 + (lane & 15);
+            f32x4 y[kMt];
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
+            if (low.adapters && row0 < m) add_adapters<kAAlong>(low, table, y, v0 + row0, s.id[j], n, lane);
+            if (n >= rows) continue;
+            const int v = row0 + (lane >> 4) * 8;
+            O* const o = out + n * ld + v;
+#pragma unroll
+            for (int i = 0; i < kMt; i += 2) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = y[i + (e >> 2)][e & 3];
+                if (v + i * 16 < m) store_out(o + i * 16, x, m - v - i * 16);
+            }
+        }
+    }
+};
+
+// dhidden of a piece of the outputs and part of it: rounded into the result if that is
+// all of the sum, else in float32, added to what earlier pieces left.
+template <typename T, bool kDirect>
+struct HiddenEpi {
+    Adapters<T> low;  // of the first part of the first piece
+    int rows, dim;
+    typename std::conditional<kDirect, T, float>::type* out;  // [splits][rows][ld]
+    int64_t ld, split;
+    bool add;
+
+    template <int kNt>
+    struct State {
+        int id[kNt];
+    };
+    template <int kWm, int kNt>
+    __device__ __forceinline__ State<kNt> prepare(int, int col0, int lane) const {
+        State<kNt> s;
+        load_ids(low.ids, low.adapters, col0 + (lane & 15), rows, s.id);
+        return s;
+    }
+    template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, int kMt, int kNt>
+    __device__ __forceinline__ void finish(f32x4 (&acc)[kMt][kNt], const State<kNt>& s, int m0, int n0, TilePlace place, int wm, int wn,
+                                           int lane, float2*) const {
+        constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
+        const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
+        TableRows<T, kMt> table;
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            hold(acc, j);
+            const int64_t n = col0 + j * 16 + (lane & 15);
+            f32x4 y[kMt];
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
+            if (low.adapters && place.split == 0 && row0 < dim) add_adapters<kAAlong>(low, table, y, row0, s.id[j], n, lane);
+            if (n >= rows) continue;
+            const int d0 = row0 + 4 * (lane >> 4);
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) {
+                const int d = d0 + i * 16;
+                if constexpr (kDirect) {
+                    const float x[4] = {y[i][0], y[i][1], y[i][2], y[i][3]};
+                    if (d < dim) store_out(out + n * ld + d, x, dim - d);
+                } else {  // ld is a multiple of 4 above dim
+                    f32x4* const o = reinterpret_cast<f32x4*>(out + place.split * split + n * ld + d);
+                    if (d < dim) *o = add ? *o + y[i] : y[i];
+                }
+            }
+        }
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int64_t ld, int64_t split, int splits, int dim, T* out,
+                                                         int64_t out_ld) {
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d >= dim) return;
+    const int64_t r = blockIdx.y;
+    float s = 0.f;
+    for (int i = 0; i < splits; ++i) s += parts[i * split + r * ld + d];
+    out[r * out_ld + d] = from_f32<T>(s);
+}
+
+// ---- sums of a row's channels with each rank -------------------------------------
+//
+// y[n][r] = scale[k] * sum over c of x[n][c] * table[k](r, c), k the row's adapter.
+// kAlong: the table is [adapters][rank][cols] (u from A); else [adapters][cols][rank]
+// (du from B), and its tiles are transposed on their way from LDS, like those of
+// the large product. A workgroup takes 16 rows and one of the adapters they have (at most 16:
+// a grid's y), its four waves every fourth step of a part of the sum.
+template <typename T>
+struct SumArgs {
+    const T* x;
+    int64_t ld;
+    int rows, cols;
+    const T* table;
+    const float* scale;
+    const int32_t* ids;
+    int adapters, rank;
+    Low<T> y;
+    float* parts;   // [splits][rows][pad], or NULL: the only part
+    int splits, steps_per_split;
+};
+
+constexpr int kSumStep = 32;  // channels of a wave's step
+
+// The slot-th of the adapters that 16 rows have; INT_MAX: they have fewer.
+__device__ __forceinline__ int slot_adapter(int id, int slot) {
+    int k = -1;
+    for (int s = 0; s <= slot && k != INT_MAX; ++s) k = wave_min(id > k ? id : INT_MAX);
+    return k;
+}
+
+template <typename T, bool kAlong, int kR>
+__global__ __launch_bounds__(256) void low_sum_kernel(SumArgs<T> s) {
+    constexpr int kRanks = kR * 16;
+    __shared__ __align__(16) float red[4][kRanks][17];
+    constexpr int kRow = kRanks + 8;  // bf16 elements of a transposed tile's row in LDS
+    __shared__ __align__(16) uint16_t tile[!kAlong && sizeof(T) == 2 ? 4 * kSumStep * kRow : 8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * kRowTile;
+    const int n = n0 + i;
+    int id = n < s.rows ? s.ids[n] : -1;
+    if (id < 0 || id >= s.adapters) id = -1;
+    const int k = slot_adapter(id, blockIdx.y);
+    const int split = blockIdx.z % s.splits, r0 = blockIdx.z / s.splits * kRanks;
+    const T* const xr = s.x + min(n, s.rows - 1) * s.ld;
+    f32x4 acc[kR];
+#pragma unroll
+    for (int t = 0; t < kR; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (k == INT_MAX) {
+        // Rows without an adapter have zeros; the first slot writes them.
+        if (blockIdx.y != 0) return;
+    } else {
+        const int64_t size = static_cast<int64_t>(s.rank) * s.cols;
+        const T* const table = s.table + k * size;
+        const int first = split * s.steps_per_split;
+        const int last = min((s.cols + kSumStep - 1) / kSumStep, first + s.steps_per_split);
+        uint16_t* const my = tile + wave * kSumStep * kRow;
+        for (int step = first + wave; step < last; step += 4) {
+            const int c0 = step * kSumStep;
+            if constexpr (sizeof(T) == 2) {
+                const int c = c0 + 8 * g, left = s.cols - c;
+                u32x4 raw{0, 0, 0, 0};
+                if (left >= 8) {
+                    __builtin_memcpy(&raw, xr + c, 16);
+                } else if (left > 0) {
+                    struct {
+                        uint16_t v[8];
+                    } q{};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) q.v[e] = xr[c + e];
+                    raw = __builtin_bit_cast(u32x4, q);
+                }
+                const bf16x8 fx = __builtin_bit_cast(bf16x8, raw);
+                if constexpr (kAlong) {
+#pragma unroll
+                    for (int t = 0; t < kR; ++t) {
+                        const int r = r0 + t * 16 + i;
+                        u32x4 w{0, 0, 0, 0};
+                        if (r < s.rank) {
+                            const T* const p = table + static_cast<int64_t>(r) * s.cols + c;
+                            if (left >= 8) {
+                                __builtin_memcpy(&w, p, 16);
+                            } else if (left > 0) {
+                                struct {
+                                    uint16_t v[8];
+                                } q{};
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (e < left) q.v[e] = p[e];
+                                w = __builtin_bit_cast(u32x4, q);
+                            }
+                        }
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), fx, acc[t], 0, 0, 0);
+                    }
+                } else {
+                    // 32 channels of the ranks, 8 a lane; columns past the rank belong to the next
+                    // channel and to outputs that nobody reads.
+                    const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank, (s.cols - c0) * static_cast<int64_t>(s.rank) * 2);
+                    constexpr int kPerRow = kRanks / 8;
+#pragma unroll
+                    for (int q = 0; q < kR; ++q) {
+                        const int at = q * 64 + lane, row = at / kPerRow, col = at % kPerRow * 8;
+                        *reinterpret_cast<u32x4*>(my + row * kRow + col) =
+                            load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    typedef __attribute__((address_space(3))) s16x4* lds4;
+#pragma unroll
+                    for (int t = 0; t < kR; ++t) {
+                        uint16_t* const p = my + (8 * g + (i >> 2)) * kRow + t * 16 + (i & 3) * 4;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * kRow));
+                        const bf16x8 fw = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc[t], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
+            } else {
+                const auto rs_x = resource(xr, s.cols * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = c0 + h * 16 + 4 * g;
+                    const f32x4 fx = __builtin_bit_cast(f32x4, load16(rs_x, static_cast<uint32_t>(c) * 4));
+#pragma unroll
+                    for (int t = 0; t < kR; ++t) {
+                        const int r = r0 + t * 16 + i;
+                        f32x4 fw{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (r < s.rank && c + e < s.cols)
+                                fw[e] = kAlong ? table[static_cast<int64_t>(r) * s.cols + c + e] : table[static_cast<int64_t>(c + e) * s.rank + r];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[e], fx[e], acc[t], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kR; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][t * 16 + 4 * g + e][i] = acc[t][e];
+    // The row's adapter is this workgroup's, or the row has none and this is the first.
+    __shared__ int owner[16];
+    if (threadIdx.x < 16) owner[threadIdx.x] = id;
+    __syncthreads();
+    for (int at = threadIdx.x; at < kRanks * kRowTile; at += 256) {
+        const int c = at / kRanks, r = at % kRanks;
+        const int who = owner[c];
+        if (n0 + c >= s.rows || r0 + r >= s.y.pad || !(who == k || (who < 0 && blockIdx.y == 0))) continue;
+        float x = 0.f;
+        if (who >= 0 && r0 + r < s.rank) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x += red[w][r][c];
+        }
+        if (s.parts)
+            s.parts[(static_cast<int64_t>(split) * s.rows + n0 + c) * s.y.pad + r0 + r] = x;
+        else
+            low_store(s.y, n0 + c, r0 + r, who >= 0 ? x * s.scale[who] : 0.f);
+    }
+}
+
+// The parts in order, times the row's scale.
+template <typename T>
+__global__ __launch_bounds__(256) void low_join_kernel(SumArgs<T> s) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(s.rows) * s.y.pad;
+    if (at >= all) return;
+    const int64_t n = at / s.y.pad;
+    float x = 0.f;
+    for (int i = 0; i < s.splits; ++i) x += s.parts[i * all + at];
+    const int id = s.ids[n];
+    low_store(s.y, n, static_cast<int>(at % s.y.pad), id >= 0 && id < s.adapters ? x * s.scale[id] : 0.f);
+}
+
+// ---- an adapter's rows -------------------------------------------------------------
+//
+// begin[k] .. begin[k + 1] of `order` are the rows of adapter k, in their order: a workgroup per
+// adapter counts the rows of those before it and lists its own.
+__global__ __launch_bounds__(1024) void order_kernel(const int32_t* ids, int rows, int adapters, int32_t* begin, int32_t* order) {
+    __shared__ int sums[16];
+    const int k = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0;
+    for (int n = threadIdx.x; n < rows; n += 1024) before += ids[n] >= 0 && ids[n] < k;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+    if (lane == 0) sums[wave] = before;
+    __syncthreads();
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) at += sums[w];
+    __syncthreads();
+    if (threadIdx.x == 0) begin[k] = at;
+    for (int base = 0; base < rows; base += 1024) {
+        const int n = base + threadIdx.x;
+        const bool mine = n < rows && ids[n] == k;
+        const uint64_t all = __ballot(mine);
+        if (lane == 0) sums[wave] = __popcll(all);
+        __syncthreads();
+        int to = at;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) to += sums[w];
+            at += sums[w];
+        }
+        if (mine) order[to + __popcll(all & ((1ull << lane) - 1))] = n;
+        __syncthreads();
+    }
+    if (k == adapters - 1 && threadIdx.x == 0) begin[adapters] = at;
+}
+
+// ---- sums over an adapter's rows ----------------------------------------------------
+//
+// g[k](r, c) = sum over the rows n of adapter k of x[n][c] * y[n][r], stored as
+// [adapters][cols][rank] (kRanksLast: dB, of dout and u) or [adapters][rank][cols] (dA, of
+// hidden and du). bf16 operands are both across the sum: they go through LDS, transposed on
+// their way to the registers. A wave takes 64 columns; the matrix instructions' M side,
+// of which a lane has 4 neighbours, is the side that lies together in memory.
+template <typename T>
+struct OuterArgs {
+    const T* x;
+    int64_t ld;
+    int cols, rank;
+    Low<T> y;
+    const int32_t* begin;
+    const int32_t* order;
+    T* out;
+};
+
+constexpr int kOuterCols = 64;  // of a wave
+
+template <typename T, bool kRanksLast, int kR>
+__global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
+    constexpr int kRanks = kR * 16, kC = kOuterCols / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int k = blockIdx.z, r0 = blockIdx.y * kRanks;
+    const int c0 = (blockIdx.x * 4 + wave) * kOuterCols;
+    const int from = s.begin[k], count = s.begin[k + 1] - from;
+    const int32_t* const rows = s.order + from;
+    f32x4 acc[kC][kR];
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(T) == 2) {
+        constexpr int kXRow = kOuterCols + 8, kYRow = kRanks + 8;
+        __shared__ __align__(16) uint16_t xs[4][32 * kXRow];
+        __shared__ __align__(16) uint16_t ys[2][32 * kYRow];
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        auto frag = [&](uint16_t* base, int ld, int col) {
+            uint16_t* const p = base + (8 * g + (i >> 2)) * ld + col + (i & 3) * 4;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ld));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        for (int n0 = 0; n0 < count; n0 += 32) {
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int at = q * 8 + (lane >> 3), c = c0 + (lane & 7) * 8;
+                struct {
+                    uint16_t v[8];
+                } v{};
+                if (n0 + at < count && c < s.cols) {
+                    const T* const p = s.x + rows[n0 + at] * s.ld + c;
+                    if (c + 8 <= s.cols) {
+                        __builtin_memcpy(&v, p, 16);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (c + e < s.cols) v.v[e] = p[e];
+                    }
+                }
+                *reinterpret_cast<u32x4*>(&xs[wave][at * kXRow + (lane & 7) * 8]) = __builtin_bit_cast(u32x4, v);
+            }
+            for (int at = threadIdx.x; at < 2 * 32 * kRanks / 8; at += 256) {
+                const int plane = at / (32 * kRanks / 8), u = at % (32 * kRanks / 8), row = u / (kRanks / 8), col = u % (kRanks / 8) * 8;
+                u32x4 v{0, 0, 0, 0};
+                if (n0 + row < count && r0 + col < s.y.pad)
+                    v = *reinterpret_cast<const u32x4*>(s.y.p + plane * s.y.plane + static_cast<int64_t>(rows[n0 + row]) * s.y.pad + r0 + col);
+                *reinterpret_cast<u32x4*>(&ys[plane][row * kYRow + col]) = v;
+            }
+            __syncthreads();
+            bf16x8 fy[2][kR];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int r = 0; r < kR; ++r) fy[p][r] = frag(ys[p], kYRow, r * 16);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                const bf16x8 fx = frag(xs[wave], kXRow, c * 16);
+#pragma unroll
+                for (int p = 1; p >= 0; --p)
+#pragma unroll
+                    for (int r = 0; r < kR; ++r)
+                        acc[c][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fy[p][r], fx, acc[c][r], 0, 0, 0)
+                                               : __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fy[p][r], acc[c][r], 0, 0, 0);
+            }
+        }
+    } else {
+        for (int n0 = 0; n0 < count; n0 += 4) {
+            const bool there = n0 + g < count;
+            const int64_t n = rows[min(n0 + g, count - 1)];
+            float fx[kC], fy[kR];
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                const int col = c0 + c * 16 + i;
+                fx[c] = there && col < s.cols ? s.x[n * s.ld + col] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < kR; ++r) {
+                const int at = r0 + r * 16 + i;
+                fy[r] = there && at < s.y.pad ? s.y.p[n * s.y.pad + at] : 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int r = 0; r < kR; ++r)
+                    acc[c][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x4f32(fy[r], fx[c], acc[c][r], 0, 0, 0)
+                                           : __builtin_amdgcn_mfma_f32_16x16x4f32(fx[c], fy[r], acc[c][r], 0, 0, 0);
+        }
+    }
+    T* const out = s.out + static_cast<int64_t>(k) * s.cols * s.rank;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            const float x[4] = {acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]};
+            const int col = c0 + c * 16 + (kRanksLast ? i : 4 * g), rank = r0 + r * 16 + (kRanksLast ? 4 * g : i);
+            if (col >= s.cols || rank >= s.rank) continue;
+            if (kRanksLast)
+                store_out(out + static_cast<int64_t>(col) * s.rank + rank, x, s.rank - rank);
+            else
+                store_out(out + static_cast<int64_t>(rank) * s.cols + col, x, s.cols - col);
+        }
+}
+
+// A of the adapters that have rows, transposed: [adapters][dim][rank].
+template <typename T>
+__global__ __launch_bounds__(256) void transpose_kernel(const T* a, int rank, int dim, const int32_t* begin, T* to) {
+    const int k = blockIdx.y;
+    if (begin[k] == begin[k + 1]) return;
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d >= dim) return;
+    const T* const p = a + static_cast<int64_t>(k) * rank * dim + d;
+    T* const q = to + (static_cast<int64_t>(k) * dim + d) * rank;
+    for (int r = 0; r < rank; ++r) q[r] = p[static_cast<int64_t>(r) * dim];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at < n) p[at] = T(0);
+}
+template <typename T>
+void zero(T* p, int64_t n, hipStream_t st) {
+    constexpr int64_t kMost = int64_t{256} << 22;
+    for (int64_t at = 0; at < n; at += kMost) zero_kernel<T><<<static_cast<unsigned>((std::min(n - at, kMost) + 255) / 256), 256, 0, st>>>(p + at, std::min(n - at, kMost));
+}
+
+// f(rank tiles of a workgroup)
+template <typename F>
+void by_rank(int rank, F f) {
+    if (rank <= 16)
+        f(std::integral_constant<int, 1>{});
+    else if (rank <= 32)
+        f(std::integral_constant<int, 2>{});
+    else
+        f(std::integral_constant<int, 4>{});
+}
+
+template <typename T>
+struct Call {
+    const ge_project_args& x;
+    const Plan& plan;
+    const Buffers& b;
+    hipStream_t st;
+
+    int64_t hidden_ld() const { return x.rows > 1 ? x.hidden_stride : x.dim; }
+    int64_t dout_ld() const { return x.rows > 1 ? x.dout_stride : x.out_dim; }
+    Operand rows(const void* p, int64_t ld, int64_t n, int dim, bool packed, int64_t kpad, void* to) const {
+        return packed ? head::packed_rows(static_cast<const T*>(p), ld, n, dim, kpad, to, st) : Operand{p, ld, (n - 1) * ld + dim};
+    }
+    Operand weights(int v0, int n) const {
+        const int64_t ld = x.out_dim > 1 ? x.weight_stride : x.dim;
+        return rows(static_cast<const T*>(x.weight) + v0 * ld, ld, n, x.dim, plan.pack_w, plan.kpad, b.wpack);
+    }
+    template <int kBm, int kBn, int kWm, int kWn, bool kA, bool kB, typename Epi>
+    void run(const Operand& a, const Operand& bb, int64_t k, int m, int n, int splits, int group, const Epi& e) const {
+        head::run_tiles<T, kBm, kBn, kWm, kWn, kA, kB>(a, bb, k, m, n, splits, group, e, st);
+    }
+    Low<T> low(void* p) const {
+        const int pad = static_cast<int>(rank_pad(x.rank));
+        return Low<T>{static_cast<T*>(p), static_cast<int64_t>(x.rows) * pad, pad};
+    }
+    Adapters<T> adapters(const void* table, int64_t m, void* u) const {
+        if (x.adapters == 0) return Adapters<T>{};
+        return Adapters<T>{static_cast<const T*>(table), m, x.rank, x.adapters, x.adapter, low(u)};
+    }
+    template <bool kAlong>
+    void low_sum(const void* in, int64_t ld, int cols, const void* table, void* to, int splits) const {
+        SumArgs<T> s{static_cast<const T*>(in), ld, x.rows, cols, static_cast<const T*>(table), x.scale, x.adapter, x.adapters, x.rank,
+                     low(to), splits > 1 ? b.du_parts : nullptr, splits, 0};
+        s.steps_per_split = ((cols + kSumStep - 1) / kSumStep + splits - 1) / splits;
+        const int slots = std::min(kRowTile, x.adapters);
+        by_rank(x.rank, [&](auto r) {
+            constexpr int kR = decltype(r)::value;
+            const int ranks = (s.y.pad + kR * 16 - 1) / (kR * 16);  // the padding too
+            low_sum_kernel<T, kAlong, kR><<<dim3((x.rows + kRowTile - 1) / kRowTile, slots, splits * ranks), 256, 0, st>>>(s);
+        });
+        if (splits > 1) low_join_kernel<T><<<static_cast<unsigned>((static_cast<int64_t>(x.rows) * s.y.pad + 255) / 256), 256, 0, st>>>(s);
+    }
+    template <bool kRanksLast>
+    void outer(const void* in, int64_t ld, int cols, void* y, void* out) const {
+        OuterArgs<T> s{static_cast<const T*>(in), ld, cols, x.rank, low(y), b.order, b.order + x.adapters + 1, static_cast<T*>(out)};
+        by_rank(x.rank, [&](auto r) {
+            constexpr int kR = decltype(r)::value;
+            outer_kernel<T, kRanksLast, kR>
+                <<<dim3((cols + 4 * kOuterCols - 1) / (4 * kOuterCols), (x.rank + kR * 16 - 1) / (kR * 16), x.adapters), 256, 0, st>>>(s);
+        });
+    }
+    template <typename Epi>
+    void product(const Operand& w, const Operand& h, int n, const Epi& e) const {
+        const int64_t k = plan.pack_w && plan.pack_h ? plan.kpad : x.dim;
+        if constexpr (sizeof(T) == 4) {
+            if (plan.tile_n == 32)
+                run<128, 32, 4, 1, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else if (plan.tile_n == 64)
+                run<128, 64, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else if (plan.tile_n == 96)
+                run<128, 96, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
+            else
+                run<128, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
+        } else if (plan.tile_n == head::kSmallTileN) {
+            run<head::kSmallTileM, head::kSmallTileN, 4, 1, true, true>(w, h, k, n, x.rows, 1, 4, e);
+        } else if (plan.tile_n == 128) {
+            run<256, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
+        } else {
+            run<256, 256, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
+        }
+    }
+    template <typename O>
+    void forward() const {
+        if (x.adapters) low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u, 1);
+        const Operand h = rows(x.hidden, hidden_ld(), x.rows, x.dim, plan.pack_h, plan.kpad, b.hpack);
+        const int64_t ld = x.rows > 1 ? x.out_stride : x.out_dim;
+        for (int v0 = 0; v0 < x.out_dim; v0 += plan.piece) {
+            const int n = std::min(plan.piece, x.out_dim - v0);
+            const OutEpi<T, O> e{adapters(x.b, x.out_dim, b.u), x.rows, n, v0, static_cast<O*>(x.out) + v0, ld};
+            product(weights(v0, n), h, n, e);
+        }
+    }
+    template <typename Epi>
+    void hidden(const Operand& w, const Operand& d, int n, const Epi& e) const {
+        constexpr int kTile = sizeof(T) == 4 ? 128 : 256;
+        if (sizeof(T) == 2 && x.rows <= 128)
+            run<kTile, 128, 2, 2, false, true>(w, d, n, x.dim, x.rows, plan.splits, 6, e);
+        else
+            run<kTile, kTile, 2, 2, false, true>(w, d, n, x.dim, x.rows, plan.splits, 6, e);
+    }
+    void backward() const {
+        const bool low_rank = x.adapters > 0;
+        if (low_rank && (x.dhidden || x.da)) low_sum<false>(x.dout, dout_ld(), x.out_dim, x.b, b.du, plan.low_splits);
+        if (low_rank) order_kernel<<<x.adapters, 1024, 0, st>>>(x.adapter, x.rows, x.adapters, b.order, b.order + x.adapters + 1);
+        if (x.dhidden) {
+            if (low_rank)
+                transpose_kernel<T><<<dim3((x.dim + 255) / 256, x.adapters), 256, 0, st>>>(static_cast<const T*>(x.a), x.rank, x.dim, b.order,
+                                                                                         static_cast<T*>(b.at));
+            T* const dh = static_cast<T*>(x.dhidden);
+            const int64_t dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
+            const int64_t hld = (x.dim + 3) / 4 * 4;
+            const bool direct = plan.splits == 1 && plan.piece >= x.out_dim;
+            for (int v0 = 0; v0 < x.out_dim; v0 += plan.piece) {
+                const int n = std::min(plan.piece, x.out_dim - v0);
+                const int64_t npad = head::round_up(n, head::kPadK);
+                const Operand w = weights(v0, n);
+                const Operand d = rows(static_cast<const T*>(x.dout) + v0, dout_ld(), x.rows, n, plan.pack_d, npad, b.dpack);
+                const Adapters<T> low = v0 == 0 ? adapters(b.at, x.dim, b.du) : Adapters<T>{};
+                if (direct)
+                    hidden(w, d, n, HiddenEpi<T, true>{low, x.rows, x.dim, dh, dh_ld, 0, false});
+                else
+                    hidden(w, d, n, HiddenEpi<T, false>{low, x.rows, x.dim, b.dhidden, hld, x.rows * hld, v0 > 0});
+            }
+            if (!direct)
+                for_rows(x.rows, [&](int64_t r, unsigned n) {
+                    hidden_sum_kernel<T><<<dim3((x.dim + 255) / 256, n), 256, 0, st>>>(b.dhidden + r * hld, hld, x.rows * hld, plan.splits,
+                                                                                     x.dim, dh + r * dh_ld, dh_ld);
+                });
+        }
+        if (x.da) outer<false>(x.hidden, hidden_ld(), x.dim, b.du, x.da);
+        if (x.db) {
+            low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u, 1);
+            outer<true>(x.dout, dout_ld(), x.out_dim, b.u, x.db);
+        }
+    }
+    void no_rows() const {  // the adapters' gradients are zeros
+        const int64_t n = static_cast<int64_t>(x.adapters) * x.rank;
+        if (x.da) zero(static_cast<T*>(x.da), n * x.dim, st);
+        if (x.db) zero(static_cast<T*>(x.db), n * x.out_dim, st);
+    }
+};
+
+template <typename T>
+void launch(const ge_project_args& x, const Plan& plan, const Buffers& b, bool backward, hipStream_t st) {
+    const Call<T> call{x, plan, b, st};
+    if (backward && x.rows == 0)
+        call.no_rows();
+    else if (backward)
+        call.backward();
+    else if (x.rows == 0)
+        return;
+    else if (x.out_dtype == GE_DTYPE_F32)
+        call.template forward<float>();
+    else
+        call.template forward<uint16_t>();
+}
+
+int hip_error(hipError_t e, const char* what) {
+    (void)hipGetLastError();  // reported here: the next launch's check shall not find it
+    char msg[256];
+    plan_fail(msg, sizeof(msg), 0, "%s: %s", what, hipGetErrorString(e));
+    return report(GE_ERR_DEVICE, msg);
+}
+
+// Switches the calling thread to `device` for the lifetime of the object.
+struct OnDevice {
+    int prev = -1;
+    bool ok = true;
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev != device) ok = hipSetDevice(device) == hipSuccess;
+    }
+    ~OnDevice() {
+        int cur = -1;
+        if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
+    }
+};
+
+}  // namespace
+}  // namespace projection
+}  // namespace ge
+
+struct ge_projection {
+    int device;
+    ge::projection::Capacity cap;
+    ge::projection::Buffers buf;
+};
+
+extern "C" {
+
+int ge_projection_create(int device, int max_rows, int max_dim, int max_out, int max_rank, int max_adapters, int dtype, int train,
+                         ge_projection** out) {
+    using namespace ge::projection;
+    char msg[256] = "";
+    if (!out) return ge::report(GE_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    if (const int rc = check_create(max_rows, max_dim, max_out, max_rank, max_adapters, dtype, msg, sizeof(msg))) return ge::report(rc, msg);
+    int n = 0;
+    hipDeviceProp_t prop;
+    if (hipGetDeviceCount(&n) != hipSuccess || device < 0 || device >= n || hipGetDeviceProperties(&prop, device) != hipSuccess ||
+        std::strncmp(prop.gcnArchName, "gfx950", 6) != 0) {
+        ge::plan_fail(msg, sizeof(msg), 0, "device %d is not a gfx950 device (%d devices)", device, n);
+        return ge::report(GE_ERR_NO_DEVICE, msg);
+    }
+    OnDevice guard(device);
+    if (!guard.ok) return ge::report(GE_ERR_DEVICE, "hipSetDevice failed");
+    ge_projection* h = new (std::nothrow) ge_projection{};
+    if (!h) return ge::report(GE_ERR_DEVICE, "out of host memory");
+    h->device = device;
+    Capacity& c = h->cap;
+    c = Capacity{max_rows, max_dim, max_out, max_rank, max_adapters, dtype, train != 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    size_workspace(c);
+    hipError_t e = hipSuccess;
+    auto alloc = [&](auto*& p, int64_t bytes) {
+        if (e == hipSuccess && bytes > 0) e = hipMalloc(reinterpret_cast<void**>(&p), static_cast<size_t>(bytes));
+    };
+    Buffers& b = h->buf;
+    alloc(b.hpack, c.hpack);
+    alloc(b.wpack, c.wpack);
+    alloc(b.u, c.u);
+    alloc(b.du, c.du);
+    alloc(b.du_parts, c.du_parts);
+    alloc(b.order, c.order);
+    alloc(b.at, c.at);
+    alloc(b.dpack, c.dpack);
+    alloc(b.dhidden, c.dhidden);
+    if (e != hipSuccess) {
+        ge_projection_destroy(h);
+        return hip_error(e, "ge_projection_create");
+    }
+    *out = h;
+    return GE_OK;
+}
+
+void ge_projection_destroy(ge_projection* h) {
+    if (!h) return;
+    ge::projection::OnDevice guard(h->device);
+    const ge::projection::Buffers& b = h->buf;
+    for (void* p : {b.hpack, b.wpack, b.u, b.du, static_cast<void*>(b.du_parts), static_cast<void*>(b.order), b.at, b.dpack,
+                    static_cast<void*>(b.dhidden)})
+        (void)hipFree(p);
+    delete h;
+}
+
+static int project_call(ge_projection* h, void* stream, const ge_project_args* args, bool backward) {
+    using namespace ge::projection;
+    char msg[256] = "";
+    if (!h || !args) return ge::report(GE_ERR_INVALID_ARG, "projection or args is NULL");
+    Plan plan{};
+    if (const int rc = check_project(h->cap, *args, backward, plan, msg, sizeof(msg))) return ge::report(rc, msg);
+    OnDevice guard(h->device);
+    if (!guard.ok) return ge::report(GE_ERR_DEVICE, "hipSetDevice failed");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (h->cap.dtype == GE_DTYPE_F32)
+        launch<float>(*args, plan, h->buf, backward, st);
+    else
+        launch<uint16_t>(*args, plan, h->buf, backward, st);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GE_OK : hip_error(e, "launch (projection)");
+}
+
+int ge_project(ge_projection* h, void* stream, const ge_project_args* args) { return project_call(h, stream, args, false); }
+int ge_project_backward(ge_projection* h, void* stream, const ge_project_args* args) { return project_call(h, stream, args, true); }
+
+}  // extern "C"

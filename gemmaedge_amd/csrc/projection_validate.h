@@ -1,0 +1,177 @@
+// Host-side checks and geometry of the projection's calls (include/gemmaedge_projection.h),
+// kept apart from the HIP launches so that they can be built and run without a
+// device. Nothing here reads device memory.
+#pragma once
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/gemmaedge_projection.h"
+#include "head_validate.h"
+
+namespace ge {
+namespace projection {
+
+using head::aligned_to;
+using head::dtype_ok;
+using head::elem_size;
+using head::kTile32;
+using head::kTileM;
+using head::kUnits;
+using head::round_up;
+using head::stride_ok;
+
+constexpr int kRowTile = 16;        // rows of a workgroup of the low-rank sums
+constexpr int kMaxLowSplits = 64;   // parts of such a sum over the outputs
+constexpr int kLowBlocks = 1024;    // workgroups that they are split up for
+
+// Ranks are padded to whole steps of the matrix instructions.
+inline int64_t rank_pad(int rank) { return round_up(rank, 32); }
+
+// What a handle was created for and the workspaces' sizes in bytes.
+struct Capacity {
+    int max_rows, max_dim, max_out, max_rank, max_adapters, dtype;
+    bool train;
+    int64_t hpack;    // hidden states in padded rows
+    int64_t wpack;    // a piece of the weights in padded rows
+    int64_t u, du;    // the rows' low-rank values
+    int64_t du_parts; // float32 parts of du
+    int64_t order;    // rows sorted by adapter, and where each one's begin
+    int64_t at;       // A transposed
+    int64_t dpack;    // a piece of dout in padded rows
+    int64_t dhidden;  // float32 parts of the hidden states' gradient
+};
+
+inline void size_workspace(Capacity& c) {
+    const int64_t rows = c.max_rows, es = elem_size(c.dtype), dim = round_up(c.max_dim, head::kPadK);
+    const int64_t out = round_up(c.max_out, kTileM);
+    c.hpack = es * rows * dim;
+    c.wpack = es * dim * std::min(out, std::max<int64_t>(kTileM, ((64LL << 20) / (2 * dim)) / kTileM * kTileM));
+    const int64_t upad = rank_pad(c.max_rank);
+    c.u = c.max_adapters ? 4 * rows * upad : 0;
+    c.du = c.du_parts = c.order = c.at = c.dpack = c.dhidden = 0;
+    if (!c.train) return;
+    c.dpack = es * rows * std::min(out, std::max<int64_t>(kTileM, (256LL << 20) / (es * rows) / kTileM * kTileM));
+    const int64_t tiles = (rows + 255) / 256 * ((dim + 255) / 256);
+    c.dhidden = 4 * std::min<int64_t>(256 * 256 * std::max<int64_t>(tiles, 1024),
+                                      std::min<int64_t>(head::kMaxSplits, (out + 63) / 64) * rows * round_up(c.max_dim, 4));
+    if (!c.max_adapters) return;
+    c.du = c.u;
+    const int64_t row_tiles = (rows + kRowTile - 1) / kRowTile;
+    c.du_parts = 4 * upad * std::min(kMaxLowSplits * rows, kRowTile * std::max<int64_t>(kLowBlocks, row_tiles));
+    c.order = 4 * (rows + c.max_adapters + 1);
+    c.at = es * c.max_adapters * static_cast<int64_t>(c.max_dim) * c.max_rank;
+}
+
+inline int check_create(int max_rows, int max_dim, int max_out, int max_rank, int max_adapters, int dtype, char* msg, size_t n) {
+    if (max_rows < 1 || max_dim < 1 || max_out < 1 || max_rank < 0 || max_adapters < 0 || (max_rank == 0) != (max_adapters == 0))
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "max_rows=%d max_dim=%d max_out=%d max_rank=%d max_adapters=%d", max_rows, max_dim,
+                         max_out, max_rank, max_adapters);
+    if (!dtype_ok(dtype)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dtype %d", dtype);
+    if (max_dim > GE_PROJECT_MAX_DIM || max_out > (1 << 24) || max_rows > (1 << 22) || max_rank > GE_PROJECT_MAX_RANK ||
+        max_adapters > GE_PROJECT_MAX_ADAPTERS)
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "max_rows %d / max_dim %d / max_out %d / max_rank %d / max_adapters %d above %d / %d / %d / %d / %d",
+                         max_rows, max_dim, max_out, max_rank, max_adapters, 1 << 22, GE_PROJECT_MAX_DIM, 1 << 24, GE_PROJECT_MAX_RANK,
+                         GE_PROJECT_MAX_ADAPTERS);
+    return GE_OK;
+}
+
+// How a call runs.
+struct Plan {
+    bool pack_h, pack_w, pack_d;  // operands copied into padded rows first
+    int64_t kpad;                 // packed rows' length
+    int tile_m, tile_n;           // of the forward product
+    int piece;                    // outputs of a launch
+    int splits;                   // parts of the outputs' sum in dhidden
+    int low_splits;               // and in du
+};
+
+// Parts of a low-rank sum over k elements: enough workgroups, of 128 elements at least.
+inline int low_splits(int rows, int k) {
+    const int tiles = (rows + kRowTile - 1) / kRowTile;
+    return std::max(1, std::min(std::min(kLowBlocks / std::max(tiles, 1), kMaxLowSplits), k / 128));
+}
+
+inline int check_project(const Capacity& c, const ge_project_args& x, bool backward, Plan& plan, char* msg, size_t n) {
+    if (x.rows < 0 || x.dim < 1 || x.out_dim < 1 || x.adapters < 0)
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "rows %d, dim %d, out_dim %d, adapters %d", x.rows, x.dim, x.out_dim, x.adapters);
+    if (x.adapters > 0 && x.rank < 1) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "rank %d", x.rank);
+    if (x.rows > c.max_rows || x.dim > c.max_dim || x.out_dim > c.max_out || x.adapters > c.max_adapters ||
+        (x.adapters > 0 && x.rank > c.max_rank))
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "rows %d / dim %d / out_dim %d / rank %d / adapters %d above capacity %d / %d / %d / %d / %d",
+                         x.rows, x.dim, x.out_dim, x.rank, x.adapters, c.max_rows, c.max_dim, c.max_out, c.max_rank, c.max_adapters);
+    if (backward && !c.train) return plan_fail(msg, n, GE_ERR_CAPACITY, "the handle was created without train");
+    if (!backward && !dtype_ok(x.out_dtype)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "out_dtype %d", x.out_dtype);
+    const size_t es = elem_size(c.dtype);
+    if (x.rows > 0) {
+        if (!x.hidden || !x.weight || (!backward && !x.out) || (backward && !x.dout))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "hidden, weight, out or dout is NULL");
+        if (!stride_ok(x.hidden_stride, x.rows, x.dim) || !stride_ok(x.weight_stride, x.out_dim, x.dim) ||
+            (!backward && !stride_ok(x.out_stride, x.rows, x.out_dim)) || (backward && !stride_ok(x.dout_stride, x.rows, x.out_dim)) ||
+            (backward && x.dhidden && !stride_ok(x.dhidden_stride, x.rows, x.dim)))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "rows overlap: a stride below dim %d or out_dim %d", x.dim, x.out_dim);
+        if (x.adapters > 0 && (!x.a || !x.b || !x.scale || !x.adapter))
+            return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a, b, scale or adapter is NULL");
+    }
+    if (backward && x.adapters == 0 && (x.da || x.db)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "da or db without adapters");
+    if (!aligned_to(x.hidden, es) || !aligned_to(x.weight, es) || !aligned_to(x.a, es) || !aligned_to(x.b, es) || !aligned_to(x.scale, 4) ||
+        !aligned_to(x.adapter, 4) || (!backward && !aligned_to(x.out, elem_size(x.out_dtype))) || !aligned_to(x.dout, es) ||
+        !aligned_to(x.dhidden, es) || !aligned_to(x.da, es) || !aligned_to(x.db, es))
+        return plan_fail(msg, n, GE_ERR_INVALID_ARG, "a tensor is not aligned to its elements");
+
+    // As in the vocabulary loss: bf16 tiles are fetched 16 bytes a lane into LDS, other
+    // rows are packed first; offsets in a tile have 31 bits.
+    auto direct = [&](const void* p, int64_t stride, int rows, int dim) {
+        if (rows > 1 && stride > head::kMaxStride) return false;
+        return c.dtype == GE_DTYPE_F32 || (aligned_to(p, 16) && (rows <= 1 || stride % 8 == 0) && dim % 8 == 0);
+    };
+    plan.pack_h = !direct(x.hidden, x.hidden_stride, x.rows, x.dim);
+    plan.pack_w = !direct(x.weight, x.weight_stride, x.out_dim, x.dim);
+    plan.pack_d = backward && !direct(x.dout, x.dout_stride, x.rows, x.out_dim);
+    plan.kpad = round_up(x.dim, head::kPadK);
+    if (c.dtype == GE_DTYPE_F32) {
+        plan.tile_m = kTile32;
+        plan.tile_n = 32;
+        int64_t best = x.rows <= 32 ? 0 : INT64_MAX;
+        for (const int tile : {128, 96, 64}) {
+            const int64_t cost = round_up(x.rows, tile) / tile * (tile + 20);
+            if (cost < best) {
+                best = cost;
+                plan.tile_n = tile;
+            }
+        }
+    } else {
+        const bool small = x.rows <= head::kSmallRows;
+        plan.tile_m = small ? head::kSmallTileM : kTileM;
+        plan.tile_n = small ? head::kSmallTileN : x.rows <= 128 ? 128 : 256;
+    }
+    const int64_t out_pad = round_up(x.out_dim, kTileM);
+    const int64_t row_tiles = (std::max(x.rows, 1) + plan.tile_n - 1) / plan.tile_n;
+    int64_t piece = std::min(out_pad, head::kMostTiles / row_tiles * plan.tile_m / kTileM * kTileM);
+    if (plan.pack_w) piece = std::min(piece, c.wpack / (static_cast<int64_t>(es) * plan.kpad) / kTileM * kTileM);
+    if (plan.pack_d) piece = std::min(piece, c.dpack / (static_cast<int64_t>(es) * x.rows) / kTileM * kTileM);
+    plan.piece = static_cast<int>(piece);
+    plan.splits = plan.low_splits = 1;
+    if (backward) {
+        // Parts of the sum over a piece, as in the loss's: rounds of tiles times the steps of one.
+        const int64_t tile = c.dtype == GE_DTYPE_F32 ? kTile32 : 256, slots = c.dtype == GE_DTYPE_F32 ? 2 * kUnits : kUnits;
+        const int64_t tiles = (x.rows + tile - 1) / tile * ((x.dim + tile - 1) / tile);
+        const int64_t steps = (std::min<int64_t>(piece, x.out_dim) + 63) / 64;
+        const int64_t most_bytes = 4 * std::max<int64_t>(x.rows, 1) * round_up(x.dim, 4);
+        const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(head::kMaxSplits, steps), c.dhidden / most_bytes));
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= fit; ++s) {
+            const int64_t cost = (tiles * s + slots - 1) / slots * ((steps + s - 1) / s + 12);
+            if (cost < best) {
+                best = cost;
+                plan.splits = static_cast<int>(s);
+            }
+        }
+        plan.low_splits = low_splits(x.rows, x.out_dim);
+    }
+    return GE_OK;
+}
+
+}  // namespace projection
+}  // namespace ge
