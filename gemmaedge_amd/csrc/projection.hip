@@ -45,7 +45,7 @@ struct Buffers {
     void* wpack;
     void* u;
     void* du;
-    float* du_parts;
+    float* parts;
     int32_t* order;
     void* at;
     void* dpack;
@@ -350,15 +350,19 @@ struct HiddenEpi {
     }
 };
 
+// The parts of dhidden in order, rounded once: 4 channels a thread (ld is a multiple of 4 above dim).
 template <typename T>
-__global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int64_t ld, int64_t split, int splits, int dim, T* out,
+__global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int64_t ld, int64_t split, int splits, int64_t rows, int dim, T* out,
                                                          int64_t out_ld) {
-    const int d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= dim) return;
-    const int64_t r = blockIdx.y;
-    float s = 0.f;
-    for (int i = 0; i < splits; ++i) s += parts[i * split + r * ld + d];
-    out[r * out_ld + d] = from_f32<T>(s);
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    const int64_t r = at / ld;
+    const int d = static_cast<int>(at % ld);
+    if (r >= rows || d >= dim) return;
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) sum += *reinterpret_cast<const f32x4*>(parts + i * split + at);
+    const float x[4] = {sum[0], sum[1], sum[2], sum[3]};
+    store_out(out + r * out_ld + d, x, dim - d);
 }
 
 // ---- sums of a row's channels with each rank -------------------------------------
@@ -366,8 +370,8 @@ __global__ __launch_bounds__(256) void hidden_sum_kernel(const float* parts, int
 // y[n][r] = scale[k] * sum over c of x[n][c] * table[k](r, c), k the row's adapter.
 // kAlong: the table is [adapters][rank][cols] (u from A); else [adapters][cols][rank]
 // (du from B), and its tiles are transposed on their way from LDS, like those of
-// the large product. A workgroup takes 16 rows and one of the adapters they have (at most 16:
-// a grid's y), its four waves every fourth step of a part of the sum.
+// the large product. A workgroup takes a tile of rows and one of the adapters they have (at most as
+// many as rows: a grid's y), and a part of the sum.
 template <typename T>
 struct SumArgs {
     const T* x;
@@ -382,121 +386,186 @@ struct SumArgs {
     int splits, steps_per_split;
 };
 
-constexpr int kSumStep = 32;  // channels of a wave's step
-
-// The slot-th of the adapters that 16 rows have; INT_MAX: they have fewer.
+// The slot-th of the adapters that a wave's lanes have; INT_MAX: they have fewer.
 __device__ __forceinline__ int slot_adapter(int id, int slot) {
-    int k = -1;
-    for (int s = 0; s <= slot && k != INT_MAX; ++s) k = wave_min(id > k ? id : INT_MAX);
-    return k;
+    uint64_t left = __ballot(id >= 0);
+    for (; left; --slot) {
+        const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        if (slot == 0) return k;
+        left &= ~__ballot(id == k);
+    }
+    return INT_MAX;
 }
 
+template <typename T>
+__device__ __forceinline__ int row_adapter(const SumArgs<T>& s, int n) {
+    const int id = n < s.rows ? s.ids[n] : -1;
+    return id < s.adapters ? id : -1;
+}
+
+// A row's sum with rank r: into its part, or as the value itself. `who`: the row's adapter.
+template <typename T>
+__device__ __forceinline__ void low_result(const SumArgs<T>& s, int split, int64_t n, int r, float x, int who) {
+    if (who < 0 || r >= s.rank) x = 0.f;
+    if (s.parts)
+        s.parts[(static_cast<int64_t>(split) * s.rows + n) * s.y.pad + r] = x;
+    else
+        low_store(s.y, n, r, who >= 0 ? x * s.scale[who] : 0.f);
+}
+
+// The first `left` of 8 elements at p (any address), zeros behind them.
+__device__ __forceinline__ u32x4 load_row8(const uint16_t* p, int left) {
+    u32x4 raw{0, 0, 0, 0};
+    if (left >= 8) {
+        __builtin_memcpy(&raw, p, 16);
+    } else if (left > 0) {
+        struct {
+            uint16_t v[8];
+        } q{};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) q.v[e] = p[e];
+        raw = __builtin_bit_cast(u32x4, q);
+    }
+    return raw;
+}
+
+// A tile of bf16 columns in LDS, rows `ld` elements apart: 16 columns from `col` on of 32 rows,
+// transposed into a fragment.
+__device__ __forceinline__ bf16x8 frag_across(uint16_t* tile, int ld, int col, int lane) {
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    const int i = lane & 15, g = lane >> 4;
+    uint16_t* const p = tile + (8 * g + (i >> 2)) * ld + col + (i & 3) * 4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ld));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Few rows, or float32: a workgroup has 16 rows, and its waves take every kSumWaves-th step of 32 channels,
+// kBatch of them at a time, whose loads are in flight together. Bound by their latency: 64
+// rows of 2,816 channels with 22 adapters of rank 16: 5 us (18 us a step at a time with four waves).
+constexpr int kSumStep = 32;
+constexpr int kSumWaves = 8;
+
 template <typename T, bool kAlong, int kR>
-__global__ __launch_bounds__(256) void low_sum_kernel(SumArgs<T> s) {
-    constexpr int kRanks = kR * 16;
-    __shared__ __align__(16) float red[4][kRanks][17];
+__global__ __launch_bounds__(64 * kSumWaves) void low_sum_kernel(SumArgs<T> s) {
+    constexpr int kRanks = kR * 16, kBatch = kR == 4 ? 2 : 4;
+    __shared__ __align__(16) float red[kSumWaves][kRanks][17];
     constexpr int kRow = kRanks + 8;  // bf16 elements of a transposed tile's row in LDS
-    __shared__ __align__(16) uint16_t tile[!kAlong && sizeof(T) == 2 ? 4 * kSumStep * kRow : 8];
+    constexpr bool kTiled = !kAlong && sizeof(T) == 2;
+    __shared__ __align__(16) uint16_t tiles[kTiled ? kSumWaves * kBatch * kSumStep * kRow : 8];
+    __shared__ int owner[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * kRowTile;
-    const int n = n0 + i;
-    int id = n < s.rows ? s.ids[n] : -1;
-    if (id < 0 || id >= s.adapters) id = -1;
+    const int id = row_adapter(s, n0 + i);
     const int k = slot_adapter(id, blockIdx.y);
+    // Rows without an adapter have zeros; the first slot writes them.
+    if (k == INT_MAX && blockIdx.y != 0) return;
     const int split = blockIdx.z % s.splits, r0 = blockIdx.z / s.splits * kRanks;
-    const T* const xr = s.x + min(n, s.rows - 1) * s.ld;
     f32x4 acc[kR];
 #pragma unroll
     for (int t = 0; t < kR; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (k == INT_MAX) {
-        // Rows without an adapter have zeros; the first slot writes them.
-        if (blockIdx.y != 0) return;
-    } else {
-        const int64_t size = static_cast<int64_t>(s.rank) * s.cols;
-        const T* const table = s.table + k * size;
+    if (k != INT_MAX && r0 < s.rank) {
+        const T* const xr = s.x + min(n0 + i, s.rows - 1) * s.ld;
+        const T* const table = s.table + k * (static_cast<int64_t>(s.rank) * s.cols);
         const int first = split * s.steps_per_split;
         const int last = min((s.cols + kSumStep - 1) / kSumStep, first + s.steps_per_split);
-        uint16_t* const my = tile + wave * kSumStep * kRow;
-        for (int step = first + wave; step < last; step += 4) {
-            const int c0 = step * kSumStep;
+        for (int step = first + wave; step < last; step += kSumWaves * kBatch) {
             if constexpr (sizeof(T) == 2) {
-                const int c = c0 + 8 * g, left = s.cols - c;
-                u32x4 raw{0, 0, 0, 0};
-                if (left >= 8) {
-                    __builtin_memcpy(&raw, xr + c, 16);
-                } else if (left > 0) {
-                    struct {
-                        uint16_t v[8];
-                    } q{};
+                uint16_t* const my = tiles + (kTiled ? wave * kBatch * kSumStep * kRow : 0);
+                u32x4 fx[kBatch], fw[kBatch][kR];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < left) q.v[e] = xr[c + e];
-                    raw = __builtin_bit_cast(u32x4, q);
-                }
-                const bf16x8 fx = __builtin_bit_cast(bf16x8, raw);
-                if constexpr (kAlong) {
+                for (int b = 0; b < kBatch; ++b) {
+                    const int at = step + b * kSumWaves, c0 = at * kSumStep, c = c0 + 8 * g;
+                    const int left = at < last ? s.cols - c : 0;
+                    fx[b] = load_row8(xr + c, left);
+                    if constexpr (kAlong) {
 #pragma unroll
-                    for (int t = 0; t < kR; ++t) {
-                        const int r = r0 + t * 16 + i;
-                        u32x4 w{0, 0, 0, 0};
-                        if (r < s.rank) {
-                            const T* const p = table + static_cast<int64_t>(r) * s.cols + c;
-                            if (left >= 8) {
-                                __builtin_memcpy(&w, p, 16);
-                            } else if (left > 0) {
-                                struct {
-                                    uint16_t v[8];
-                                } q{};
+                        for (int t = 0; t < kR; ++t)  // ranks past the last: outputs that nobody reads
+                            fw[b][t] = load_row8(table + static_cast<int64_t>(min(r0 + t * 16 + i, s.rank - 1)) * s.cols + c, left);
+                    } else {
+                        // 32 channels of the ranks, 8 a lane; columns past the rank belong to the next
+                        // channel and to outputs that nobody reads.
+                        const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank,
+                                                 at < last ? (s.cols - c0) * static_cast<int64_t>(s.rank) * 2 : 0);
+                        constexpr int kPerRow = kRanks / 8;
 #pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if (e < left) q.v[e] = p[e];
-                                w = __builtin_bit_cast(u32x4, q);
-                            }
+                        for (int q = 0; q < kR; ++q) {
+                            const int unit = q * 64 + lane, row = unit / kPerRow, col = unit % kPerRow * 8;
+                            fw[b][q] = load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
                         }
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), fx, acc[t], 0, 0, 0);
                     }
-                } else {
-                    // 32 channels of the ranks, 8 a lane; columns past the rank belong to the next
-                    // channel and to outputs that nobody reads.
-                    const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank, (s.cols - c0) * static_cast<int64_t>(s.rank) * 2);
+                }
+                if constexpr (!kAlong) {
                     constexpr int kPerRow = kRanks / 8;
 #pragma unroll
-                    for (int q = 0; q < kR; ++q) {
-                        const int at = q * 64 + lane, row = at / kPerRow, col = at % kPerRow * 8;
-                        *reinterpret_cast<u32x4*>(my + row * kRow + col) =
-                            load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                    typedef __attribute__((address_space(3))) s16x4* lds4;
+                    for (int b = 0; b < kBatch; ++b)
 #pragma unroll
-                    for (int t = 0; t < kR; ++t) {
-                        uint16_t* const p = my + (8 * g + (i >> 2)) * kRow + t * 16 + (i & 3) * 4;
-                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * kRow));
-                        const bf16x8 fw = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc[t], 0, 0, 0);
-                    }
+                        for (int q = 0; q < kR; ++q) {
+                            const int unit = q * 64 + lane, row = unit / kPerRow, col = unit % kPerRow * 8;
+                            *reinterpret_cast<u32x4*>(my + (b * kSumStep + row) * kRow + col) = fw[b][q];
+                        }
                     __builtin_amdgcn_wave_barrier();
                 }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                    for (int t = 0; t < kR; ++t) {
+                        bf16x8 w;
+                        if constexpr (kAlong)
+                            w = __builtin_bit_cast(bf16x8, fw[b][t]);
+                        else
+                            w = frag_across(my + b * kSumStep * kRow, kRow, t * 16, lane);
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(bf16x8, fx[b]), acc[t], 0, 0, 0);
+                    }
+                __builtin_amdgcn_wave_barrier();
             } else {
-                const auto rs_x = resource(xr, s.cols * static_cast<int64_t>(sizeof(T)));
+                f32x4 fx[kBatch][2], fw[kBatch][2][kR];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = c0 + h * 16 + 4 * g;
-                    const f32x4 fx = __builtin_bit_cast(f32x4, load16(rs_x, static_cast<uint32_t>(c) * 4));
+                for (int b = 0; b < kBatch; ++b)
 #pragma unroll
-                    for (int t = 0; t < kR; ++t) {
-                        const int r = r0 + t * 16 + i;
-                        f32x4 fw{0.f, 0.f, 0.f, 0.f};
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = step + b * kSumWaves, c = at * kSumStep + h * 16 + 4 * g;
+                        const bool there = at < last;
+                        const f32x4 none{0.f, 0.f, 0.f, 0.f};
+                        fx[b][h] = none;
+                        if (there && c + 4 <= s.cols) {
+                            __builtin_memcpy(&fx[b][h], xr + c, 16);
+                        } else if (there) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (r < s.rank && c + e < s.cols)
-                                fw[e] = kAlong ? table[static_cast<int64_t>(r) * s.cols + c + e] : table[static_cast<int64_t>(c + e) * s.rank + r];
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < s.cols) fx[b][h][e] = xr[c + e];
+                        }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[e], fx[e], acc[t], 0, 0, 0);
+                        for (int t = 0; t < kR; ++t) {
+                            const int r = min(r0 + t * 16 + i, s.rank - 1);
+                            fw[b][h][t] = none;
+                            if constexpr (kAlong) {
+                                const T* const p = table + static_cast<int64_t>(r) * s.cols + c;
+                                if (there && c + 4 <= s.cols) {
+                                    __builtin_memcpy(&fw[b][h][t], p, 16);
+                                } else if (there) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (c + e < s.cols) fw[b][h][t][e] = p[e];
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (there && c + e < s.cols) fw[b][h][t][e] = table[static_cast<int64_t>(c + e) * s.rank + r];
+                            }
+                        }
                     }
-                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int t = 0; t < kR; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[b][h][t][e], fx[b][h][e], acc[t], 0, 0, 0);
             }
         }
     }
@@ -504,23 +573,105 @@ __global__ __launch_bounds__(256) void low_sum_kernel(SumArgs<T> s) {
     for (int t = 0; t < kR; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) red[wave][t * 16 + 4 * g + e][i] = acc[t][e];
-    // The row's adapter is this workgroup's, or the row has none and this is the first.
-    __shared__ int owner[16];
     if (threadIdx.x < 16) owner[threadIdx.x] = id;
     __syncthreads();
-    for (int at = threadIdx.x; at < kRanks * kRowTile; at += 256) {
+    for (int at = threadIdx.x; at < kRanks * kRowTile; at += 64 * kSumWaves) {
         const int c = at / kRanks, r = at % kRanks;
-        const int who = owner[c];
+        const int who = owner[c];  // this workgroup's adapter, or none and this is the first
         if (n0 + c >= s.rows || r0 + r >= s.y.pad || !(who == k || (who < 0 && blockIdx.y == 0))) continue;
         float x = 0.f;
-        if (who >= 0 && r0 + r < s.rank) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) x += red[w][r][c];
+        for (int w = 0; w < kSumWaves; ++w) x += red[w][r][c];
+        low_result(s, split, n0 + c, r0 + r, x, who);
+    }
+}
+
+// Many bf16 rows: a workgroup has 64, 16 a wave, which share the table's tiles of 64 channels in two
+// LDS buffers in turn; the next tile and the next rows' channels are on their way meanwhile.
+constexpr int kWideRows = 64, kWideStep = 64;
+
+template <bool kAlong, int kR>
+__global__ __launch_bounds__(256) void low_wide_kernel(SumArgs<uint16_t> s) {
+    constexpr int kRanks = kR * 16;
+    constexpr int kRow = (kAlong ? kWideStep : kRanks) + 8, kRowsOf = kAlong ? kRanks : kWideStep;
+    constexpr int kUnits = kRanks * kWideStep / 8, kPer = (kUnits + 255) / 256;
+    __shared__ __align__(16) uint16_t tiles[2][kRowsOf * kRow];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * kWideRows, n = n0 + wave * 16 + i;
+    const int all_ids = row_adapter(s, n0 + lane);
+    const int k = slot_adapter(all_ids, blockIdx.y);
+    if (k == INT_MAX && blockIdx.y != 0) return;
+    const int split = blockIdx.z % s.splits, r0 = blockIdx.z / s.splits * kRanks;
+    const int who = __shfl(all_ids, wave * 16 + i);
+    f32x4 acc[kR];
+#pragma unroll
+    for (int t = 0; t < kR; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (k != INT_MAX && r0 < s.rank) {
+        const uint16_t* const xr = s.x + min(n, s.rows - 1) * s.ld;
+        const uint16_t* const table = s.table + k * (static_cast<int64_t>(s.rank) * s.cols);
+        const int first = split * s.steps_per_split;
+        const int last = min((s.cols + kWideStep - 1) / kWideStep, first + s.steps_per_split);
+        u32x4 fx[2], next[2], w[kPer];
+        auto load = [&](int step) {
+            const int c0 = step * kWideStep;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) next[h] = load_row8(xr + c0 + h * 32 + 8 * g, s.cols - (c0 + h * 32 + 8 * g));
+            const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank, (s.cols - c0) * static_cast<int64_t>(s.rank) * 2);
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) {
+                const int unit = q * 256 + threadIdx.x;
+                if (unit >= kUnits) break;
+                if constexpr (kAlong) {
+                    const int row = unit / (kWideStep / 8), c = c0 + unit % (kWideStep / 8) * 8;
+                    w[q] = load_row8(table + static_cast<int64_t>(min(r0 + row, s.rank - 1)) * s.cols + c, s.cols - c);
+                } else {
+                    const int row = unit / (kRanks / 8), col = unit % (kRanks / 8) * 8;
+                    w[q] = load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
+                }
+            }
+        };
+        if (first < last) load(first);
+        for (int step = first; step < last; ++step) {
+            uint16_t* const tile = tiles[(step - first) & 1];
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) {
+                const int unit = q * 256 + threadIdx.x;
+                if (unit >= kUnits) break;
+                constexpr int kPerRow = (kAlong ? kWideStep : kRanks) / 8;
+                *reinterpret_cast<u32x4*>(tile + unit / kPerRow * kRow + unit % kPerRow * 8) = w[q];
+            }
+            fx[0] = next[0];
+            fx[1] = next[1];
+            __syncthreads();  // a buffer is written again two steps on, behind the next barrier
+            if (step + 1 < last) load(step + 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < kR; ++t) {
+                    bf16x8 f;
+                    if constexpr (kAlong)
+                        f = *reinterpret_cast<const bf16x8*>(tile + (t * 16 + i) * kRow + h * 32 + 8 * g);
+                    else
+                        f = frag_across(tile + h * 32 * kRow, kRow, t * 16, lane);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, fx[h]), acc[t], 0, 0, 0);
+                }
         }
-        if (s.parts)
-            s.parts[(static_cast<int64_t>(split) * s.rows + n0 + c) * s.y.pad + r0 + r] = x;
-        else
-            low_store(s.y, n0 + c, r0 + r, who >= 0 ? x * s.scale[who] : 0.f);
+    }
+    if (n >= s.rows || !(who == k || (who < 0 && blockIdx.y == 0))) return;
+#pragma unroll
+    for (int t = 0; t < kR; ++t) {
+        const int r = r0 + t * 16 + 4 * g;
+        if (r >= s.y.pad) continue;
+        if (s.parts) {  // 4 neighbours; the padding is a multiple of 32
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = who >= 0 && r + e < s.rank ? acc[t][e] : 0.f;
+            *reinterpret_cast<f32x4*>(s.parts + (static_cast<int64_t>(split) * s.rows + n) * s.y.pad + r) = x;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) low_result(s, split, n, r + e, acc[t][e], who);
+        }
     }
 }
 
@@ -531,6 +682,7 @@ __global__ __launch_bounds__(256) void low_join_kernel(SumArgs<T> s) {
     if (at >= all) return;
     const int64_t n = at / s.y.pad;
     float x = 0.f;
+#pragma unroll 8
     for (int i = 0; i < s.splits; ++i) x += s.parts[i * all + at];
     const int id = s.ids[n];
     low_store(s.y, n, static_cast<int>(at % s.y.pad), id >= 0 && id < s.adapters ? x * s.scale[id] : 0.f);
@@ -588,127 +740,186 @@ struct OuterArgs {
     const int32_t* begin;
     const int32_t* order;
     T* out;
+    float* parts;  // [splits], each of the output's size, or NULL
+    int splits;
+    int64_t size;  // of all adapters
 };
 
 constexpr int kOuterCols = 64;  // of a wave
+constexpr int kOuterRows = 64;  // of a step (bf16)
 
 template <typename T, bool kRanksLast, int kR>
 __global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
     constexpr int kRanks = kR * 16, kC = kOuterCols / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int k = blockIdx.z, r0 = blockIdx.y * kRanks;
+    const int k = blockIdx.z / s.splits, split = blockIdx.z % s.splits, r0 = blockIdx.y * kRanks;
     const int c0 = (blockIdx.x * 4 + wave) * kOuterCols;
-    const int from = s.begin[k], count = s.begin[k + 1] - from;
-    const int32_t* const rows = s.order + from;
+    const int begin = s.begin[k], mine = s.begin[k + 1] - begin;
+    // this part's rows, whole steps of them
+    const int steps = (mine + kOuterRows - 1) / kOuterRows, each = (steps + s.splits - 1) / s.splits * kOuterRows;
+    const int from = min(mine, split * each), count = min(mine, from + each) - from;
+    const int32_t* const rows = s.order + begin + from;
     f32x4 acc[kC][kR];
 #pragma unroll
     for (int c = 0; c < kC; ++c)
 #pragma unroll
         for (int r = 0; r < kR; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     if constexpr (sizeof(T) == 2) {
+        // A wave's columns are its own, the ranks the workgroup's, in two buffers in turn. The next
+        // step's loads are in flight while this one is multiplied, and the rows' numbers a step ahead of them.
         constexpr int kXRow = kOuterCols + 8, kYRow = kRanks + 8;
-        __shared__ __align__(16) uint16_t xs[4][32 * kXRow];
-        __shared__ __align__(16) uint16_t ys[2][32 * kYRow];
-        typedef __attribute__((address_space(3))) s16x4* lds4;
-        auto frag = [&](uint16_t* base, int ld, int col) {
-            uint16_t* const p = base + (8 * g + (i >> 2)) * ld + col + (i & 3) * 4;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ld));
-            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        constexpr int kX = kOuterRows / 8, kYUnits = 2 * kOuterRows * kRanks / 8, kY = (kYUnits + 255) / 256;
+        __shared__ __align__(16) uint16_t xs[4][kOuterRows * kXRow];
+        __shared__ __align__(16) uint16_t ys[2][2 * kOuterRows * kYRow];
+        u32x4 x[kX], y[kY];
+        int xn[kX], yn[kY];
+        const int c = c0 + (lane & 7) * 8;
+        auto y_row = [&](int q) { return (q * 256 + static_cast<int>(threadIdx.x)) / (kRanks / 8) % kOuterRows; };
+        auto number = [&](int n0) {
+#pragma unroll
+            for (int q = 0; q < kX; ++q) {
+                const int at = n0 + q * 8 + (lane >> 3);
+                xn[q] = at < count ? rows[at] : -1;
+            }
+#pragma unroll
+            for (int q = 0; q < kY; ++q) {
+                const int at = n0 + y_row(q);
+                yn[q] = at < count ? rows[at] : -1;
+            }
         };
-        for (int n0 = 0; n0 < count; n0 += 32) {
+        auto load = [&]() {
+#pragma unroll
+            for (int q = 0; q < kX; ++q) x[q] = load_row8(s.x + xn[q] * s.ld + c, xn[q] >= 0 ? s.cols - c : 0);
+#pragma unroll
+            for (int q = 0; q < kY; ++q) {
+                const int at = q * 256 + threadIdx.x, plane = at / (kOuterRows * kRanks / 8), col = r0 + at % (kRanks / 8) * 8;
+                y[q] = u32x4{0, 0, 0, 0};
+                if (yn[q] >= 0 && at < kYUnits && col < s.y.pad)
+                    y[q] = *reinterpret_cast<const u32x4*>(s.y.p + plane * s.y.plane + static_cast<int64_t>(yn[q]) * s.y.pad + col);
+            }
+        };
+        number(0);
+        load();
+        number(kOuterRows);
+        for (int n0 = 0, turn = 0; n0 < count; n0 += kOuterRows, turn ^= 1) {
+            uint16_t* const xt = xs[wave];
+            uint16_t* const yt = ys[turn];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < kX; ++q) *reinterpret_cast<u32x4*>(xt + (q * 8 + (lane >> 3)) * kXRow + (lane & 7) * 8) = x[q];
+#pragma unroll
+            for (int q = 0; q < kY; ++q) {
+                const int at = q * 256 + threadIdx.x, plane = at / (kOuterRows * kRanks / 8), col = at % (kRanks / 8) * 8;
+                if (at < kYUnits) *reinterpret_cast<u32x4*>(yt + (plane * kOuterRows + y_row(q)) * kYRow + col) = y[q];
+            }
             __syncthreads();
+            if (n0 + kOuterRows < count) {
+                load();
+                number(n0 + 2 * kOuterRows);
+            }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int at = q * 8 + (lane >> 3), c = c0 + (lane & 7) * 8;
-                struct {
-                    uint16_t v[8];
-                } v{};
-                if (n0 + at < count && c < s.cols) {
-                    const T* const p = s.x + rows[n0 + at] * s.ld + c;
-                    if (c + 8 <= s.cols) {
-                        __builtin_memcpy(&v, p, 16);
-                    } else {
+            for (int h = 0; h < kOuterRows / 32; ++h) {
+                bf16x8 fy[2][kR];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (c + e < s.cols) v.v[e] = p[e];
-                    }
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) fy[p][r] = frag_across(yt + (p * kOuterRows + h * 32) * kYRow, kYRow, r * 16, lane);
+#pragma unroll
+                for (int t = 0; t < kC; ++t) {
+                    const bf16x8 fx = frag_across(xt + h * 32 * kXRow, kXRow, t * 16, lane);
+#pragma unroll
+                    for (int p = 1; p >= 0; --p)
+#pragma unroll
+                        for (int r = 0; r < kR; ++r)
+                            acc[t][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fy[p][r], fx, acc[t][r], 0, 0, 0)
+                                                   : __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fy[p][r], acc[t][r], 0, 0, 0);
                 }
-                *reinterpret_cast<u32x4*>(&xs[wave][at * kXRow + (lane & 7) * 8]) = __builtin_bit_cast(u32x4, v);
-            }
-            for (int at = threadIdx.x; at < 2 * 32 * kRanks / 8; at += 256) {
-                const int plane = at / (32 * kRanks / 8), u = at % (32 * kRanks / 8), row = u / (kRanks / 8), col = u % (kRanks / 8) * 8;
-                u32x4 v{0, 0, 0, 0};
-                if (n0 + row < count && r0 + col < s.y.pad)
-                    v = *reinterpret_cast<const u32x4*>(s.y.p + plane * s.y.plane + static_cast<int64_t>(rows[n0 + row]) * s.y.pad + r0 + col);
-                *reinterpret_cast<u32x4*>(&ys[plane][row * kYRow + col]) = v;
-            }
-            __syncthreads();
-            bf16x8 fy[2][kR];
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int r = 0; r < kR; ++r) fy[p][r] = frag(ys[p], kYRow, r * 16);
-#pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                const bf16x8 fx = frag(xs[wave], kXRow, c * 16);
-#pragma unroll
-                for (int p = 1; p >= 0; --p)
-#pragma unroll
-                    for (int r = 0; r < kR; ++r)
-                        acc[c][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fy[p][r], fx, acc[c][r], 0, 0, 0)
-                                               : __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx, fy[p][r], acc[c][r], 0, 0, 0);
             }
         }
     } else {
-        for (int n0 = 0; n0 < count; n0 += 4) {
-            const bool there = n0 + g < count;
-            const int64_t n = rows[min(n0 + g, count - 1)];
-            float fx[kC], fy[kR];
+        constexpr int kDeep = kR == 4 ? 2 : 4;  // groups of 4 rows whose loads are in flight together
+        for (int n0 = 0; n0 < count; n0 += 4 * kDeep) {
+            float fx[kDeep][kC], fy[kDeep][kR];
+            int64_t n[kDeep];
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                const int col = c0 + c * 16 + i;
-                fx[c] = there && col < s.cols ? s.x[n * s.ld + col] : 0.f;
+            for (int b = 0; b < kDeep; ++b) n[b] = rows[min(n0 + 4 * b + g, count - 1)];
+#pragma unroll
+            for (int b = 0; b < kDeep; ++b) {
+                const bool there = n0 + 4 * b + g < count;
+#pragma unroll
+                for (int t = 0; t < kC; ++t) {
+                    const int col = c0 + t * 16 + i;
+                    fx[b][t] = there && col < s.cols ? s.x[n[b] * s.ld + col] : 0.f;
+                }
+#pragma unroll
+                for (int r = 0; r < kR; ++r) {
+                    const int at = r0 + r * 16 + i;
+                    fy[b][r] = there && at < s.y.pad ? s.y.p[n[b] * s.y.pad + at] : 0.f;
+                }
             }
 #pragma unroll
-            for (int r = 0; r < kR; ++r) {
-                const int at = r0 + r * 16 + i;
-                fy[r] = there && at < s.y.pad ? s.y.p[n * s.y.pad + at] : 0.f;
-            }
+            for (int b = 0; b < kDeep; ++b)
 #pragma unroll
-            for (int c = 0; c < kC; ++c)
+                for (int t = 0; t < kC; ++t)
 #pragma unroll
-                for (int r = 0; r < kR; ++r)
-                    acc[c][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x4f32(fy[r], fx[c], acc[c][r], 0, 0, 0)
-                                           : __builtin_amdgcn_mfma_f32_16x16x4f32(fx[c], fy[r], acc[c][r], 0, 0, 0);
+                    for (int r = 0; r < kR; ++r)
+                        acc[t][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x4f32(fy[b][r], fx[b][t], acc[t][r], 0, 0, 0)
+                                               : __builtin_amdgcn_mfma_f32_16x16x4f32(fx[b][t], fy[b][r], acc[t][r], 0, 0, 0);
         }
     }
-    T* const out = s.out + static_cast<int64_t>(k) * s.cols * s.rank;
+    const int64_t base = static_cast<int64_t>(k) * s.cols * s.rank;
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
+    for (int t = 0; t < kC; ++t)
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
-            const float x[4] = {acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]};
-            const int col = c0 + c * 16 + (kRanksLast ? i : 4 * g), rank = r0 + r * 16 + (kRanksLast ? 4 * g : i);
+            const float x[4] = {acc[t][r][0], acc[t][r][1], acc[t][r][2], acc[t][r][3]};
+            const int col = c0 + t * 16 + (kRanksLast ? i : 4 * g), rank = r0 + r * 16 + (kRanksLast ? 4 * g : i);
             if (col >= s.cols || rank >= s.rank) continue;
-            if (kRanksLast)
-                store_out(out + static_cast<int64_t>(col) * s.rank + rank, x, s.rank - rank);
+            const int64_t at = base + (kRanksLast ? static_cast<int64_t>(col) * s.rank + rank : static_cast<int64_t>(rank) * s.cols + col);
+            const int n = kRanksLast ? s.rank - rank : s.cols - col;
+            if (s.parts)
+                store_out(s.parts + split * s.size + at, x, n);
             else
-                store_out(out + static_cast<int64_t>(rank) * s.cols + col, x, s.cols - col);
+                store_out(s.out + at, x, n);
         }
 }
 
-// A of the adapters that have rows, transposed: [adapters][dim][rank].
+// An adapter's gradient from its parts, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void outer_join_kernel(OuterArgs<T> s) {
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (at >= s.size) return;
+    const int n = static_cast<int>(min(s.size - at, int64_t{4}));
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < s.splits; ++i) {
+        const float* const p = s.parts + i * s.size + at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += e < n ? p[e] : 0.f;
+    }
+    store_out(s.out + at, x, n);
+}
+
+// A of the adapters that have rows, transposed: [adapters][dim][rank], 8 ranks a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T* a, int rank, int dim, const int32_t* begin, T* to) {
-    const int k = blockIdx.y;
+    const int k = blockIdx.z;
     if (begin[k] == begin[k + 1]) return;
-    const int d = blockIdx.x * 256 + threadIdx.x;
+    const int d = blockIdx.x * 256 + threadIdx.x, r0 = blockIdx.y * 8;
     if (d >= dim) return;
-    const T* const p = a + static_cast<int64_t>(k) * rank * dim + d;
-    T* const q = to + (static_cast<int64_t>(k) * dim + d) * rank;
-    for (int r = 0; r < rank; ++r) q[r] = p[static_cast<int64_t>(r) * dim];
+    const T* const p = a + (static_cast<int64_t>(k) * rank + r0) * dim + d;
+    T* const q = to + (static_cast<int64_t>(k) * dim + d) * rank + r0;
+    T v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = r0 + r < rank ? p[static_cast<int64_t>(r) * dim] : T(0);
+    if (r0 + 8 <= rank) {
+        __builtin_memcpy(q, v, sizeof(v));
+    } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r0 + r < rank) q[r] = v[r];
+    }
 }
 
 template <typename T>
@@ -762,26 +973,39 @@ struct Call {
         return Adapters<T>{static_cast<const T*>(table), m, x.rank, x.adapters, x.adapter, low(u)};
     }
     template <bool kAlong>
-    void low_sum(const void* in, int64_t ld, int cols, const void* table, void* to, int splits) const {
+    void low_sum(const void* in, int64_t ld, int cols, const void* table, void* to) const {
+        const bool wide = sizeof(T) == 2 && x.rows > kFewRows;
+        const int tile = wide ? kWideRows : kRowTile, step = wide ? kWideStep : kSumStep;
+        const int splits = low_splits(x.rows, cols, wide);
         SumArgs<T> s{static_cast<const T*>(in), ld, x.rows, cols, static_cast<const T*>(table), x.scale, x.adapter, x.adapters, x.rank,
-                     low(to), splits > 1 ? b.du_parts : nullptr, splits, 0};
-        s.steps_per_split = ((cols + kSumStep - 1) / kSumStep + splits - 1) / splits;
-        const int slots = std::min(kRowTile, x.adapters);
+                     low(to), splits > 1 ? b.parts : nullptr, splits, 0};
+        s.steps_per_split = ((cols + step - 1) / step + splits - 1) / splits;
         by_rank(x.rank, [&](auto r) {
             constexpr int kR = decltype(r)::value;
             const int ranks = (s.y.pad + kR * 16 - 1) / (kR * 16);  // the padding too
-            low_sum_kernel<T, kAlong, kR><<<dim3((x.rows + kRowTile - 1) / kRowTile, slots, splits * ranks), 256, 0, st>>>(s);
+            const dim3 grid((x.rows + tile - 1) / tile, std::min(tile, x.adapters), splits * ranks);
+            if constexpr (sizeof(T) == 2) {
+                if (wide) {
+                    low_wide_kernel<kAlong, kR><<<grid, 256, 0, st>>>(s);
+                    return;
+                }
+            }
+            low_sum_kernel<T, kAlong, kR><<<grid, 64 * kSumWaves, 0, st>>>(s);
         });
         if (splits > 1) low_join_kernel<T><<<static_cast<unsigned>((static_cast<int64_t>(x.rows) * s.y.pad + 255) / 256), 256, 0, st>>>(s);
     }
     template <bool kRanksLast>
     void outer(const void* in, int64_t ld, int cols, void* y, void* out) const {
-        OuterArgs<T> s{static_cast<const T*>(in), ld, cols, x.rank, low(y), b.order, b.order + x.adapters + 1, static_cast<T*>(out)};
+        const int64_t size = static_cast<int64_t>(x.adapters) * cols * x.rank;
+        const int splits = outer_splits(x.rows, x.adapters, cols, size, plan.parts);
+        OuterArgs<T> s{static_cast<const T*>(in), ld, cols, x.rank, low(y), b.order, b.order + x.adapters + 1, static_cast<T*>(out),
+                       splits > 1 ? b.parts : nullptr, splits, size};
         by_rank(x.rank, [&](auto r) {
             constexpr int kR = decltype(r)::value;
-            outer_kernel<T, kRanksLast, kR>
-                <<<dim3((cols + 4 * kOuterCols - 1) / (4 * kOuterCols), (x.rank + kR * 16 - 1) / (kR * 16), x.adapters), 256, 0, st>>>(s);
+            outer_kernel<T, kRanksLast, kR><<<dim3((cols + 4 * kOuterCols - 1) / (4 * kOuterCols), (x.rank + kR * 16 - 1) / (kR * 16), x.adapters * splits),
+                                              256, 0, st>>>(s);
         });
+        if (splits > 1) outer_join_kernel<T><<<static_cast<unsigned>(((size + 3) / 4 + 255) / 256), 256, 0, st>>>(s);
     }
     template <typename Epi>
     void product(const Operand& w, const Operand& h, int n, const Epi& e) const {
@@ -805,7 +1029,7 @@ struct Call {
     }
     template <typename O>
     void forward() const {
-        if (x.adapters) low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u, 1);
+        if (x.adapters) low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u);
         const Operand h = rows(x.hidden, hidden_ld(), x.rows, x.dim, plan.pack_h, plan.kpad, b.hpack);
         const int64_t ld = x.rows > 1 ? x.out_stride : x.out_dim;
         for (int v0 = 0; v0 < x.out_dim; v0 += plan.piece) {
@@ -824,12 +1048,12 @@ struct Call {
     }
     void backward() const {
         const bool low_rank = x.adapters > 0;
-        if (low_rank && (x.dhidden || x.da)) low_sum<false>(x.dout, dout_ld(), x.out_dim, x.b, b.du, plan.low_splits);
+        if (low_rank && (x.dhidden || x.da)) low_sum<false>(x.dout, dout_ld(), x.out_dim, x.b, b.du);
         if (low_rank) order_kernel<<<x.adapters, 1024, 0, st>>>(x.adapter, x.rows, x.adapters, b.order, b.order + x.adapters + 1);
         if (x.dhidden) {
             if (low_rank)
-                transpose_kernel<T><<<dim3((x.dim + 255) / 256, x.adapters), 256, 0, st>>>(static_cast<const T*>(x.a), x.rank, x.dim, b.order,
-                                                                                         static_cast<T*>(b.at));
+                transpose_kernel<T><<<dim3((x.dim + 255) / 256, (x.rank + 7) / 8, x.adapters), 256, 0, st>>>(
+                    static_cast<const T*>(x.a), x.rank, x.dim, b.order, static_cast<T*>(b.at));
             T* const dh = static_cast<T*>(x.dhidden);
             const int64_t dh_ld = x.rows > 1 ? x.dhidden_stride : x.dim;
             const int64_t hld = (x.dim + 3) / 4 * 4;
@@ -846,14 +1070,12 @@ struct Call {
                     hidden(w, d, n, HiddenEpi<T, false>{low, x.rows, x.dim, b.dhidden, hld, x.rows * hld, v0 > 0});
             }
             if (!direct)
-                for_rows(x.rows, [&](int64_t r, unsigned n) {
-                    hidden_sum_kernel<T><<<dim3((x.dim + 255) / 256, n), 256, 0, st>>>(b.dhidden + r * hld, hld, x.rows * hld, plan.splits,
-                                                                                     x.dim, dh + r * dh_ld, dh_ld);
-                });
+                hidden_sum_kernel<T><<<static_cast<unsigned>((x.rows * hld / 4 + 255) / 256), 256, 0, st>>>(b.dhidden, hld, x.rows * hld, plan.splits,
+                                                                                                    x.rows, x.dim, dh, dh_ld);
         }
         if (x.da) outer<false>(x.hidden, hidden_ld(), x.dim, b.du, x.da);
         if (x.db) {
-            low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u, 1);
+            low_sum<true>(x.hidden, hidden_ld(), x.dim, x.a, b.u);
             outer<true>(x.dout, dout_ld(), x.out_dim, b.u, x.db);
         }
     }
@@ -943,7 +1165,7 @@ int ge_projection_create(int device, int max_rows, int max_dim, int max_out, int
     alloc(b.wpack, c.wpack);
     alloc(b.u, c.u);
     alloc(b.du, c.du);
-    alloc(b.du_parts, c.du_parts);
+    alloc(b.parts, c.parts);
     alloc(b.order, c.order);
     alloc(b.at, c.at);
     alloc(b.dpack, c.dpack);
@@ -960,7 +1182,7 @@ void ge_projection_destroy(ge_projection* h) {
     if (!h) return;
     ge::projection::OnDevice guard(h->device);
     const ge::projection::Buffers& b = h->buf;
-    for (void* p : {b.hpack, b.wpack, b.u, b.du, static_cast<void*>(b.du_parts), static_cast<void*>(b.order), b.at, b.dpack,
+    for (void* p : {b.hpack, b.wpack, b.u, b.du, static_cast<void*>(b.parts), static_cast<void*>(b.order), b.at, b.dpack,
                     static_cast<void*>(b.dhidden)})
         (void)hipFree(p);
     delete h;

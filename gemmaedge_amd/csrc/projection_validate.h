@@ -22,9 +22,12 @@ using head::kUnits;
 using head::round_up;
 using head::stride_ok;
 
-constexpr int kRowTile = 16;        // rows of a workgroup of the low-rank sums
-constexpr int kMaxLowSplits = 64;   // parts of such a sum over the outputs
-constexpr int kLowBlocks = 1024;    // workgroups that they are split up for
+constexpr int kRowTile = 16;        // rows of a workgroup of the low-rank sums,
+constexpr int kWideRows = 64;       // and of their form for many bf16 rows,
+constexpr int kFewRows = 128;       // which more rows than this take
+constexpr int kMaxLowSplits = 32;   // parts of such a sum
+constexpr int kLowBlocks = 512;     // workgroups that they are split up for
+constexpr int64_t kOuterBytes = 64LL << 20;  // most memory for the parts of an adapter's gradient
 
 // Ranks are padded to whole steps of the matrix instructions.
 inline int64_t rank_pad(int rank) { return round_up(rank, 32); }
@@ -36,7 +39,7 @@ struct Capacity {
     int64_t hpack;    // hidden states in padded rows
     int64_t wpack;    // a piece of the weights in padded rows
     int64_t u, du;    // the rows' low-rank values
-    int64_t du_parts; // float32 parts of du
+    int64_t parts;    // float32 parts of u, du, dA or dB, one after the other
     int64_t order;    // rows sorted by adapter, and where each one's begin
     int64_t at;       // A transposed
     int64_t dpack;    // a piece of dout in padded rows
@@ -50,7 +53,9 @@ inline void size_workspace(Capacity& c) {
     c.wpack = es * dim * std::min(out, std::max<int64_t>(kTileM, ((64LL << 20) / (2 * dim)) / kTileM * kTileM));
     const int64_t upad = rank_pad(c.max_rank);
     c.u = c.max_adapters ? 4 * rows * upad : 0;
-    c.du = c.du_parts = c.order = c.at = c.dpack = c.dhidden = 0;
+    // no call has more parts than fill the card, or than this many
+    c.parts = c.max_adapters ? 4 * upad * std::min(kMaxLowSplits * rows, kWideRows * std::max<int64_t>(kLowBlocks, (rows + kRowTile - 1) / kRowTile)) : 0;
+    c.du = c.order = c.at = c.dpack = c.dhidden = 0;
     if (!c.train) return;
     c.dpack = es * rows * std::min(out, std::max<int64_t>(kTileM, (256LL << 20) / (es * rows) / kTileM * kTileM));
     const int64_t tiles = (rows + 255) / 256 * ((dim + 255) / 256);
@@ -58,8 +63,9 @@ inline void size_workspace(Capacity& c) {
                                       std::min<int64_t>(head::kMaxSplits, (out + 63) / 64) * rows * round_up(c.max_dim, 4));
     if (!c.max_adapters) return;
     c.du = c.u;
-    const int64_t row_tiles = (rows + kRowTile - 1) / kRowTile;
-    c.du_parts = 4 * upad * std::min(kMaxLowSplits * rows, kRowTile * std::max<int64_t>(kLowBlocks, row_tiles));
+    // a small call's parts, and as many of a large one's as fit
+    const int64_t least = 4LL * c.max_adapters * c.max_rank * std::max(c.max_dim, c.max_out);
+    c.parts = std::max(c.parts, std::min(kOuterBytes, kMaxLowSplits * least));
     c.order = 4 * (rows + c.max_adapters + 1);
     c.at = es * c.max_adapters * static_cast<int64_t>(c.max_dim) * c.max_rank;
 }
@@ -84,13 +90,23 @@ struct Plan {
     int tile_m, tile_n;           // of the forward product
     int piece;                    // outputs of a launch
     int splits;                   // parts of the outputs' sum in dhidden
-    int low_splits;               // and in du
+    int64_t parts;                // bytes for those of the low-rank sums
 };
 
-// Parts of a low-rank sum over k elements: enough workgroups, of 128 elements at least.
-inline int low_splits(int rows, int k) {
-    const int tiles = (rows + kRowTile - 1) / kRowTile;
-    return std::max(1, std::min(std::min(kLowBlocks / std::max(tiles, 1), kMaxLowSplits), k / 128));
+// Parts of a low-rank sum over k elements: enough workgroups, of 4 steps at least.
+inline int low_splits(int rows, int k, bool wide) {
+    const int tile = wide ? kWideRows : kRowTile, least = wide ? 256 : 1024;
+    const int tiles = (rows + tile - 1) / tile;
+    return std::max(1, std::min(std::min(kLowBlocks / std::max(tiles, 1), kMaxLowSplits), k / least));
+}
+
+// Parts of an adapter's gradient, of `size` elements for all of them: enough workgroups
+// of 256 columns, of 256 rows each if the rows are spread evenly.
+inline int outer_splits(int rows, int adapters, int cols, int64_t size, int64_t bytes) {
+    const int64_t blocks = (cols + 255) / 256 * static_cast<int64_t>(adapters);
+    const int64_t most = std::min<int64_t>(bytes / (4 * size), 65535 / adapters);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxLowSplits, kLowBlocks / blocks),
+                                                                  std::min<int64_t>(most, rows / (256LL * adapters)))));
 }
 
 inline int check_project(const Capacity& c, const ge_project_args& x, bool backward, Plan& plan, char* msg, size_t n) {
@@ -152,7 +168,8 @@ inline int check_project(const Capacity& c, const ge_project_args& x, bool backw
     if (plan.pack_w) piece = std::min(piece, c.wpack / (static_cast<int64_t>(es) * plan.kpad) / kTileM * kTileM);
     if (plan.pack_d) piece = std::min(piece, c.dpack / (static_cast<int64_t>(es) * x.rows) / kTileM * kTileM);
     plan.piece = static_cast<int>(piece);
-    plan.splits = plan.low_splits = 1;
+    plan.splits = 1;
+    plan.parts = c.parts;
     if (backward) {
         // Parts of the sum over a piece, as in the loss's: rounds of tiles times the steps of one.
         const int64_t tile = c.dtype == GE_DTYPE_F32 ? kTile32 : 256, slots = c.dtype == GE_DTYPE_F32 ? 2 * kUnits : kUnits;
@@ -168,7 +185,6 @@ inline int check_project(const Capacity& c, const ge_project_args& x, bool backw
                 plan.splits = static_cast<int>(s);
             }
         }
-        plan.low_splits = low_splits(x.rows, x.out_dim);
     }
     return GE_OK;
 }

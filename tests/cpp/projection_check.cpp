@@ -128,12 +128,19 @@ static void plans() {
             if (p.pack_w) CHECK(es * n * p.kpad <= c.wpack);
             if (dtype == GE_DTYPE_BF16 && !p.pack_w) CHECK(x.weight_stride % 8 == 0 || x.out_dim == 1);
             CHECK(4 * x.rows * rank_pad(x.rank) <= c.u);
+            for (const bool wide : {false, true})
+                for (const int k : {x.dim, x.out_dim}) {
+                    const int64_t parts = low_splits(x.rows, k, wide);
+                    CHECK(parts >= 1 && (parts == 1 || 4 * parts * x.rows * rank_pad(x.rank) <= c.parts));
+                }
             if (!back) continue;
             if (p.pack_d) CHECK(es * x.rows * round_up(n, kPadK) <= c.dpack);
             CHECK(p.splits >= 1 && (p.splits == 1 || 4 * p.splits * x.rows * round_up(x.dim, 4) <= c.dhidden));
             CHECK(4LL * x.rows * round_up(x.dim, 4) <= c.dhidden);
-            CHECK(p.low_splits >= 1 && p.low_splits <= kMaxLowSplits);
-            CHECK(p.low_splits == 1 || 4LL * p.low_splits * x.rows * rank_pad(x.rank) <= c.du_parts);
+            for (const int cols : {x.dim, x.out_dim}) {
+                const int64_t size = static_cast<int64_t>(x.adapters) * x.rank * cols, parts = outer_splits(x.rows, x.adapters, cols, size, p.parts);
+                CHECK(parts >= 1 && parts * x.adapters <= 65535 && (parts == 1 || 4 * parts * size <= c.parts));
+            }
             CHECK(4LL * x.rows * rank_pad(x.rank) <= c.du);
             CHECK(4LL * (x.rows + x.adapters + 1) <= c.order);
             CHECK(es * x.adapters * x.dim * x.rank <= c.at);
