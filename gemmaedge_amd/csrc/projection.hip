@@ -80,20 +80,6 @@ __device__ __forceinline__ int wave_min(int x) {
     return __builtin_amdgcn_readfirstlane(x);
 }
 
-// The first n of 8 (or 4) elements, zeros for the others.
-__device__ __forceinline__ bf16x8 keep_below(u32x4 v, int n) {
-    if (n < 8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = 2 * e + 1 < n ? v[e] : 2 * e < n ? v[e] & 0xffffu : 0u;
-    }
-    return __builtin_bit_cast(bf16x8, v);
-}
-__device__ __forceinline__ f32x4 keep_below4(u32x4 v, int n) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < n ? v[e] : 0u;
-    return __builtin_bit_cast(f32x4, v);
-}
-
 // At most 2^31 - 16 bytes from p on, `left` of which are the operand's.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t left) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(max(int64_t{0}, min(left, int64_t{0x7ffffff0}))),
@@ -102,17 +88,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_
 __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t at) {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(at), 0, 0));
 }
-// 8 bf16 elements. The hardware checks bounds four bytes at a time, so the last of an odd
-// number of elements has to be loaded by itself; `odd` where there can be one.
-__device__ __forceinline__ u32x4 load8(__amdgpu_buffer_rsrc_t rs, uint32_t at, bool odd) {
-    if (!odd) return load16(rs, at);
+// The first n of a lane's elements of type T (8 or 4): what the others' bits are cut off by.
+template <typename T>
+__device__ __forceinline__ u32x4 mask_below(int n) {
+    u32x4 m;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        m[q] = sizeof(T) == 4 ? (q < n ? 0xffffffffu : 0u) : 2 * q + 1 < n ? 0xffffffffu : 2 * q < n ? 0xffffu : 0u;
+    return m;
+}
+// The hardware checks bounds four bytes at a time and reads a zero for the last of an odd number
+// of bf16 elements: `last`, read by itself, as element e of a lane's 8, to be added to that.
+__device__ __forceinline__ u32x4 at_element(int e, uint16_t last) {
     u32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint16_t lo = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(at + 4 * e), 0, 0);
-        const uint16_t hi = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(at + 4 * e + 2), 0, 0);
-        v[e] = lo | static_cast<uint32_t>(hi) << 16;
-    }
+    for (int q = 0; q < 4; ++q) v[q] = e >> 1 == q ? static_cast<uint32_t>(last) << 16 * (e & 1) : 0u;
     return v;
 }
 
@@ -138,92 +128,141 @@ __device__ __forceinline__ void hold(f32x4 (&acc)[kMt][kNt], int j) {
     }
 }
 
-// Ranks that a fragment of an adapter's rows has, and of how many the registers keep them.
+// Ranks of a chunk: of a fragment of an adapter's rows. Tall tiles have no registers for a
+// second one.
 template <typename T>
-constexpr int kFragRanks = sizeof(T) == 2 ? 32 : 16;
-constexpr int kKept = 2;
+constexpr int kChunk = sizeof(T) == 2 ? 32 : 16;
 
-// An adapter's rows of a wave, as the matrix instructions take them: kept while the
-// columns that follow have the same adapter.
+template <typename T>
+using Frag = typename std::conditional<sizeof(T) == 2, bf16x8, f32x4>::type;
+
+// An adapter's rows of a wave for the chunk of ranks from r0 on, as the matrix instructions take them.
+template <bool kAAlong, typename T, int kMt>
+__device__ __forceinline__ void load_table(const Adapters<T>& x, int64_t m0, int adapter, int r0, int lane, Frag<T> (&f)[kMt]) {
+    const int i = lane & 15, r = r0 + (kChunk<T> / 4) * (lane >> 4), left = x.rank - r;
+    // Rows past the last are another adapter's, or nothing: outputs that nobody reads.
+    const T* const end = x.table + x.adapters * x.m * x.rank;
+    const T* const p = x.table + (adapter * x.m + m0) * x.rank;
+    const auto rs = resource(p, (end - p) * static_cast<int64_t>(sizeof(T)));
+    const u32x4 below = mask_below<T>(left);
+    u32x4 tail{0, 0, 0, 0};
+    int last_row = -1;
+    if constexpr (sizeof(T) == 2) {
+        if ((x.rank & 1) && adapter == x.adapters - 1) {
+            last_row = static_cast<int>(min(x.m - 1 - m0, int64_t{INT_MAX}));
+            tail = at_element(left - 1, end[-1]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kMt; ++t) {
+        const int row = kAAlong ? epi_row(t, i) : t * 16 + i;
+        u32x4 v = load16(rs, left > 0 ? static_cast<uint32_t>(row * x.rank + r) * sizeof(T) : 0x80000000u) & below;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] |= row == last_row ? tail[q] : 0u;
+        }
+        f[t] = __builtin_bit_cast(Frag<T>, v);
+    }
+}
+
+// The row's own values for the same ranks, zeros without an adapter; bf16: both planes.
+struct RowValues {
+    u32x4 v[2];
+};
+template <typename T>
+__device__ __forceinline__ RowValues load_values(const Adapters<T>& x, int id, int64_t n, int r0, int lane) {
+    RowValues u;
+    u.v[0] = u.v[1] = u32x4{0, 0, 0, 0};
+    if (id >= 0) {
+        const T* const p = x.u.p + n * x.u.pad + r0 + (kChunk<T> / 4) * (lane >> 4);
+        u.v[0] = *reinterpret_cast<const u32x4*>(p);
+        if constexpr (sizeof(T) == 2) u.v[1] = *reinterpret_cast<const u32x4*>(p + x.u.plane);
+    }
+    return u;
+}
+
+// acc += table u for the lanes whose row is this adapter's. Products with the rows that are not its
+// own are left out, not added as zeros: an infinity in one request's adapter stays there.
 template <typename T, int kMt>
-struct TableRows {
-    typename std::conditional<sizeof(T) == 2, bf16x8, f32x4>::type f[kKept][kMt];
-    int k = -1, from = -1;
-    template <bool kAAlong>
-    __device__ __forceinline__ void load(const Adapters<T>& x, int64_t m0, int adapter, int r0, int lane) {
-        if (adapter == k && r0 == from) return;
-        k = adapter;
-        from = r0;
-        constexpr int kEach = sizeof(T) == 2 ? 8 : 4;  // ranks of a lane
-        const int i = lane & 15, g = lane >> 4;
-        const int64_t first = adapter * x.m + m0;
-        // Rows past the last lie behind the resource's end.
-        const auto rs = resource(x.table + first * x.rank, (x.m - m0) * x.rank * static_cast<int64_t>(sizeof(T)));
+__device__ __forceinline__ void add_products(const Frag<T> (&f)[kMt], const RowValues& u, bool mine, f32x4 (&acc)[kMt]) {
 #pragma unroll
-        for (int c = 0; c < kKept; ++c) {
-            const int r = r0 + c * kFragRanks<T> + kEach * g, left = x.rank - r;
-            if (r0 + c * kFragRanks<T> >= x.rank) break;
+    for (int t = 0; t < kMt; ++t) {
+        f32x4 y{0.f, 0.f, 0.f, 0.f};
+        if constexpr (sizeof(T) == 2) {
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t], __builtin_bit_cast(bf16x8, u.v[1]), y, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t], __builtin_bit_cast(bf16x8, u.v[0]), y, 0, 0, 0);
+        } else {
+            const f32x4 fu = __builtin_bit_cast(f32x4, u.v[0]);
 #pragma unroll
-            for (int t = 0; t < kMt; ++t) {
-                const int row = kAAlong ? epi_row(t, i) : t * 16 + i;
-                const uint32_t at = left > 0 ? static_cast<uint32_t>(row * x.rank + r) * sizeof(T) : 0x80000000u;
-                if constexpr (sizeof(T) == 2)
-                    f[c][t] = keep_below(load8(rs, at, x.rank & 1), left);
-                else
-                    f[c][t] = keep_below4(load16(rs, at), left);
+            for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][e], fu[e], y, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] += mine ? y[e] : 0.f;
+    }
+}
+
+// Adds table[k] u to columns of accumulators, one after the other, whose lanes i, i + 16, ... have row
+// n = n0 + i of adapter k = id, and whose first row along M is m0. A row's values are on their
+// way a column ahead. Tall tiles keep two chunks of the adapter's rows while the columns that
+// follow have the same; short ones, whose columns are rows of many requests, have those of
+// kBatch adapters in flight together (64 rows, 22 adapters of rank 16, width 2,816, 262,144 outputs:
+// 467 us one at a time, 415 us in twos or threes).
+template <bool kAAlong, typename T, int kMt, int kNt>
+struct AdapterSum {
+    static constexpr int kBatch = kMt <= 2 ? 2 : 1, kKept = kMt > 4 ? 2 : 1;
+    const Adapters<T>& x;
+    const int (&id)[kNt];
+    int64_t m0, n0;
+    int lane;
+    RowValues next[kKept];
+    Frag<T> f[kBatch][kKept][kMt];
+    int kept = -1;
+    __device__ __forceinline__ AdapterSum(const Adapters<T>& a, const int (&ids)[kNt], int64_t m, int64_t n, int l)
+        : x(a), id(ids), m0(m), n0(n), lane(l) {
+        if (x.adapters) values(0, 0, next);
+    }
+    __device__ __forceinline__ void values(int j, int r0, RowValues (&u)[kKept]) const {
+#pragma unroll
+        for (int c = 0; c < kKept; ++c)
+            if (r0 + c * kChunk<T> < x.rank) u[c] = load_values(x, id[j], n0 + j * 16, r0 + c * kChunk<T>, lane);
+    }
+    __device__ __forceinline__ void add(int j, f32x4 (&acc)[kMt]) {
+        constexpr int kStep = kKept * kChunk<T>;
+        if (!x.adapters) return;
+        RowValues u[kKept];
+#pragma unroll
+        for (int c = 0; c < kKept; ++c) u[c] = next[c];
+        if (j + 1 < kNt) values(j + 1, 0, next);
+        uint64_t left = __ballot(id[j] >= 0);
+        while (left) {
+            int k[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                k[b] = -1;
+                if (left) {
+                    k[b] = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left));
+                    left &= ~__ballot(id[j] == k[b]);
+                }
+            }
+            for (int r0 = 0; r0 < x.rank; r0 += kStep) {
+                if (x.rank > kStep) values(j, r0, u);
+                if (kBatch > 1 || k[0] != kept || x.rank > kStep) {
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                        for (int c = 0; c < kKept; ++c)
+                            if (k[b] >= 0 && r0 + c * kChunk<T> < x.rank) load_table<kAAlong>(x, m0, k[b], r0 + c * kChunk<T>, lane, f[b][c]);
+                    kept = k[0];
+                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                    for (int c = 0; c < kKept; ++c)
+                        if (k[b] >= 0 && r0 + c * kChunk<T> < x.rank) add_products<T>(f[b][c], u[c], id[j] == k[b], acc);
             }
         }
     }
 };
-
-// Adds table[k] u to a column of accumulators, whose lanes i, i + 16, ... have row n = n0 + i of
-// adapter k = id, and whose first row along M is m0. An adapter's products with the rows that
-// are not its own are left out, not added as zeros: an infinity in one request's
-// adapter stays there.
-template <bool kAAlong, typename T, int kMt>
-__device__ __forceinline__ void add_adapters(const Adapters<T>& x, TableRows<T, kMt>& rows, f32x4 (&acc)[kMt], int64_t m0, int id, int64_t n,
-                                             int lane) {
-    constexpr int kStep = kFragRanks<T>;
-    const int g = lane >> 4;
-    uint64_t left = __ballot(id >= 0);
-    while (left) {
-        const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const bool mine = id == k;
-        left &= ~__ballot(mine);
-        const T* const u = x.u.p + n * x.u.pad + (kStep / 4) * g;
-        for (int r0 = 0; r0 < x.rank; r0 += kKept * kStep) {
-            u32x4 p[kKept][2];
-#pragma unroll
-            for (int c = 0; c < kKept; ++c) {
-                p[c][0] = p[c][1] = u32x4{0, 0, 0, 0};
-                const int r = r0 + c * kStep;
-                if (mine && r < x.rank) {
-                    p[c][0] = *reinterpret_cast<const u32x4*>(u + r);
-                    if constexpr (sizeof(T) == 2) p[c][1] = *reinterpret_cast<const u32x4*>(u + x.u.plane + r);
-                }
-            }
-            rows.template load<kAAlong>(x, m0, k, r0, lane);
-#pragma unroll
-            for (int c = 0; c < kKept; ++c) {
-                if (r0 + c * kStep >= x.rank) break;
-#pragma unroll
-                for (int t = 0; t < kMt; ++t) {
-                    f32x4 y{0.f, 0.f, 0.f, 0.f};
-                    if constexpr (sizeof(T) == 2) {
-                        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows.f[c][t], __builtin_bit_cast(bf16x8, p[c][1]), y, 0, 0, 0);
-                        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows.f[c][t], __builtin_bit_cast(bf16x8, p[c][0]), y, 0, 0, 0);
-                    } else {
-                        const f32x4 fu = __builtin_bit_cast(f32x4, p[c][0]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.f[c][t][e], fu[e], y, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][e] += mine ? y[e] : 0.f;
-                }
-            }
-        }
-    }
-}
 
 // The adapters of a lane's rows, -1: none.
 template <int kNt>
@@ -276,7 +315,8 @@ struct OutEpi {
                                            float2*) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
-        TableRows<T, kMt> table;
+        if (row0 >= m) return;
+        AdapterSum<kAAlong, T, kMt, kNt> sum(low, s.id, v0 + row0, col0 + (lane & 15), lane);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             hold(acc, j);
@@ -284,7 +324,7 @@ struct OutEpi {
             f32x4 y[kMt];
 #pragma unroll
             for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
-            if (low.adapters && row0 < m) add_adapters<kAAlong>(low, table, y, v0 + row0, s.id[j], n, lane);
+            sum.add(j, y);
             if (n >= rows) continue;
             const int v = row0 + (lane >> 4) * 8;
             O* const o = out + n * ld + v;
@@ -324,7 +364,8 @@ struct HiddenEpi {
                                            int lane, float2*) const {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
-        TableRows<T, kMt> table;
+        if (row0 >= dim) return;
+        AdapterSum<kAAlong, T, kMt, kNt> sum(low, s.id, row0, col0 + (lane & 15), lane);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             hold(acc, j);
@@ -332,7 +373,7 @@ struct HiddenEpi {
             f32x4 y[kMt];
 #pragma unroll
             for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
-            if (low.adapters && place.split == 0 && row0 < dim) add_adapters<kAAlong>(low, table, y, row0, s.id[j], n, lane);
+            if (place.split == 0) sum.add(j, y);
             if (n >= rows) continue;
             const int d0 = row0 + 4 * (lane >> 4);
 #pragma unroll
@@ -469,6 +510,8 @@ __global__ __launch_bounds__(64 * kSumWaves) void low_sum_kernel(SumArgs<T> s) {
     if (k != INT_MAX && r0 < s.rank) {
         const T* const xr = s.x + min(n0 + i, s.rows - 1) * s.ld;
         const T* const table = s.table + k * (static_cast<int64_t>(s.rank) * s.cols);
+        const T* const end = s.table + s.adapters * (static_cast<int64_t>(s.rank) * s.cols);
+        const bool odd = (s.rank & 1) && k == s.adapters - 1;
         const int first = split * s.steps_per_split;
         const int last = min((s.cols + kSumStep - 1) / kSumStep, first + s.steps_per_split);
         for (int step = first + wave; step < last; step += kSumWaves * kBatch) {
@@ -487,13 +530,15 @@ __global__ __launch_bounds__(64 * kSumWaves) void low_sum_kernel(SumArgs<T> s) {
                     } else {
                         // 32 channels of the ranks, 8 a lane; columns past the rank belong to the next
                         // channel and to outputs that nobody reads.
-                        const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank,
-                                                 at < last ? (s.cols - c0) * static_cast<int64_t>(s.rank) * 2 : 0);
+                        const uint16_t* const p = table + static_cast<int64_t>(c0) * s.rank;
+                        const auto rs = resource(p, (end - p) * 2);
+                        const int rows = at < last ? s.cols - c0 : 0;
                         constexpr int kPerRow = kRanks / 8;
 #pragma unroll
                         for (int q = 0; q < kR; ++q) {
                             const int unit = q * 64 + lane, row = unit / kPerRow, col = unit % kPerRow * 8;
-                            fw[b][q] = load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
+                            fw[b][q] = load16(rs, row < rows && r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u);
+                            if (odd && row == rows - 1) fw[b][q] |= at_element(s.rank - 1 - r0 - col, end[-1]);
                         }
                     }
                 }
@@ -610,6 +655,8 @@ __global__ __launch_bounds__(256) void low_wide_kernel(SumArgs<uint16_t> s) {
     if (k != INT_MAX && r0 < s.rank) {
         const uint16_t* const xr = s.x + min(n, s.rows - 1) * s.ld;
         const uint16_t* const table = s.table + k * (static_cast<int64_t>(s.rank) * s.cols);
+        const uint16_t* const end = s.table + s.adapters * (static_cast<int64_t>(s.rank) * s.cols);
+        const bool odd = (s.rank & 1) && k == s.adapters - 1;
         const int first = split * s.steps_per_split;
         const int last = min((s.cols + kWideStep - 1) / kWideStep, first + s.steps_per_split);
         u32x4 fx[2], next[2], w[kPer];
@@ -617,7 +664,8 @@ __global__ __launch_bounds__(256) void low_wide_kernel(SumArgs<uint16_t> s) {
             const int c0 = step * kWideStep;
 #pragma unroll
             for (int h = 0; h < 2; ++h) next[h] = load_row8(xr + c0 + h * 32 + 8 * g, s.cols - (c0 + h * 32 + 8 * g));
-            const auto rs = resource(table + static_cast<int64_t>(c0) * s.rank, (s.cols - c0) * static_cast<int64_t>(s.rank) * 2);
+            const uint16_t* const p = table + static_cast<int64_t>(c0) * s.rank;
+            const auto rs = resource(p, (end - p) * 2);
 #pragma unroll
             for (int q = 0; q < kPer; ++q) {
                 const int unit = q * 256 + threadIdx.x;
@@ -627,7 +675,8 @@ __global__ __launch_bounds__(256) void low_wide_kernel(SumArgs<uint16_t> s) {
                     w[q] = load_row8(table + static_cast<int64_t>(min(r0 + row, s.rank - 1)) * s.cols + c, s.cols - c);
                 } else {
                     const int row = unit / (kRanks / 8), col = unit % (kRanks / 8) * 8;
-                    w[q] = load8(rs, r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u, s.rank & 1);
+                    w[q] = load16(rs, row < s.cols - c0 && r0 + col < s.rank ? static_cast<uint32_t>(row * s.rank + r0 + col) * 2 : 0x80000000u);
+                    if (odd && c0 + row == s.cols - 1) w[q] |= at_element(s.rank - 1 - r0 - col, end[-1]);
                 }
             }
         };
@@ -1021,6 +1070,8 @@ struct Call {
                 run<128, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 8, e);
         } else if (plan.tile_n == head::kSmallTileN) {
             run<head::kSmallTileM, head::kSmallTileN, 4, 1, true, true>(w, h, k, n, x.rows, 1, 4, e);
+        } else if (plan.tile_n == 64) {
+            run<head::kSmallTileM, 64, 4, 1, true, true>(w, h, k, n, x.rows, 1, 4, e);
         } else if (plan.tile_n == 128) {
             run<256, 128, 2, 2, true, true>(w, h, k, n, x.rows, 1, 6, e);
         } else {

@@ -79,6 +79,7 @@ static void refusals() {
         refuses(GE_ERR_INVALID_ARG, back, [](auto& x) { x.hidden_stride = 63; });
         refuses(GE_ERR_INVALID_ARG, back, [](auto& x) { x.weight_stride = 63; });
         refuses(GE_ERR_INVALID_ARG, back, [](auto& x) { x.hidden = at(4097); });
+        refuses(GE_ERR_INVALID_ARG, back, [](auto& x) { x.b = at(4097); });
         refuses(GE_ERR_INVALID_ARG, back, [](auto& x) { x.scale = static_cast<float*>(at(4098)); });
     }
     refuses(GE_ERR_INVALID_ARG, false, [](auto& x) { x.out = nullptr; });
