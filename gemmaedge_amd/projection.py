@@ -84,41 +84,42 @@ class Projection:
         self.close()
 
     def _args(self, hidden, weight, a, b, scale, adapter):
+        """The fields up to ``adapter``, checked."""
         if hidden.dim() != 2 or weight.dim() != 2:
             raise ValueError(f"hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}: [rows, dim] and [out, dim] are wanted")
-        (rows, dim), out = hidden.shape, weight.shape[0]
-        H._want(hidden, "hidden", self.dtype, (rows, dim), self.device)
-        H._want(weight, "weight", self.dtype, (out, dim), self.device)
-        x = ProjectArgs()
-        x.hidden, x.hidden_stride, x.weight, x.weight_stride = hidden.data_ptr(), H._stride(hidden), weight.data_ptr(), H._stride(weight)
-        x.rows, x.dim, x.out_dim = rows, dim, out
-        given = [t is not None for t in (a, b, scale, adapter)]
-        if not any(given):
-            return x, rows, dim, out
-        if not all(given):
+        device, dtype = self.device, self.dtype
+        rows, dim = shape = hidden.shape
+        out = weight.shape[0]
+        H._want(hidden, "hidden", dtype, shape, device)
+        H._want(weight, "weight", dtype, (out, dim), device)
+        head = (hidden.data_ptr(), hidden.stride(0) if rows > 1 else dim, weight.data_ptr(), weight.stride(0) if out > 1 else dim, rows, dim, out)
+        if a is None and b is None and scale is None and adapter is None:
+            return head + (0, 0, None, None, None, None)
+        if a is None or b is None or scale is None or adapter is None:
             raise ValueError("a, b, scale and adapter are given together")
         if a.dim() != 3:
             raise ValueError(f"a has shape {tuple(a.shape)}: [adapters, rank, dim] is wanted")
-        k, r = a.shape[:2]
-        for t, what, dtype, shape in ((a, "a", self.dtype, (k, r, dim)), (b, "b", self.dtype, (k, out, r)), (scale, "scale", torch.float32, (k,)),
-                                      (adapter, "adapter", torch.int32, (rows,))):
-            H._want(t, what, dtype, shape, self.device)
-            if not t.is_contiguous():
-                raise ValueError(f"{what} must be contiguous")
-        x.a, x.b, x.scale, x.adapter, x.rank, x.adapters = a.data_ptr(), b.data_ptr(), scale.data_ptr(), adapter.data_ptr(), r, k
-        return x, rows, dim, out
+        k, r, _ = a.shape
+        H._want(a, "a", dtype, (k, r, dim), device)
+        H._want(b, "b", dtype, (k, out, r), device)
+        H._want(scale, "scale", torch.float32, (k,), device)
+        H._want(adapter, "adapter", torch.int32, (rows,), device)
+        if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and adapter.is_contiguous()):
+            raise ValueError("a, b, scale and adapter must be contiguous")
+        return head + (r, k, a.data_ptr(), b.data_ptr(), scale.data_ptr(), adapter.data_ptr())
 
     def project(self, hidden, weight, a=None, b=None, scale=None, adapter=None, out=None, out_dtype=None, stream=None):
         """[rows, dim] hidden states times [out, dim] weights, and for each row whose
         ``adapter`` (int32 [rows]) k lies within [0, adapters) also scale[k] * b[k] @ (a[k] @ row):
         ``a`` [adapters, rank, dim], ``b`` [adapters, out, rank], ``scale`` float32 [adapters].
         Returns [rows, out] of ``out_dtype`` (None: the operands'; float32 or bfloat16), ``out`` if given."""
-        x, rows, _, n = self._args(hidden, weight, a, b, scale, adapter)
+        x = self._args(hidden, weight, a, b, scale, adapter)
+        rows, n = x[4], x[6]
         if out is not None and out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out has dtype {out.dtype}: {out_dtype} is wanted")
         handle, side = H._stream(stream, self.device)
         out = H._output(out, "out", (out.dtype if out is not None else out_dtype or self.dtype), (rows, n), self.device, side)
-        x.out, x.out_stride, x.out_dtype = out.data_ptr(), H._stride(out), H._dtype(out, "out")
+        x = ProjectArgs(*x, out.data_ptr(), H._stride(out), H._dtype(out, "out"))
         H._check(_library().ge_project(self._h, handle, ctypes.byref(x)))
         H._used(side, hidden, weight, a, b, scale, adapter, out)
         return out
@@ -128,7 +129,8 @@ class Projection:
         """Gradients of ``project`` for the gradient ``dout`` [rows, out] (the operands' dtype) of
         its output. Returns (dhidden, da, db), None for what is not wanted (``need_hidden``,
         ``need_adapters``) or, without adapters, not there. The weight has no gradient here."""
-        x, rows, dim, n = self._args(hidden, weight, a, b, scale, adapter)
+        x = ProjectArgs(*self._args(hidden, weight, a, b, scale, adapter))
+        rows, dim, n = x.rows, x.dim, x.out_dim
         H._want(dout, "dout", self.dtype, (rows, n), self.device)
         if a is None and (da is not None or db is not None):
             raise ValueError("da or db without adapters")

@@ -56,6 +56,7 @@ class RuleConfig:
             raise ValueError(f"{self}: finite values and a repetition_penalty above 0 are wanted")
 
 
+_NOTHING = RuleConfig().params()
 _ready = False
 
 
@@ -79,9 +80,11 @@ def row_params(configs: Sequence[RuleConfig], device="cuda"):
     return t.to(device)
 
 
-def _list(t, what, dtype, device):
-    """A flat list of any length."""
-    H._want(t, what, dtype, (t.numel(),), device)
+def _list(t, what, dtype, n, device):
+    """The address of a flat list of n elements."""
+    if t.dtype != dtype or t.numel() != n or t.get_device() != device.index or not t.is_contiguous():
+        H._want(t, what, dtype, (n,), device)
+    return t.data_ptr()
 
 
 def apply(logits, config: RuleConfig | None = None, out=None, out_dtype=None, history=None, history_offsets=None, ring=None,
@@ -112,69 +115,72 @@ def apply(logits, config: RuleConfig | None = None, out=None, out_dtype=None, hi
     rows, vocab = logits.shape
     if vocab == 0:
         raise ValueError("empty logits")
-    a = RuleArgs()
-    a.dtype = H._dtype(logits, "logits")
+    i32 = torch.int32
+    dtype = H._dtype(logits, "logits")
     H._want(logits, "logits", logits.dtype, logits.shape, device)
     if row_params is None:
-        config = RuleConfig() if config is None else config
-        config.check()
-        a.params = config.params()
+        params, rule_rows = (_NOTHING if config is None else config.params()), None
     else:
-        H._want(row_params, "row_params", torch.uint8, (rows * ctypes.sizeof(RuleParams),), device)
+        params, rule_rows = _NOTHING, _list(row_params, "row_params", torch.uint8, rows * ctypes.sizeof(RuleParams), device)
     if out is not None and out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out has dtype {out.dtype}: {out_dtype} is wanted")
+    ids = offsets = places = lens = prompt = None
+    capacity = 0
     if history is not None:
         if history_offsets is None:
             raise ValueError("history without history_offsets")
-        _list(history, "history", torch.int32, device)
-        H._want(history_offsets, "history_offsets", torch.int32, (rows + 1,), device)
-        a.history, a.history_offsets = history.data_ptr(), history_offsets.data_ptr()
-        if history.numel() == 0:  # its address may be NULL: no ids at all
-            a.history = None
+        n = history.numel()
+        ids, offsets = _list(history, "history", i32, n, device), _list(history_offsets, "history_offsets", i32, rows + 1, device)
+        if n == 0:  # its address may be NULL: no ids at all
+            ids = offsets = None
     if ring is not None:
         if history is not None:
             raise ValueError("history and ring are exclusive")
         if ring.dim() != 2 or not ring.is_contiguous() or ring.shape[1] < 1 or ring_len is None:
             raise ValueError("ring: contiguous [rows, capacity] with ring_len is wanted")
-        H._want(ring, "ring", torch.int32, (rows, ring.shape[1]), device)
-        H._want(ring_len, "ring_len", torch.int32, (rows,), device)
-        a.ring, a.ring_len, a.ring_capacity = ring.data_ptr(), ring_len.data_ptr(), ring.shape[1]
+        capacity = ring.shape[1]
+        H._want(ring, "ring", i32, (rows, capacity), device)
+        places, lens = ring.data_ptr(), _list(ring_len, "ring_len", i32, rows, device)
     if prompt_len is not None:
-        H._want(prompt_len, "prompt_len", torch.int32, (rows,), device)
+        prompt = _list(prompt_len, "prompt_len", i32, rows, device)
+    bias = bias_at = bias_to = None
     if bias_ids is not None:
         if bias_values is None or bias_offsets is None:
             raise ValueError("bias_ids without bias_values or bias_offsets")
-        _list(bias_ids, "bias_ids", torch.int32, device)
-        H._want(bias_values, "bias_values", torch.float32, (bias_ids.numel(),), device)
-        H._want(bias_offsets, "bias_offsets", torch.int32, (rows + 1,), device)
-        if bias_ids.numel():
-            a.bias_ids, a.bias_values, a.bias_offsets = bias_ids.data_ptr(), bias_values.data_ptr(), bias_offsets.data_ptr()
+        n = bias_ids.numel()
+        bias, bias_to = _list(bias_ids, "bias_ids", i32, n, device), _list(bias_values, "bias_values", torch.float32, n, device)
+        bias_at = _list(bias_offsets, "bias_offsets", i32, rows + 1, device)
+        if n == 0:
+            bias = bias_at = bias_to = None
+    words = which = None
+    masks = mask_stride = 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[1] < -(-vocab // 32):
             raise ValueError(f"mask has shape {tuple(mask.shape)}: [masks, {-(-vocab // 32)} words] is wanted")
-        H._want(mask, "mask", torch.int32, mask.shape, device)
+        masks = mask.shape[0]
+        H._want(mask, "mask", i32, mask.shape, device)
         if mask_rows is not None:
-            H._want(mask_rows, "mask_rows", torch.int32, (rows,), device)
-        elif mask.shape[0] < rows:
-            raise ValueError(f"{mask.shape[0]} masks for {rows} rows without mask_rows")
-        if mask.shape[0]:
-            a.mask, a.mask_stride, a.masks, a.mask_rows = mask.data_ptr(), H._stride(mask), mask.shape[0], S._ptr(mask_rows)
+            which = _list(mask_rows, "mask_rows", i32, rows, device)
+        elif masks < rows:
+            raise ValueError(f"{masks} masks for {rows} rows without mask_rows")
+        if masks:
+            words, mask_stride = mask.data_ptr(), H._stride(mask)
+        else:
+            which = None
     elif mask_rows is not None:
         raise ValueError("mask_rows without mask")
-    if flags is not None:
-        H._want(flags, "flags", torch.int32, (rows,), device)
+    flags_out = None if flags is None else _list(flags, "flags", i32, rows, device)
     handle, side = H._stream(stream, device)
     out = H._output(out, "out", (out.dtype if out is not None else out_dtype or logits.dtype), (rows, vocab), device, side)
-    a.out_dtype = H._dtype(out, "out")
-    a.logits, a.rows, a.vocab, a.row_stride = logits.data_ptr(), rows, vocab, H._stride(logits)
-    a.out, a.out_stride = out.data_ptr(), H._stride(out)
-    a.row_params, a.prompt_len, a.flags_out = S._ptr(row_params), S._ptr(prompt_len), S._ptr(flags)
-    if torch.cuda.current_device() == device.index:
+    a = RuleArgs(logits.data_ptr(), dtype, rows, vocab, H._stride(logits), out.data_ptr(), H._dtype(out, "out"), H._stride(out), params,
+                 rule_rows, ids, offsets, places, lens, capacity, prompt, bias, bias_to, bias_at, words, mask_stride, masks, which, flags_out)
+    if torch._C._cuda_getDevice() == device.index:
         rc = _library().ge_apply_rules(handle, ctypes.byref(a))
     else:
         with torch.cuda.device(device):
             rc = _library().ge_apply_rules(handle, ctypes.byref(a))
     H._check(rc)
-    H._used(side, logits, out, history, history_offsets, ring, ring_len, prompt_len, bias_ids, bias_values, bias_offsets, mask,
-            mask_rows, row_params, flags)
+    if side is not None:
+        H._used(side, logits, out, history, history_offsets, ring, ring_len, prompt_len, bias_ids, bias_values, bias_offsets, mask,
+                mask_rows, row_params, flags)
     return out.view(shape) if len(shape) == 1 else out
