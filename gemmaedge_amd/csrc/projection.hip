@@ -144,25 +144,34 @@ __device__ __forceinline__ void load_table(const Adapters<T>& x, int64_t m0, int
     const T* const end = x.table + x.adapters * x.m * x.rank;
     const T* const p = x.table + (adapter * x.m + m0) * x.rank;
     const auto rs = resource(p, (end - p) * static_cast<int64_t>(sizeof(T)));
-    const u32x4 below = mask_below<T>(left);
-    u32x4 tail{0, 0, 0, 0};
-    int last_row = -1;
-    if constexpr (sizeof(T) == 2) {
-        if ((x.rank & 1) && adapter == x.adapters - 1) {
-            last_row = static_cast<int>(min(x.m - 1 - m0, int64_t{INT_MAX}));
-            tail = at_element(left - 1, end[-1]);
-        }
-    }
+    u32x4 v[kMt];
 #pragma unroll
     for (int t = 0; t < kMt; ++t) {
         const int row = kAAlong ? epi_row(t, i) : t * 16 + i;
-        u32x4 v = load16(rs, left > 0 ? static_cast<uint32_t>(row * x.rank + r) * sizeof(T) : 0x80000000u) & below;
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] |= row == last_row ? tail[q] : 0u;
-        }
-        f[t] = __builtin_bit_cast(Frag<T>, v);
+        v[t] = load16(rs, left > 0 ? static_cast<uint32_t>(row * x.rank + r) * sizeof(T) : 0x80000000u);
     }
+    if (x.rank % (kChunk<T> / 4)) {  // a row ends within a lane's elements
+        const u32x4 below = mask_below<T>(left);
+        u32x4 tail{0, 0, 0, 0};
+        int last_row = -1;
+        if constexpr (sizeof(T) == 2) {
+            if ((x.rank & 1) && adapter == x.adapters - 1) {
+                last_row = static_cast<int>(min(x.m - 1 - m0, int64_t{INT_MAX}));
+                tail = at_element(left - 1, end[-1]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kMt; ++t) {
+            v[t] &= below;
+            if constexpr (sizeof(T) == 2) {
+                const int row = kAAlong ? epi_row(t, i) : t * 16 + i;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[t][q] |= row == last_row ? tail[q] : 0u;
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kMt; ++t) f[t] = __builtin_bit_cast(Frag<T>, v[t]);
 }
 
 // The row's own values for the same ranks, zeros without an adapter; bf16: both planes.
