@@ -192,39 +192,73 @@ __device__ __forceinline__ RowValues load_values(const Adapters<T>& x, int id, i
 
 // acc += table u for the lanes whose row is this adapter's. Products with the rows that are not its
 // own are left out, not added as zeros: an infinity in one request's adapter stays there.
-template <typename T, int kMt>
-__device__ __forceinline__ void add_products(const Frag<T> (&f)[kMt], const RowValues& u, bool mine, f32x4 (&acc)[kMt]) {
+template <typename T>
+__device__ __forceinline__ void add_product(const Frag<T>& f, const RowValues& u, bool mine, f32x4& acc) {
+    f32x4 y{0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(T) == 2) {
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, u.v[1]), y, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, u.v[0]), y, 0, 0, 0);
+    } else {
+        const f32x4 fu = __builtin_bit_cast(f32x4, u.v[0]);
 #pragma unroll
-    for (int t = 0; t < kMt; ++t) {
-        f32x4 y{0.f, 0.f, 0.f, 0.f};
-        if constexpr (sizeof(T) == 2) {
-            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t], __builtin_bit_cast(bf16x8, u.v[1]), y, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[t], __builtin_bit_cast(bf16x8, u.v[0]), y, 0, 0, 0);
-        } else {
-            const f32x4 fu = __builtin_bit_cast(f32x4, u.v[0]);
+        for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[e], fu[e], y, 0, 0, 0);
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[t][e], fu[e], y, 0, 0, 0);
+    for (int e = 0; e < 4; ++e) acc[e] += mine ? y[e] : 0.f;
+}
+
+// Adds table[k] u to the accumulators, whose column j has row n0 + 16 j in lanes i, i + 16, ... (n0: of
+// lane i), of adapter k = id[j], and whose first row along M is m0.
+//
+// Short tiles, whose columns are rows of many requests: one adapter after the other over all
+// columns, its rows loaded once (64 rows, 22 adapters of rank 16, width 2,816, 262,144 outputs: 352
+// us, 279 of them without adapters; column by column 372 us; two adapters' rows in flight
+// together take registers and with them workgroups of a compute unit, which hide more: 384 us).
+template <bool kAAlong, typename T, int kMt, int kNt>
+__device__ __forceinline__ void add_adapters(const Adapters<T>& x, const int (&id)[kNt], int64_t m0, int64_t n0, int lane, f32x4 (&acc)[kMt][kNt]) {
+    if (!x.adapters) return;
+    for (int r0 = 0; r0 < x.rank; r0 += kChunk<T>) {
+        RowValues u[kNt];
+        uint64_t left[kNt];
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+            u[j] = load_values(x, id[j], n0 + j * 16, r0, lane);
+            left[j] = __ballot(id[j] >= 0);
         }
+        for (;;) {
+            int k = -1;
+            Frag<T> f[kMt];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] += mine ? y[e] : 0.f;
+            for (int j = 0; j < kNt; ++j)
+                if (k < 0 && left[j]) k = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left[j]));
+            if (k >= 0) {
+#pragma unroll
+                for (int j = 0; j < kNt; ++j) left[j] &= ~__ballot(id[j] == k);
+                load_table<kAAlong>(x, m0, k, r0, lane, f);
+            }
+            if (k < 0) break;
+            // Columns without this adapter add nothing: that is cheaper than branches around them.
+#pragma unroll
+            for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+                for (int t = 0; t < kMt; ++t) add_product<T>(f[t], u[j], id[j] == k && k >= 0, acc[t][j]);
+            }
+        }
     }
 }
 
-// Adds table[k] u to columns of accumulators, one after the other, whose lanes i, i + 16, ... have row
-// n = n0 + i of adapter k = id, and whose first row along M is m0. A row's values are on their
-// way a column ahead. Tall tiles keep two chunks of the adapter's rows while the columns that
-// follow have the same; short ones, whose columns are rows of many requests, have those of
-// kBatch adapters in flight together (64 rows, 22 adapters of rank 16, width 2,816, 262,144 outputs:
-// 467 us one at a time, 415 us in twos or threes).
+// Tall tiles, whose accumulators are read once and not written again: column by column, a row's values on
+// their way a column ahead, two chunks of the adapter's rows kept while the columns that follow
+// have the same adapter.
 template <bool kAAlong, typename T, int kMt, int kNt>
 struct AdapterSum {
-    static constexpr int kBatch = kMt <= 2 ? 2 : 1, kKept = kMt > 4 ? 2 : 1;
+    static constexpr int kKept = 2;
     const Adapters<T>& x;
     const int (&id)[kNt];
     int64_t m0, n0;
     int lane;
     RowValues next[kKept];
-    Frag<T> f[kBatch][kKept][kMt];
+    Frag<T> f[kKept][kMt];
     int kept = -1;
     __device__ __forceinline__ AdapterSum(const Adapters<T>& a, const int (&ids)[kNt], int64_t m, int64_t n, int l)
         : x(a), id(ids), m0(m), n0(n), lane(l) {
@@ -244,34 +278,36 @@ struct AdapterSum {
         if (j + 1 < kNt) values(j + 1, 0, next);
         uint64_t left = __ballot(id[j] >= 0);
         while (left) {
-            int k[kBatch];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                k[b] = -1;
-                if (left) {
-                    k[b] = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left));
-                    left &= ~__ballot(id[j] == k[b]);
-                }
-            }
+            const int k = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left));
+            left &= ~__ballot(id[j] == k);
             for (int r0 = 0; r0 < x.rank; r0 += kStep) {
                 if (x.rank > kStep) values(j, r0, u);
-                if (kBatch > 1 || k[0] != kept || x.rank > kStep) {
-#pragma unroll
-                    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-                        for (int c = 0; c < kKept; ++c)
-                            if (k[b] >= 0 && r0 + c * kChunk<T> < x.rank) load_table<kAAlong>(x, m0, k[b], r0 + c * kChunk<T>, lane, f[b][c]);
-                    kept = k[0];
-                }
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b)
+                if (k != kept || x.rank > kStep) {
 #pragma unroll
                     for (int c = 0; c < kKept; ++c)
-                        if (k[b] >= 0 && r0 + c * kChunk<T> < x.rank) add_products<T>(f[b][c], u[c], id[j] == k[b], acc);
+                        if (r0 + c * kChunk<T> < x.rank) load_table<kAAlong>(x, m0, k, r0 + c * kChunk<T>, lane, f[c]);
+                    kept = k;
+                }
+#pragma unroll
+                for (int c = 0; c < kKept; ++c)
+                    if (r0 + c * kChunk<T> < x.rank) {
+#pragma unroll
+                        for (int t = 0; t < kMt; ++t) add_product<T>(f[c][t], u[c], id[j] == k, acc[t]);
+                    }
             }
         }
     }
 };
+template <int kMt, int kNt>
+constexpr bool kTall = kMt * kNt >= 32;
+
+// Nothing by columns: short tiles have it all by then.
+struct NoSum {
+    template <typename... Args>
+    __device__ __forceinline__ explicit NoSum(const Args&...) {}
+};
+template <bool kAAlong, typename T, int kMt, int kNt>
+using ColumnSum = typename std::conditional<kTall<kMt, kNt>, AdapterSum<kAAlong, T, kMt, kNt>, NoSum>::type;
 
 // The adapters of a lane's rows, -1: none.
 template <int kNt>
@@ -325,7 +361,8 @@ struct OutEpi {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
         if (row0 >= m) return;
-        AdapterSum<kAAlong, T, kMt, kNt> sum(low, s.id, v0 + row0, col0 + (lane & 15), lane);
+        if constexpr (!kTall<kMt, kNt>) add_adapters<kAAlong>(low, s.id, v0 + row0, col0 + (lane & 15), lane, acc);
+        ColumnSum<kAAlong, T, kMt, kNt> sum(low, s.id, v0 + row0, col0 + (lane & 15), lane);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             hold(acc, j);
@@ -333,7 +370,7 @@ struct OutEpi {
             f32x4 y[kMt];
 #pragma unroll
             for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
-            sum.add(j, y);
+            if constexpr (kTall<kMt, kNt>) sum.add(j, y);
             if (n >= rows) continue;
             const int v = row0 + (lane >> 4) * 8;
             O* const o = out + n * ld + v;
@@ -374,7 +411,10 @@ struct HiddenEpi {
         constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
         const int row0 = m0 + wm * kWm, col0 = n0 + wn * kWn;
         if (row0 >= dim) return;
-        AdapterSum<kAAlong, T, kMt, kNt> sum(low, s.id, row0, col0 + (lane & 15), lane);
+        if constexpr (!kTall<kMt, kNt>) {
+            if (place.split == 0) add_adapters<kAAlong>(low, s.id, row0, col0 + (lane & 15), lane, acc);
+        }
+        ColumnSum<kAAlong, T, kMt, kNt> sum(low, s.id, row0, col0 + (lane & 15), lane);
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
             hold(acc, j);
@@ -382,7 +422,9 @@ struct HiddenEpi {
             f32x4 y[kMt];
 #pragma unroll
             for (int i = 0; i < kMt; ++i) y[i] = acc[i][j];
-            if (place.split == 0) sum.add(j, y);
+            if constexpr (kTall<kMt, kNt>) {
+                if (place.split == 0) sum.add(j, y);
+            }
             if (n >= rows) continue;
             const int d0 = row0 + 4 * (lane >> 4);
 #pragma unroll
@@ -907,7 +949,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
             }
         }
     } else {
-        constexpr int kDeep = kR == 4 ? 2 : 4;  // groups of 4 rows whose loads are in flight together
+        constexpr int kDeep = kR == 4 ? 4 : 8;  // groups of 4 rows whose loads are in flight together
         for (int n0 = 0; n0 < count; n0 += 4 * kDeep) {
             float fx[kDeep][kC], fy[kDeep][kR];
             int64_t n[kDeep];

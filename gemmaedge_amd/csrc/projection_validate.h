@@ -96,7 +96,7 @@ struct Plan {
 // Parts of a low-rank sum over k elements: enough workgroups, of a few steps a wave at least;
 // a join costs 4.5 us.
 inline int low_splits(int rows, int k, bool wide) {
-    const int tile = wide ? kWideRows : kRowTile, least = wide ? 256 : 4096;
+    const int tile = wide ? kWideRows : kRowTile, least = wide ? 256 : 2048;
     const int tiles = (rows + tile - 1) / tile;
     return std::max(1, std::min(std::min(kLowBlocks / std::max(tiles, 1), kMaxLowSplits), k / least));
 }
@@ -159,8 +159,8 @@ inline int check_project(const Capacity& c, const ge_project_args& x, bool backw
             }
         }
     } else {
-        // 64 rows with 22 adapters, width 2,816, 262,144 outputs: 415 us in tiles of 64 rows, 430
-        // in two of 32, between which the weights pass LDS twice
+        // 64 rows, width 2,816, 262,144 outputs: 279 us in tiles of 64 rows, 351 in two of 32, for
+        // which the weights pass LDS twice
         const bool small = x.rows <= head::kSmallRows;
         plan.tile_m = small ? head::kSmallTileM : kTileM;
         plan.tile_n = x.rows <= head::kSmallTileN ? head::kSmallTileN : small ? 64 : x.rows <= 128 ? 128 : 256;
