@@ -135,6 +135,27 @@ def test_pieces_of_dout():
     check(4096, 64, 40001, 8, 3, "bf16", seed=9, runs=50)
 
 
+@pytest.mark.parametrize("dt", ("bf16", "f32"))
+def test_rows_far_apart(dt):
+    """Rows whose offsets in a tile pass 31 bits are packed first."""
+    from gemmaedge_amd import projection as P
+
+    far = (1 << 21) + 16
+    s, dout = inputs(20, 64, 70, 8, 3, DT[dt])
+    p = P.Projection(20, 64, 70, 8, 3, dtype=DT[dt], train=True)
+    want = [p.project(**s), *p.project_backward(dout, **s)]
+    apart = dict(s)
+    for k in ("hidden", "weight"):
+        wide = torch.empty(s[k].shape[0], far, device="cuda", dtype=DT[dt])
+        wide[:, :64] = s[k]
+        apart[k] = wide[:, :64]
+    wide = torch.empty(20, far, device="cuda", dtype=DT[dt])
+    wide[:, :70] = dout
+    got = [p.project(**apart), *p.project_backward(wide[:, :70], **apart)]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 def test_many_adapters():
     check(500, 128, 400, 4, 700, "bf16")
     check(300, 64, 200, 4, 700, "f32")

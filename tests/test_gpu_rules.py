@@ -128,7 +128,7 @@ def make(rows, vocab, dt, history=0, bias=0, masks=False, cap=0.0, per_row=False
     (5, 33, 40, 9, True, 2.0, True, 0), (4, 2048, 0, 5, False, 0.0, False, 0), (6, 2049, 700, 0, True, 0.0, False, 3),
     (9, 4100, 5000, 300, True, 0.0, True, 8), (2, 50257, 9000, 70, True, 30.0, False, 0), (7, 20001, 0, 0, True, 0.0, False, 0),
     (150, 33001, 90, 20, True, 0.0, True, 0), (70, 70000, 40, 0, False, 0.0, False, 2), (65, 66000, 300, 30, True, 30.0, True, 0),
-    (3, 262144, 4097, 40, False, 0.0, False, 0)])
+    (3, 262144, 4097, 40, False, 0.0, False, 0), (100, 70001, 6001, 20, True, 0.0, True, 0), (90, 70001, 50, 6001, False, 0.0, False, 0)])
 def test_rules(rows, vocab, history, bias, masks, cap, per_row, pad, dt, to):
     from gemmaedge_amd import rules as R
 
