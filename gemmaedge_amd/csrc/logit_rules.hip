@@ -91,8 +91,7 @@ __device__ __forceinline__ void for_list(const int32_t* ids, int n, F f) {
                 for (int e = 0; e < 4; ++e) f(static_cast<int>(i) + k * kStep + e, q[k].v[e]);
             }
     }
-    const int rest = (n & ~3) + static_cast<int>(threadIdx.x);
-    if (rest < n && threadIdx.x < 3) f(rest, ids[rest]);
+    if (threadIdx.x < (n & 3)) f((n & ~3) + static_cast<int>(threadIdx.x), ids[(n & ~3) + threadIdx.x]);
 }
 
 // ---- what a row asks for ----------------------------------------------------------
@@ -306,7 +305,8 @@ __device__ __forceinline__ void count_direct(const Lists& lists, int t0, int len
 template <typename T, typename O>
 __device__ __forceinline__ void single(const ge_rule_args& x, int64_t row, int t0, int end, SingleLds& lds) {
     const Lists lists(x, row);
-    if (lists.n + lists.biases == 0) return;
+    const int64_t all = static_cast<int64_t>(lists.n) + lists.biases;  // each up to 2^31 - 1
+    if (all == 0) return;
     const ge_rule_params p = row_rules(x, row);
     const uint32_t* const mask = row_mask(x, row);
     const T* const in = static_cast<const T*>(x.logits) + row * x.row_stride;
@@ -314,7 +314,7 @@ __device__ __forceinline__ void single(const ge_rule_args& x, int64_t row, int t
     auto finish = [&](int token, T raw, uint32_t word, int bias) {
         out[token] = from_f32<O>(penalised(softcap(to_f32(raw), p.softcap), p, word, bias, lists.bias_values));
     };
-    if (end - t0 <= kDirect || lists.n > kMostHashed || lists.n + lists.biases > kMostHashed) {
+    if (end - t0 <= kDirect || all > kMostHashed) {
         const auto& d = lds.direct;
         for (int first = t0; first < end; first += kDirect) {
             const int length = min(kDirect, end - first);
@@ -377,11 +377,11 @@ __device__ __forceinline__ void single(const ge_rule_args& x, int64_t row, int t
     for (int first = 0; first < kSlots; first += kSingleThreads) {
         const int s = first + threadIdx.x;
         const bool mine = s < kSlots && h.key[s] >= 0;
-        const uint64_t all = __ballot(mine);
+        const uint64_t in_use = __ballot(mine);
         int base = 0;
-        if ((threadIdx.x & 63) == 0 && all) base = atomicAdd(&h.n_used, __popcll(all));
+        if ((threadIdx.x & 63) == 0 && in_use) base = atomicAdd(&h.n_used, __popcll(in_use));
         base = __shfl(base, 0);
-        if (mine) h.used[base + __popcll(all & ((1ull << (threadIdx.x & 63)) - 1))] = static_cast<uint16_t>(s);
+        if (mine) h.used[base + __popcll(in_use & ((1ull << (threadIdx.x & 63)) - 1))] = static_cast<uint16_t>(s);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < h.n_used; i += kSingleThreads) {

@@ -221,6 +221,31 @@ def test_no_rows_and_empty_lists():
     assert torch.equal(got, y)
 
 
+@pytest.mark.parametrize("to", ("new", "inplace"))
+def test_longest_lists(to):
+    """A history and a list of biases whose lengths add up to more than 31 bits, in one of so many rows
+    that a slice of the vocabulary has more tokens than are counted by a word each."""
+    from gemmaedge_amd import rules as R
+
+    rows, vocab, n, m = 512, 8200, 4999, 2 ** 31 - 1
+    x = torch.randn(rows, vocab, device="cuda")
+    ids = (torch.arange(n, device="cuda") % 4999).int()
+    offs = torch.full((rows + 1,), n, dtype=torch.int32, device="cuda")
+    offs[0] = 0
+    bias_ids = torch.arange(vocab, device="cuda", dtype=torch.int32).repeat(m // vocab + 1)[:m]
+    values = torch.full((m,), math.nan, device="cuda")
+    last = torch.randn(vocab, device="cuda")
+    values[m - vocab:] = last
+    bias_offs = torch.full((rows + 1,), m, dtype=torch.int32, device="cuda")
+    bias_offs[0] = 0
+    want = x.clone()
+    want[0, :n] -= 1.5
+    want[0, bias_ids[m - vocab:].long()] += last
+    got = R.apply(x, R.RuleConfig(presence_penalty=1.5), out=x if to == "inplace" else None, history=ids, history_offsets=offs,
+                  bias_ids=bias_ids, bias_values=values, bias_offsets=bias_offs)
+    assert torch.equal(got, want)
+
+
 def test_more_rows_than_a_launch():
     from gemmaedge_amd import rules as R
 
