@@ -14,6 +14,7 @@ namespace ge {
 namespace rules {
 
 constexpr int kMostVocab = 1 << 30;
+constexpr int kMostRows = 1 << 24;
 
 inline int size_of(int dtype) { return dtype == GE_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == GE_DTYPE_F32 || dtype == GE_DTYPE_BF16; }
@@ -26,7 +27,8 @@ inline bool in_place(const ge_rule_args& x) { return x.out == x.logits; }
 
 inline int check_rules(const ge_rule_args& x, char* msg, size_t n) {
     if (x.rows < 0 || x.vocab < 1) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "rows %d, vocab %d", x.rows, x.vocab);
-    if (x.vocab > kMostVocab) return plan_fail(msg, n, GE_ERR_CAPACITY, "vocab %d above %d", x.vocab, kMostVocab);
+    if (x.rows > kMostRows || x.vocab > kMostVocab)
+        return plan_fail(msg, n, GE_ERR_CAPACITY, "rows %d / vocab %d above %d / %d", x.rows, x.vocab, kMostRows, kMostVocab);
     if (!dtype_ok(x.dtype) || !dtype_ok(x.out_dtype))
         return plan_fail(msg, n, GE_ERR_INVALID_ARG, "dtype %d, out_dtype %d", x.dtype, x.out_dtype);
     if (!x.row_params) {

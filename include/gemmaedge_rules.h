@@ -50,7 +50,7 @@ typedef struct ge_rule_params {
 typedef struct ge_rule_args {
     const void* logits;        /* device, row r at logits + r * row_stride elements */
     int32_t dtype;             /* GE_DTYPE_F32 or GE_DTYPE_BF16 */
-    int32_t rows;              /* >= 0 */
+    int32_t rows;              /* 0 .. 2^24 */
     int32_t vocab;             /* 1 .. 2^30 */
     int64_t row_stride;        /* >= vocab */
     void* out;                 /* device, rows out_stride elements apart: another memory than the

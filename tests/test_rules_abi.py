@@ -78,6 +78,8 @@ def test_other_refusals():
     L = R._library()
     assert L.ge_apply_rules(None, None) == S.GE_ERR_INVALID_ARG
     assert L.ge_apply_rules(None, ctypes.byref(_args(vocab=(1 << 30) + 1, row_stride=1 << 31, out_stride=1 << 31))) == S.GE_ERR_CAPACITY
+    assert L.ge_apply_rules(None, ctypes.byref(_args(rows=(1 << 24) + 1))) == S.GE_ERR_CAPACITY
+    assert L.ge_apply_rules(None, ctypes.byref(_args(rows=(1 << 31) - 1, mask=None))) == S.GE_ERR_CAPACITY
     assert L.ge_apply_rules(None, ctypes.byref(_args(rows=0, logits=None, out=None))) == S.GE_OK
 
 
