@@ -135,6 +135,11 @@ def test_pieces_of_dout():
     check(4096, 64, 40001, 8, 3, "bf16", seed=9, runs=50)
 
 
+def test_pieces_of_more_rows_than_a_grid_has():
+    # dhidden's parts of 70,001 rows, whose dout is packed 1,792 outputs at a time.
+    check(70001, 36, 1801, 4, 2, "bf16", seed=5, runs=700)
+
+
 @pytest.mark.parametrize("dt", ("bf16", "f32"))
 def test_rows_far_apart(dt):
     """Rows whose offsets in a tile pass 31 bits are packed first."""
