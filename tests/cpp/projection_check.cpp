@@ -135,7 +135,7 @@ static void plans() {
                     CHECK(parts >= 1 && (parts == 1 || 4 * parts * x.rows * rank_pad(x.rank) <= c.parts));
                 }
             if (!back) continue;
-            if (p.pack_d) CHECK(es * x.rows * round_up(n, kPadK) <= c.dpack);
+            if (p.pack_d) CHECK(es * x.rows * round_up(n, kPadK) <= c.dpack && round_up(n, kPadK) <= ge::head::kMaxStride);
             CHECK(p.splits >= 1 && (p.splits == 1 || 4 * p.splits * x.rows * round_up(x.dim, 4) <= c.dhidden));
             CHECK(4LL * x.rows * round_up(x.dim, 4) <= c.dhidden);
             for (const int cols : {x.dim, x.out_dim}) {
