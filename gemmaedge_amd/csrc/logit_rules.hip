@@ -202,6 +202,11 @@ __device__ __forceinline__ uint32_t unit_mask(const uint32_t* mask, int t, int n
     return mask && n > 0 ? mask[t >> 5] >> (t & 31) & kAll : kAll;
 }
 
+// Bound by memory: 512 rows of 262,144 bf16 logits, capped and masked, into float32 212 us, 3.8 TB/s read and
+// written (4.9 is what a copy reaches); without the table of softcaps their evaluation
+// bounds it. Two units a thread from 2^24 tokens on: more loads in flight, while fewer
+// tokens make more workgroups of one.
+//
 // Every token of the rows from `first_row` on, in pieces of kUnits units a thread, `pieces` to a row, of
 // which a workgroup takes every `step`-th from `item` on: it makes the table once, and a
 // piece's loads are in flight while the one before is worked on.
@@ -301,7 +306,10 @@ __device__ __forceinline__ void count_direct(const Lists& lists, int t0, int len
     __syncthreads();
 }
 
-// The tokens of the row's lists that lie in [t0, end).
+// The tokens of the row's lists that lie in [t0, end). Bound by latency (the list, its atomics in LDS,
+// the mask's word and the logit, one after the other), with long lists by LDS atomics on the
+// same word where a few tokens make up much of a list: 512 rows with up to 2,000 ids 37 us, 9 rows
+// with up to 60,000, of which one token is 7 %, 14 us, one row with 700 ids in place 7 us.
 template <typename T, typename O>
 __device__ __forceinline__ void single(const ge_rule_args& x, int64_t row, int t0, int end, SingleLds& lds) {
     const Lists lists(x, row);
@@ -391,7 +399,7 @@ __device__ __forceinline__ void single(const ge_rule_args& x, int64_t row, int t
 }
 
 // A piece of kDirect tokens of a row that is capped in place: its words are counted first, then
-// every token passes.
+// every token passes. The logits' loads are in flight while the lists are counted.
 template <typename T>
 __device__ __forceinline__ void merged(const ge_rule_args& x, int64_t row, int t0, SingleLds& lds) {
     constexpr int kUnits = kDirect / (kSingleThreads * kUnit);
@@ -428,7 +436,9 @@ __device__ __forceinline__ void merged(const ge_rule_args& x, int64_t row, int t
     }
 }
 
-// What is not allowed of `units` units a thread from t0 on.
+// What is not allowed of kUnits units a thread from t0 on: reads the mask, and writes what it leaves out.
+// 64 rows of 262,144 tokens with grammars that allow few of them, and histories of 300 ids
+// beside: 15.6 us, 6 of which are the bytes; the rest is the lists' latency.
 template <typename T, int kUnits>
 __device__ __forceinline__ void forbid(const ge_rule_args& x, int64_t row, int t0) {
     T* const out = static_cast<T*>(x.out) + row * x.out_stride;
