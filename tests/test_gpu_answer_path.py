@@ -107,3 +107,25 @@ def test_decode_loop():
             history[r].append(got)
             assert int(ring[r, (n + 1) % CAPACITY]) == got
     assert compared > STEPS * ROWS // 2
+
+
+@pytest.mark.parametrize("cfg", (dict(temperature=0.0), dict(temperature=0.8, top_k=40), dict(temperature=0.8, top_k=0, top_p=1.0)))
+def test_a_row_that_may_answer_nothing_is_done(cfg):
+    """The rules' flags as the sampler's done state: the sampler leaves those rows alone."""
+    from gemmaedge_amd import rules as R
+    from gemmaedge_amd import sampler as S
+
+    rows, vocab = 3, 5003
+    logits = torch.randn(rows, vocab, device="cuda")
+    mask = torch.zeros(rows, -(-vocab // 32), dtype=torch.int32, device="cuda")
+    mask[0, 3], mask[2, 100] = 1 << 7, 0b11
+    done, flags = torch.zeros(2, rows, dtype=torch.int32, device="cuda")
+    ring, lens = torch.zeros(rows, 4, dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    R.apply(logits, out=logits, mask=mask, flags=flags)
+    done |= flags
+    sampler = S.Sampler(rows, vocab, 4)
+    tokens, _, got = sampler.sample(logits, S.SamplingConfig(**cfg), torch.tensor([0.5, 0.5, 0.25], device="cuda"), ring=ring, ring_len=lens, done=done)
+    torch.cuda.synchronize()
+    assert done.tolist() == [0, 1, 0] and lens.tolist() == [1, 0, 1]
+    assert int(tokens[0]) == 103 and int(tokens[1]) == -1 and int(tokens[2]) in (3200, 3201)
+    assert int(got[1]) & S.GE_FLAG_DONE
