@@ -235,8 +235,10 @@ __device__ __forceinline__ void product(f32x4& c, bf16x8 a, bf16x8 b) {
 // it gets acc[mt][nt], whose element j is row epi_row(mt, 4 * (lane / 16) + j)
 // (A along k) or mt * 16 + 4 * (lane / 16) + j (across k) of the wave's rows and
 // column nt * 16 + lane % 16 of its columns. `prepare` loads what it needs of them.
+// Tiles of 128 x 64 are bound by the loads of three workgroups on a compute unit, which the
+// registers have to leave room for (projection, 64 rows with adapters: 345 us, with two 390).
 template <int kBm, int kBn, int kWavesM, int kWavesN, bool kAAlong, bool kBAlong, typename Epi>
-__global__ __launch_bounds__(64 * kWavesM * kWavesN) void gemm_kernel(GemmArgs g, Epi epi) {
+__global__ __launch_bounds__(64 * kWavesM * kWavesN, kBm == 128 && kBn == 64 ? 3 : 1) void gemm_kernel(GemmArgs g, Epi epi) {
     constexpr int kWaves = kWavesM * kWavesN;
     constexpr int kWm = kBm / kWavesM, kWn = kBn / kWavesN;
     constexpr int kMt = kWm / 16, kNt = kWn / 16;

@@ -17,7 +17,7 @@
 // TB/s), with many the matrix cores (4,096 rows, width 2,816, 262,144 outputs, 9 adapters of rank 32:
 // 5.3 ms, 1,150 TFLOP/s; 4.8 of them without adapters). Adapters inside it save the outputs' second
 // pass; what they cost is their rows' bytes and the epilogue's time, in which nothing is loaded
-// for the next tile: 8,192 rows, 2,816 to 11,264, 5 adapters of rank 64, 544 us, 436 without.
+// for the next tile: 8,192 rows, 2,816 to 11,264, 5 adapters of rank 64, 549 us, 436 without.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -60,11 +60,13 @@ struct Buffers {
 // ---- low-rank values ------------------------------------------------------------
 //
 // The rows' u and du, `pad` (rank_pad) values each, zeros behind the rank: float32
-// rows, or bf16 in two planes, the value rounded and what that left.
+// rows, or bf16 in three planes, of which each has the next 8 bits, cut off: together
+// the float32 value itself, for magnitudes from 2^-102 on. Two planes would leave 2^-17
+// of it out, which float32 outputs show, and which turns one rounding to bf16 in some hundreds.
 template <typename T>
 struct Low {
     T* p;
-    int64_t plane;  // elements from the first plane to the second (bf16)
+    int64_t plane;  // elements from a plane to the next (bf16)
     int pad;
 };
 template <typename T>
@@ -73,16 +75,13 @@ __device__ __forceinline__ void low_store(const Low<T>& u, int64_t row, int r, f
     if constexpr (sizeof(T) == 4) {
         *to = x;
     } else {
-        const uint16_t hi = to_bf16(x);
-        to[0] = hi;
-        to[u.plane] = to_bf16(x - to_f32(hi));
-    }
-}
-
-__device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
+        for (int p = 0; p < kLowPlanes; ++p) {
+            const uint32_t top = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
+            to[p * u.plane] = static_cast<uint16_t>(top >> 16);
+            x -= __builtin_bit_cast(float, top);
+        }
+    }
 }
 
 // At most 2^31 - 16 bytes from p on, `left` of which are the operand's.
@@ -179,18 +178,20 @@ __device__ __forceinline__ void load_table(const Adapters<T>& x, int64_t m0, int
     for (int t = 0; t < kMt; ++t) f[t] = __builtin_bit_cast(Frag<T>, v[t]);
 }
 
-// The row's own values for the same ranks, zeros without an adapter; bf16: both planes.
+// The row's own values for the same ranks, zeros without an adapter; bf16: all planes.
+template <typename T>
 struct RowValues {
-    u32x4 v[2];
+    static constexpr int kPlanes = sizeof(T) == 2 ? kLowPlanes : 1;
+    u32x4 v[kPlanes];
 };
 template <typename T>
-__device__ __forceinline__ RowValues load_values(const Adapters<T>& x, int id, int64_t n, int r0, int lane) {
-    RowValues u;
-    u.v[0] = u.v[1] = u32x4{0, 0, 0, 0};
-    if (id >= 0) {
-        const T* const p = x.u.p + n * x.u.pad + r0 + (kChunk<T> / 4) * (lane >> 4);
-        u.v[0] = *reinterpret_cast<const u32x4*>(p);
-        if constexpr (sizeof(T) == 2) u.v[1] = *reinterpret_cast<const u32x4*>(p + x.u.plane);
+__device__ __forceinline__ RowValues<T> load_values(const Adapters<T>& x, int id, int64_t n, int r0, int lane) {
+    RowValues<T> u;
+    const T* const p = x.u.p + n * x.u.pad + r0 + (kChunk<T> / 4) * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < RowValues<T>::kPlanes; ++i) {
+        u.v[i] = u32x4{0, 0, 0, 0};
+        if (id >= 0) u.v[i] = *reinterpret_cast<const u32x4*>(p + i * x.u.plane);
     }
     return u;
 }
@@ -198,11 +199,11 @@ __device__ __forceinline__ RowValues load_values(const Adapters<T>& x, int id, i
 // acc += table u for the lanes whose row is this adapter's. Products with the rows that are not its
 // own are left out, not added as zeros: an infinity in one request's adapter stays there.
 template <typename T>
-__device__ __forceinline__ void add_product(const Frag<T>& f, const RowValues& u, bool mine, f32x4& acc) {
+__device__ __forceinline__ void add_product(const Frag<T>& f, const RowValues<T>& u, bool mine, f32x4& acc) {
     f32x4 y{0.f, 0.f, 0.f, 0.f};
     if constexpr (sizeof(T) == 2) {
-        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, u.v[1]), y, 0, 0, 0);
-        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, u.v[0]), y, 0, 0, 0);
+#pragma unroll
+        for (int p = kLowPlanes - 1; p >= 0; --p) y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, u.v[p]), y, 0, 0, 0);
     } else {
         const f32x4 fu = __builtin_bit_cast(f32x4, u.v[0]);
 #pragma unroll
@@ -223,7 +224,7 @@ template <bool kAAlong, typename T, int kMt, int kNt>
 __device__ __forceinline__ void add_adapters(const Adapters<T>& x, const int (&id)[kNt], int64_t m0, int64_t n0, int lane, f32x4 (&acc)[kMt][kNt]) {
     if (!x.adapters) return;
     for (int r0 = 0; r0 < x.rank; r0 += kChunk<T>) {
-        RowValues u[kNt];
+        RowValues<T> u[kNt];
         uint64_t left[kNt];
 #pragma unroll
         for (int j = 0; j < kNt; ++j) {
@@ -262,14 +263,14 @@ struct AdapterSum {
     const int (&id)[kNt];
     int64_t m0, n0;
     int lane;
-    RowValues next[kKept];
+    RowValues<T> next[kKept];
     Frag<T> f[kKept][kMt];
     int kept = -1;
     __device__ __forceinline__ AdapterSum(const Adapters<T>& a, const int (&ids)[kNt], int64_t m, int64_t n, int l)
         : x(a), id(ids), m0(m), n0(n), lane(l) {
         if (x.adapters) values(0, 0, next);
     }
-    __device__ __forceinline__ void values(int j, int r0, RowValues (&u)[kKept]) const {
+    __device__ __forceinline__ void values(int j, int r0, RowValues<T> (&u)[kKept]) const {
 #pragma unroll
         for (int c = 0; c < kKept; ++c)
             if (r0 + c * kChunk<T> < x.rank) u[c] = load_values(x, id[j], n0 + j * 16, r0 + c * kChunk<T>, lane);
@@ -277,7 +278,7 @@ struct AdapterSum {
     __device__ __forceinline__ void add(int j, f32x4 (&acc)[kMt]) {
         constexpr int kStep = kKept * kChunk<T>;
         if (!x.adapters) return;
-        RowValues u[kKept];
+        RowValues<T> u[kKept];
 #pragma unroll
         for (int c = 0; c < kKept; ++c) u[c] = next[c];
         if (j + 1 < kNt) values(j + 1, 0, next);
@@ -850,9 +851,10 @@ __global__ __launch_bounds__(1024) void order_kernel(const int32_t* ids, int row
 // their way to the registers. A wave takes 64 columns; the matrix instructions' M side,
 // of which a lane has 4 neighbours, is the side that lies together in memory. An adapter's
 // rows are divided where the columns do not fill the card, and the parts joined in order.
-// 8,192 rows, 5 adapters of rank 64: dB, of 11,264 columns, 69 us (185 MB read, 2.7 TB/s) and 10 for
-// the join, dA, of 2,816, 34 and 9: bound by the steps' latency, with 440 and 330 workgroups of
-// 72 KiB of LDS, two to a compute unit.
+// 8,192 rows, 5 adapters of rank 64: dB, of 11,264 columns, 81 us (185 MB of dout, 2.3 TB/s) and 9 for
+// the join, dA, of 2,816, 36 and 9: bound by the steps' latency, with 440 and 330 workgroups, two
+// to a compute unit. Steps of 64 rows: the same with one buffer for y and two barriers a
+// step, 20 us more with two buffers, whose 92 KiB of LDS leave room for one workgroup.
 template <typename T>
 struct OuterArgs {
     const T* x;
@@ -868,7 +870,7 @@ struct OuterArgs {
 };
 
 constexpr int kOuterCols = 64;  // of a wave
-constexpr int kOuterRows = 64;  // of a step (bf16)
+constexpr int kOuterRows = 32;  // of a step (bf16)
 
 template <typename T, bool kRanksLast, int kR>
 __global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
@@ -891,9 +893,9 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
         // A wave's columns are its own, the ranks the workgroup's, in two buffers in turn. The next
         // step's loads are in flight while this one is multiplied, and the rows' numbers a step ahead of them.
         constexpr int kXRow = kOuterCols + 8, kYRow = kRanks + 8;
-        constexpr int kX = kOuterRows / 8, kYUnits = 2 * kOuterRows * kRanks / 8, kY = (kYUnits + 255) / 256;
+        constexpr int kX = kOuterRows / 8, kYUnits = kLowPlanes * kOuterRows * kRanks / 8, kY = (kYUnits + 255) / 256;
         __shared__ __align__(16) uint16_t xs[4][kOuterRows * kXRow];
-        __shared__ __align__(16) uint16_t ys[2][2 * kOuterRows * kYRow];
+        __shared__ __align__(16) uint16_t ys[2][kLowPlanes * kOuterRows * kYRow];
         u32x4 x[kX], y[kY];
         int xn[kX], yn[kY];
         const int c = c0 + (lane & 7) * 8;
@@ -942,16 +944,16 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterArgs<T> s) {
             }
 #pragma unroll
             for (int h = 0; h < kOuterRows / 32; ++h) {
-                bf16x8 fy[2][kR];
+                bf16x8 fy[kLowPlanes][kR];
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
+                for (int p = 0; p < kLowPlanes; ++p)
 #pragma unroll
                     for (int r = 0; r < kR; ++r) fy[p][r] = frag_across(yt + (p * kOuterRows + h * 32) * kYRow, kYRow, r * 16, lane);
 #pragma unroll
                 for (int t = 0; t < kC; ++t) {
                     const bf16x8 fx = frag_across(xt + h * 32 * kXRow, kXRow, t * 16, lane);
 #pragma unroll
-                    for (int p = 1; p >= 0; --p)
+                    for (int p = kLowPlanes - 1; p >= 0; --p)
 #pragma unroll
                         for (int r = 0; r < kR; ++r)
                             acc[t][r] = kRanksLast ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fy[p][r], fx, acc[t][r], 0, 0, 0)

@@ -22,6 +22,7 @@ using head::kUnits;
 using head::round_up;
 using head::stride_ok;
 
+constexpr int kLowPlanes = 3;       // bf16 numbers that hold a low-rank value of bf16 operands
 constexpr int kRowTile = 16;        // rows of a workgroup of the low-rank sums,
 constexpr int kWideRows = 64;       // and of their form for many bf16 rows,
 constexpr int kFewRows = 128;       // which more rows than this take
@@ -52,7 +53,7 @@ inline void size_workspace(Capacity& c) {
     c.hpack = es * rows * dim;
     c.wpack = es * dim * std::min(out, std::max<int64_t>(kTileM, ((64LL << 20) / (2 * dim)) / kTileM * kTileM));
     const int64_t upad = rank_pad(c.max_rank);
-    c.u = c.max_adapters ? 4 * rows * upad : 0;
+    c.u = c.max_adapters ? (c.dtype == GE_DTYPE_F32 ? 4 : 2 * kLowPlanes) * rows * upad : 0;
     // no call has more parts than fill the card, or than this many
     c.parts = c.max_adapters ? 4 * upad * std::min(kMaxLowSplits * rows, kWideRows * std::max<int64_t>(kLowBlocks, (rows + kRowTile - 1) / kRowTile)) : 0;
     c.du = c.order = c.at = c.dpack = c.dhidden = 0;

@@ -48,9 +48,9 @@ void ge_projection_destroy(ge_projection* projection);
  *   dA_k = sum over its rows of du[n] hidden[n]^T,  dB_k = sum of dout[n] u[n]^T,
  * zeros for adapters without rows. da and db are written, not added to.
  *
- * Sums are float32. bf16 operands: u and du are held in two bf16 numbers each, 16
- * bits of mantissa; float32 operands: products with the weight in three bf16
- * planes each (24 bits of magnitudes from 2^-110 to 3.38e38), those of the
+ * Sums are float32, and u and du are held in float32's 24 bits (bf16 operands: of
+ * magnitudes from 2^-102 on). float32 operands: products with the weight in three
+ * bf16 planes each (24 bits of magnitudes from 2^-110 to 3.38e38), those of the
  * adapters in float32. Adapters of a smaller rank are padded with zeros. */
 typedef struct ge_project_args {
     const void* hidden;       /* [rows][dim], hidden_stride elements apart */
