@@ -63,6 +63,11 @@ struct Buffers {
 // rows, or bf16 in three planes, of which each has the next 8 bits, cut off: together
 // the float32 value itself, for magnitudes from 2^-102 on. Two planes would leave 2^-17
 // of it out, which float32 outputs show, and which turns one rounding to bf16 in some hundreds.
+//
+// The planes of a value have its sign and none is zero unless it is, so that times an
+// infinity they are one infinity: a plane of which nothing is left shares the one before. (The
+// smallest normal number there instead would show: the matrix instructions cut sums off downwards.)
+// All planes of an infinity are that infinity, since what it leaves would be NaN.
 template <typename T>
 struct Low {
     T* p;
@@ -75,12 +80,19 @@ __device__ __forceinline__ void low_store(const Low<T>& u, int64_t row, int r, f
     if constexpr (sizeof(T) == 4) {
         *to = x;
     } else {
-#pragma unroll
-        for (int p = 0; p < kLowPlanes; ++p) {
-            const uint32_t top = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-            to[p * u.plane] = static_cast<uint16_t>(top >> 16);
-            x -= __builtin_bit_cast(float, top);
+        static_assert(kLowPlanes == 3);
+        auto top = [](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u); };
+        float hi = top(x), mid = top(x - hi), lo = x - hi - mid;
+        if (mid == 0.f) {
+            hi = x * 0.5f;
+            mid = lo = x * 0.25f;
+        } else if (lo == 0.f) {
+            mid = lo = mid * 0.5f;
         }
+        if (!(__builtin_fabsf(x) < __builtin_inff())) hi = mid = lo = x;
+        to[0] = to_bf16(hi);
+        to[u.plane] = to_bf16(mid);
+        to[2 * u.plane] = to_bf16(lo);
     }
 }
 
@@ -508,11 +520,11 @@ __device__ __forceinline__ int row_adapter(const SumArgs<T>& s, int n) {
 // A row's sum with rank r: into its part, or as the value itself. `who`: the row's adapter.
 template <typename T>
 __device__ __forceinline__ void low_result(const SumArgs<T>& s, int split, int64_t n, int r, float x, int who) {
-    if (who < 0 || r >= s.rank) x = 0.f;
+    const bool there = who >= 0 && r < s.rank;
     if (s.parts)
-        s.parts[(static_cast<int64_t>(split) * s.rows + n) * s.y.pad + r] = x;
+        s.parts[(static_cast<int64_t>(split) * s.rows + n) * s.y.pad + r] = there ? x : 0.f;
     else
-        low_store(s.y, n, r, who >= 0 ? x * s.scale[who] : 0.f);
+        low_store(s.y, n, r, there ? x * s.scale[who] : 0.f);  // zeros behind the rank whatever the scale is
 }
 
 // The first `left` of 8 elements at p (any address), zeros behind them.
@@ -803,7 +815,7 @@ __global__ __launch_bounds__(256) void low_join_kernel(SumArgs<T> s) {
         for (int i = 0; i < s.splits; ++i) x += s.parts[i * all + at];
     }
     const int id = row_adapter(s, static_cast<int>(n));
-    low_store(s.y, n, r, id >= 0 ? x * s.scale[id] : 0.f);
+    low_store(s.y, n, r, id >= 0 && r < s.rank ? x * s.scale[id] : 0.f);
 }
 
 // ---- an adapter's rows -------------------------------------------------------------

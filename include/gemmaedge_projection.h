@@ -51,7 +51,10 @@ void ge_projection_destroy(ge_projection* projection);
  * Sums are float32, and u and du are held in float32's 24 bits (bf16 operands: of
  * magnitudes from 2^-102 on). float32 operands: products with the weight in three
  * bf16 planes each (24 bits of magnitudes from 2^-110 to 3.38e38), those of the
- * adapters in float32. Adapters of a smaller rank are padded with zeros. */
+ * adapters in float32. Adapters of a smaller rank are padded with zeros.
+ *
+ * Infinities and NaN go where the formulas take them, and only there; in float32
+ * an infinity in hidden, weight or dout gives NaN in what the product with the weight makes of it. */
 typedef struct ge_project_args {
     const void* hidden;       /* [rows][dim], hidden_stride elements apart */
     int64_t hidden_stride;

@@ -116,3 +116,62 @@ def test_du(rows, dim, out, rank, adapters, dt):
     dh, da, _ = p.project_backward(dout, hidden, weight, a, b.transpose(1, 2).contiguous().to(d), scale, ids)
     assert torch.equal(dh, (du[:, at % rank] * torch.where(at % 3 == 0, -2.0, 0.5)).to(torch.float32).to(d))
     assert torch.equal(da, want.to(torch.float32).to(d))
+
+
+def whole(g, *shape):
+    """Whole numbers of 1 to 3 and their negatives: every sum of their products is exact."""
+    return torch.randint(1, 4, shape, generator=g) * (1 - 2 * torch.randint(2, shape, generator=g))
+
+
+def definition(s, dout):
+    """The formulas, a product and a sum at a time, in float64 on the CPU."""
+    h, w, g = s["hidden"].double(), s["weight"].double(), dout.double()
+    def mm(x, y):  # noqa: E306
+        return (x[:, :, None] * y[None]).sum(1)
+    out, dh = mm(h, w.t()), mm(g, w)
+    da, db = torch.zeros_like(s["a"], dtype=torch.float64), torch.zeros_like(s["b"], dtype=torch.float64)
+    for k in range(len(s["scale"])):
+        at = torch.nonzero(s["adapter"] == k)[:, 0]
+        a, b, c = s["a"][k].double(), s["b"][k].double(), s["scale"][k].double()
+        u, du = c * mm(h[at], a.t()), c * mm(g[at], b)
+        out[at] += mm(u, b.t())
+        dh[at] += mm(du, a)
+        da[k], db[k] = mm(du.t(), h[at]), mm(g[at].t(), u)
+    return dict(out=out, dh=dh, da=da, db=db)
+
+
+@pytest.mark.parametrize("where", ("a", "b", "hidden", "dout", "scale"))
+@pytest.mark.parametrize("dt", ("bf16", "f32"))
+@pytest.mark.parametrize("rows,dim,out,rank", [(4, 24, 33, 1), (40, 17, 130, 3), (130, 40, 70, 1), (300, 30, 65, 20)])
+def test_an_infinity_gives_what_the_definition_gives(rows, dim, out, rank, dt, where):
+    """One infinity in an operand: infinities and NaN of the definition, where it has them, and its numbers elsewhere."""
+    from gemmaedge_amd import projection as P
+
+    d = DT[dt]
+    g = torch.Generator().manual_seed(rows + rank)
+    s = dict(hidden=whole(g, rows, dim), weight=whole(g, out, dim), a=whole(g, 3, rank, dim), b=whole(g, 3, out, rank))
+    s = {k: v.to(d) for k, v in s.items()}
+    s["scale"], s["adapter"] = torch.tensor([1.0, 2.0, 0.5]), (torch.arange(rows) % 4).int()
+    dout = whole(g, rows, out).to(d)
+    t = dout if where == "dout" else s[where]
+    if where == "scale":
+        t[1] = -float("inf")
+    elif t.dim() == 2:
+        t[1, 5] = -float("inf")
+    else:
+        t[1, t.shape[1] // 2, t.shape[2] // 3] = float("inf")
+    want = definition(s, dout)
+    p = P.Projection(rows, dim, out, rank, 3, dtype=d, train=True)
+    on = {k: v.cuda() for k, v in s.items()}
+    got = dict(out=p.project(**on, out_dtype=torch.float32))
+    got["dh"], got["da"], got["db"] = (x for x in p.project_backward(dout.cuda(), **on))
+    for k, x in got.items():
+        x, y = x.cpu(), want[k].to(torch.float32).to(x.dtype)
+        if dt == "f32" and (where, k) in (("hidden", "out"), ("dout", "dh")):  # through the weight's product: NaN
+            assert not torch.isfinite(x[1]).any(), k
+            x, y = x.clone(), y.clone()
+            x[1] = y[1] = 0
+        assert torch.equal(torch.isnan(x), torch.isnan(y)), k
+        assert torch.equal(torch.nan_to_num(x, nan=0.0, posinf=float("inf"), neginf=-float("inf")),
+                           torch.nan_to_num(y, nan=0.0, posinf=float("inf"), neginf=-float("inf"))), k
+    assert not all(torch.isfinite(v).all() for v in want.values())
