@@ -171,7 +171,7 @@ inline int check_project(const Capacity& c, const ge_project_args& x, bool backw
     int64_t piece = std::min(out_pad, head::kMostTiles / row_tiles * plan.tile_m / kTileM * kTileM);
     if (plan.pack_w) piece = std::min(piece, c.wpack / (static_cast<int64_t>(es) * plan.kpad) / kTileM * kTileM);
     if (plan.pack_d)  // a handle for millions of rows has room for longer rows than a tile's offsets reach
-        piece = std::min(std::min<int64_t>(piece, head::kMaxStride), c.dpack / (static_cast<int64_t>(es) * x.rows) / kTileM * kTileM);
+        piece = std::min(std::min<int64_t>(piece, head::kMaxStride), c.dpack / (static_cast<int64_t>(es) * std::max(x.rows, 1)) / kTileM * kTileM);
     plan.piece = static_cast<int>(piece);
     plan.splits = 1;
     plan.parts = c.parts;

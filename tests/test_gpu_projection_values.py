@@ -175,3 +175,19 @@ def test_an_infinity_gives_what_the_definition_gives(rows, dim, out, rank, dt, w
         assert torch.equal(torch.nan_to_num(x, nan=0.0, posinf=float("inf"), neginf=-float("inf")),
                            torch.nan_to_num(y, nan=0.0, posinf=float("inf"), neginf=-float("inf"))), k
     assert not all(torch.isfinite(v).all() for v in want.values())
+
+
+@pytest.mark.parametrize("dt", ("bf16", "f32"))
+@pytest.mark.parametrize("out", (1, 1001, 1008))
+def test_no_rows(out, dt):
+    from gemmaedge_amd import projection as P
+
+    d = DT[dt]
+    p = P.Projection(3, 65, 1008, 5, 2, dtype=d, train=True)
+    s = dict(hidden=torch.empty(0, 65), weight=torch.randn(out, 65), a=torch.randn(2, 5, 65), b=torch.randn(2, out, 5))
+    s = {k: v.to(d).cuda() for k, v in s.items()}
+    s.update(scale=torch.ones(2, device="cuda"), adapter=torch.empty(0, dtype=torch.int32, device="cuda"))
+    assert p.project(**s).shape == (0, out)
+    dh, da, db = p.project_backward(torch.empty(0, out, dtype=d, device="cuda"), **s, da=torch.ones_like(s["a"]), db=torch.ones_like(s["b"]))
+    assert dh.shape == (0, 65) and not da.any() and not db.any()
+    assert p.project_backward(torch.empty(0, out, dtype=d, device="cuda"), s["hidden"], s["weight"])[0].shape == (0, 65)
