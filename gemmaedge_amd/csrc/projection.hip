@@ -1338,6 +1338,7 @@ static int project_call(ge_projection* h, void* stream, const ge_project_args* a
     if (!h || !args) return ge::report(GE_ERR_INVALID_ARG, "projection or args is NULL");
     Plan plan{};
     if (const int rc = check_project(h->cap, *args, backward, plan, msg, sizeof(msg))) return ge::report(rc, msg);
+    if (const int rc = check_memory(h->cap, *args, backward, msg, sizeof(msg))) return ge::report(rc, msg);
     OnDevice guard(h->device);
     if (!guard.ok) return ge::report(GE_ERR_DEVICE, "hipSetDevice failed");
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -194,5 +194,61 @@ inline int check_project(const Capacity& c, const ge_project_args& x, bool backw
     return GE_OK;
 }
 
+// Rows of `width` bytes in memory, `stride` >= width bytes apart. 128 bits: strides and rows that
+// check_project takes multiply to more than 63.
+struct Memory {
+    const char* what;
+    __int128 at, stride, width;
+    int64_t rows;
+};
+
+// Whether two share a byte. Columns of one buffer share none, though their ranges do.
+inline bool share(const Memory& a, const Memory& b) {
+    if (a.rows > b.rows) return share(b, a);
+    if (a.rows < 1 || a.width < 1 || b.width < 1) return false;
+    if (a.at >= b.at + (b.rows - 1) * b.stride + b.width || b.at >= a.at + (a.rows - 1) * a.stride + a.width) return false;
+    for (int64_t r = 0; r < a.rows; ++r) {
+        const __int128 from = a.at + r * a.stride;
+        // the first of b's rows that ends behind it
+        const __int128 n = from < b.at + b.width ? 0 : (from - b.at - b.width) / b.stride + 1;
+        if (n < b.rows && b.at + n * b.stride < from + a.width) return true;
+    }
+    return false;
+}
+
+// What a call writes lies apart from what it reads and from what else it writes. For a call that
+// check_project has taken.
+inline int check_memory(const Capacity& c, const ge_project_args& x, bool backward, char* msg, size_t n) {
+    const int64_t es = elem_size(c.dtype), k = x.adapters, rank = k ? x.rank : 0;
+    auto memory = [&](const char* what, const void* p, int64_t rows, __int128 width, int64_t stride, int64_t size) {
+        return Memory{what, static_cast<__int128>(reinterpret_cast<uintptr_t>(p)), static_cast<__int128>(stride) * size, width * size, p ? rows : 0};
+    };
+    auto flat = [&](const char* what, const void* p, __int128 count, int64_t size) { return memory(what, p, 1, count, 0, size); };
+    const __int128 a_size = static_cast<__int128>(k) * rank * x.dim, b_size = static_cast<__int128>(k) * rank * x.out_dim;
+    const bool any = x.rows > 0;  // nothing is read without rows
+    const Memory reads[] = {
+        memory("hidden", x.hidden, x.rows, x.dim, x.hidden_stride, es),
+        memory("weight", x.weight, any ? x.out_dim : 0, x.dim, x.weight_stride, es),
+        memory("dout", x.dout, backward ? x.rows : 0, x.out_dim, x.dout_stride, es),
+        flat("a", any ? x.a : nullptr, a_size, es),
+        flat("b", any ? x.b : nullptr, b_size, es),
+        flat("scale", any ? x.scale : nullptr, k, 4),
+        flat("adapter", k ? x.adapter : nullptr, x.rows, 4),
+    };
+    const Memory writes[] = {
+        memory("out", x.out, backward ? 0 : x.rows, x.out_dim, x.out_stride, elem_size(x.out_dtype)),
+        memory("dhidden", x.dhidden, backward ? x.rows : 0, x.dim, x.dhidden_stride, es),
+        flat("da", backward ? x.da : nullptr, a_size, es),
+        flat("db", backward ? x.db : nullptr, b_size, es),
+    };
+    for (const Memory& w : writes) {
+        for (const Memory& r : reads)
+            if (share(w, r)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "%s overlaps %s", w.what, r.what);
+        for (const Memory& v : writes)
+            if (&v < &w && share(w, v)) return plan_fail(msg, n, GE_ERR_INVALID_ARG, "%s overlaps %s", w.what, v.what);
+    }
+    return GE_OK;
+}
+
 }  // namespace projection
 }  // namespace ge

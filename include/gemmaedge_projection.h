@@ -80,7 +80,8 @@ typedef struct ge_project_args {
     void* db;                 /* backward: as b; NULL: not wanted */
 } ge_project_args;
 
-/* Outputs may not overlap inputs or each other; `out` is not read by the backward call. */
+/* Outputs may not overlap inputs or each other (refused; columns of one buffer do not overlap);
+ * `out` is not read by the backward call. */
 int ge_project(ge_projection* projection, void* stream, const ge_project_args* args);
 int ge_project_backward(ge_projection* projection, void* stream, const ge_project_args* args);
 

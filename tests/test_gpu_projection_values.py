@@ -191,3 +191,36 @@ def test_no_rows(out, dt):
     dh, da, db = p.project_backward(torch.empty(0, out, dtype=d, device="cuda"), **s, da=torch.ones_like(s["a"]), db=torch.ones_like(s["b"]))
     assert dh.shape == (0, 65) and not da.any() and not db.any()
     assert p.project_backward(torch.empty(0, out, dtype=d, device="cuda"), s["hidden"], s["weight"])[0].shape == (0, 65)
+
+
+def test_outputs_apart_from_all_else():
+    """An output over an operand is refused and leaves everything as it was; columns of one buffer are apart."""
+    from gemmaedge_amd import projection as P
+    from gemmaedge_amd import sampler as S
+
+    g = torch.Generator().manual_seed(2)
+    s = dict(hidden=whole(g, 40, 64), weight=whole(g, 64, 64), a=whole(g, 3, 4, 64), b=whole(g, 3, 64, 4))
+    s = {k: v.bfloat16().cuda() for k, v in s.items()}
+    s.update(scale=torch.ones(3, device="cuda"), adapter=(torch.arange(40, device="cuda") % 4).int())
+    dout = whole(g, 40, 64).bfloat16().cuda()
+    p = P.Projection(40, 64, 64, 4, 3, train=True)
+    before = {k: v.clone() for k, v in s.items()}
+    for out in (s["hidden"], s["weight"][24:], s["a"].view(-1)[:512].view(8, 64)):
+        n = out.shape[0]
+        with pytest.raises(S.SamplerError, match="overlaps"):
+            p.project(s["hidden"][:n], s["weight"], s["a"], s["b"], s["scale"], s["adapter"][:n], out=out)
+    for kw in (dict(dhidden=s["hidden"]), dict(dhidden=dout), dict(da=s["a"]), dict(db=s["b"]), dict(da=s["weight"].view(-1)[:768].view(3, 4, 64))):
+        with pytest.raises(S.SamplerError, match="overlaps"):
+            p.project_backward(dout, **s, **kw)
+    both = torch.empty(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(S.SamplerError, match="overlaps"):
+        p.project_backward(dout, **s, da=both, db=both.view(3, 64, 4))
+    torch.cuda.synchronize()
+    assert all(torch.equal(s[k], before[k]) for k in s)
+    wide = torch.zeros(40, 192, device="cuda", dtype=torch.bfloat16)
+    wide[:, :64] = s["hidden"]
+    wide[:, 128:] = dout
+    want, got = p.project(**s), p.project(**dict(s, hidden=wide[:, :64]), out=wide[:, 64:128])
+    assert torch.equal(got, want)
+    dh = p.project_backward(wide[:, 128:], **dict(s, hidden=wide[:, :64]), dhidden=wide[:, 64:128])[0]
+    assert torch.equal(dh, p.project_backward(dout, **s)[0])
