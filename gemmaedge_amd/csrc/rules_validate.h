@@ -20,8 +20,8 @@ inline int size_of(int dtype) { return dtype == GE_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == GE_DTYPE_F32 || dtype == GE_DTYPE_BF16; }
 inline bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Bytes from the first to behind the last element of `rows` rows.
-inline int64_t span(int rows, int vocab, int64_t stride, int size) { return ((rows - 1) * stride + vocab) * size; }
+// Bytes from the first to behind the last element of `rows` rows: up to 2^24 rows 2^40 elements apart, more than 63 bits hold.
+inline __int128 span(int rows, int vocab, int64_t stride, int size) { return (static_cast<__int128>(rows - 1) * stride + vocab) * size; }
 
 inline bool in_place(const ge_rule_args& x) { return x.out == x.logits; }
 
@@ -72,9 +72,8 @@ inline int check_rules(const ge_rule_args& x, char* msg, size_t n) {
         if (x.dtype != x.out_dtype || (x.rows > 1 && x.row_stride != x.out_stride))
             return plan_fail(msg, n, GE_ERR_INVALID_ARG, "in place with another dtype or stride");
     } else {
-        const uintptr_t a = reinterpret_cast<uintptr_t>(x.logits), b = reinterpret_cast<uintptr_t>(x.out);
-        if (a < b + static_cast<uintptr_t>(span(x.rows, x.vocab, x.out_stride, size_of(x.out_dtype))) &&
-            b < a + static_cast<uintptr_t>(span(x.rows, x.vocab, x.row_stride, size_of(x.dtype))))
+        const __int128 a = reinterpret_cast<uintptr_t>(x.logits), b = reinterpret_cast<uintptr_t>(x.out);
+        if (a < b + span(x.rows, x.vocab, x.out_stride, size_of(x.out_dtype)) && b < a + span(x.rows, x.vocab, x.row_stride, size_of(x.dtype)))
             return plan_fail(msg, n, GE_ERR_INVALID_ARG, "out overlaps the logits");
     }
     return GE_OK;
