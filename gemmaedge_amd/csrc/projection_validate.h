@@ -207,6 +207,12 @@ inline bool share(const Memory& a, const Memory& b) {
     if (a.rows > b.rows) return share(b, a);
     if (a.rows < 1 || a.width < 1 || b.width < 1) return false;
     if (a.at >= b.at + (b.rows - 1) * b.stride + b.width || b.at >= a.at + (a.rows - 1) * a.stride + a.width) return false;
+    if (a.rows > 1 && a.stride == b.stride) {
+        // b begins `first` rows and `right` bytes behind a: its row j lies beside a's rows first + j and, on the right, first + j + 1
+        const __int128 off = b.at - a.at, first = off >= 0 ? off / a.stride : -((a.stride - 1 - off) / a.stride), right = off - first * a.stride;
+        auto meet = [&](__int128 by) { return by > -b.rows && by < a.rows; };
+        return (right < a.width && meet(first)) || (right + b.width > a.stride && meet(first + 1));
+    }
     for (int64_t r = 0; r < a.rows; ++r) {
         const __int128 from = a.at + r * a.stride;
         // the first of b's rows that ends behind it

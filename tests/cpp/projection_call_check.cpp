@@ -2,6 +2,7 @@
 // address and undefined-behaviour sanitizers, at the sizes where a plan can go wrong.
 #include <cstdio>
 #include <cstdlib>
+#include <ctime>
 #include <random>
 
 #include "../../gemmaedge_amd/csrc/projection_validate.h"
@@ -80,6 +81,11 @@ static void shared_bytes() {
             }
         CHECK(share(m[0], m[1]) == want && share(m[1], m[0]) == want);
     }
+    // columns of one buffer with many rows, as quickly as others
+    const Memory left{"", 4096, 256, 128, 1 << 22}, right{"", 4096 + 128, 256, 128, 1 << 22};
+    const clock_t began = clock();
+    for (int i = 0; i < 1000; ++i) CHECK(!share(left, right) && !share(right, left));
+    CHECK(clock() - began < CLOCKS_PER_SEC);
     // the largest that check_project takes
     const Memory far{"", 1, __int128{4} << 40, 1 << 18, 1 << 24}, one{"", (__int128{4} << 63) + 1, 4, 4, 1};
     CHECK(share(far, one) && share(one, far));
