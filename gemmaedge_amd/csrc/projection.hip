@@ -17,7 +17,7 @@
 // TB/s), with many the matrix cores (4,096 rows, width 2,816, 262,144 outputs, 9 adapters of rank 32:
 // 5.3 ms, 1,150 TFLOP/s; 4.8 of them without adapters). Adapters inside it save the outputs' second
 // pass; what they cost is their rows' bytes and the epilogue's time, in which nothing is loaded
-// for the next tile: 8,192 rows, 2,816 to 11,264, 5 adapters of rank 64, 549 us, 436 without.
+// for the next tile: 8,192 rows, 2,816 to 11,264, 5 adapters of rank 64, 540 us, 436 without.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -144,8 +144,7 @@ __device__ __forceinline__ void hold(f32x4 (&acc)[kMt][kNt], int j) {
     }
 }
 
-// Ranks of a chunk: of a fragment of an adapter's rows. Tall tiles have no registers for a
-// second one.
+// Ranks of a chunk, which is a fragment of an adapter's rows.
 template <typename T>
 constexpr int kChunk = sizeof(T) == 2 ? 32 : 16;
 
@@ -557,7 +556,7 @@ __device__ __forceinline__ bf16x8 frag_across(uint16_t* tile, int ld, int col, i
 
 // Few rows, or float32: a workgroup has 16 rows, and its waves take every kSumWaves-th step of 32 channels,
 // kBatch of them at a time, whose loads are in flight together. Bound by their latency: 64
-// rows of 2,816 channels with 22 adapters of rank 16: 5 us (18 us a step at a time with four waves).
+// rows of 2,816 channels with 22 adapters of rank 16: 9.5 us (18 us a step at a time with four waves).
 constexpr int kSumStep = 32;
 constexpr int kSumWaves = 8;
 
@@ -863,8 +862,8 @@ __global__ __launch_bounds__(1024) void order_kernel(const int32_t* ids, int row
 // their way to the registers. A wave takes 64 columns; the matrix instructions' M side,
 // of which a lane has 4 neighbours, is the side that lies together in memory. An adapter's
 // rows are divided where the columns do not fill the card, and the parts joined in order.
-// 8,192 rows, 5 adapters of rank 64: dB, of 11,264 columns, 81 us (185 MB of dout, 2.3 TB/s) and 9 for
-// the join, dA, of 2,816, 36 and 9: bound by the steps' latency, with 440 and 330 workgroups, two
+// 8,192 rows, 5 adapters of rank 64: dB, of 11,264 columns, 79 us (185 MB of dout, 2.3 TB/s) and 10 for
+// the join, dA, of 2,816, 34 and 8: bound by the steps' latency, with 440 and 330 workgroups, two
 // to a compute unit. Steps of 64 rows: the same with one buffer for y and two barriers a
 // step, 20 us more with two buffers, whose 92 KiB of LDS leave room for one workgroup.
 template <typename T>
@@ -1037,7 +1036,7 @@ __global__ __launch_bounds__(256) void outer_join_kernel(OuterArgs<T> s) {
     store_out(s.out + at, x, n);
 }
 
-// A of the adapters that have rows, transposed: [adapters][dim][rank], 8 ranks a thread. Latency: 5 to 7 us.
+// A of the adapters that have rows, transposed: [adapters][dim][rank], 8 ranks a thread. Latency: 3 to 6 us.
 template <typename T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T* a, int rank, int dim, const int32_t* begin, T* to) {
     const int k = blockIdx.z;
